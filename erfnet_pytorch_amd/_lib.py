@@ -107,6 +107,10 @@ SIGNATURES = {
     "erf_adam_advance": (I, [P, P, P, D, D, P]),
     "erf_adam_fused_arena_hyper": (I, [P, P, P, P, LL, P, D, D, D, D, D, P]),
     "erf_dropout2d_mask_many_counter": (I, [P, I, P, P, P, P]),
+    "erf_adamw_chunk_elements": (I, []),
+    "erf_adamw_scale_block": (I, []),
+    "erf_adamw_set_grads": (I, [P, P, I, P]),
+    "erf_adamw_step": (I, [P, P, P, I, P, D, D, D, D, I, I, ctypes.c_uint, P]),
     "erf_sgd_fused_arena": (I, [P, P, P, LL, D, D, D, I, D, P]),
     "erf_sgd_fused_arena_hyper": (I, [P, P, P, LL, P, D, I, D, P]),
     "erf_conv1d_dgrad": (I, [P, P, P, P, P, I, I, I, I, I, I, I, P]),
@@ -155,7 +159,7 @@ SIGNATURES = {
     "erf_bn_stats_finalize_static": (I, [P, I, LL, I, P, P, P, P, F, F, P, P, P, P, P]),
 }
 # entry points whose int return value is data, not a status
-_PLAIN_INT = {"erf_version", "erf_output_conv_patch_channels", "erf_pointwise_grad_channels",
+_PLAIN_INT = {"erf_version", "erf_adamw_chunk_elements", "erf_adamw_scale_block", "erf_output_conv_patch_channels", "erf_pointwise_grad_channels",
               "erf_static_scratch_max_channels"}
 
 _fn = {}

@@ -234,6 +234,33 @@ int erf_weighted_ce_fwd(const void* logits, int dtype, const long long* target, 
 int erf_weighted_ce_bwd(const void* logits, int dtype, const long long* target, const float* weight, int N, int C,
                         long long HW, const float* coef, void* dlogits, void* stream);
 
+/* ---- optimiser over many tensors in one launch: AdamW (decoupled weight decay), moments in 32 or 8 bits.
+ * m = b1 m + (1-b1) g; v = b2 v + (1-b2) g^2; p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps).
+ * table: one device record per tensor; `dtype` (one per launch) is the element type of param and grad.
+ *   state_bits 32: exp_avg / exp_avg_sq fp32 [count], the scales unused.
+ *   state_bits 8: exp_avg / exp_avg_sq are e4m3 codes [count] of m and of sqrt(v), to be multiplied with the fp32 power of
+ *   two that each erf_adamw_scale_block() elements share (exp_avg_scale / root_scale, ceil(count / block) each); new codes are
+ *   rounded up or down at random: the bits come from (seed, step, base + element) alone, so a run can be repeated.
+ * chunks: device int pairs (tensor, chunk), every chunk of erf_adamw_chunk_elements() elements of every tensor exactly once;
+ * steps: device int per chunk, the steps taken so far; each launch adds 1.  lr: device double.
+ * Tensors of one launch must not overlap.
+ * erf_adamw_set_grads writes the grad fields of records 0..count-1; grads: HOST array, read before the call returns. */
+typedef struct {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* root_scale;
+    long long count;
+    long long base;
+} erf_adamw_tensor;
+int erf_adamw_chunk_elements(void);
+int erf_adamw_scale_block(void);
+int erf_adamw_set_grads(erf_adamw_tensor* table, const void* const* grads, int count, void* stream);
+int erf_adamw_step(const erf_adamw_tensor* table, const int* chunks, int* steps, int n_chunks, const double* lr, double beta1,
+                   double beta2, double eps, double weight_decay, int dtype, int state_bits, unsigned seed, void* stream);
+
 /* ---- optimiser: torch.optim.Adam(lr, betas, eps, weight_decay) of train/main.py:140 and
  * torch.optim.SGD(lr, momentum, weight_decay) of imagenet/main.py:83-85, over flat fp32 arenas.
  * g = grad * grad_scale + weight_decay * p (coupled L2); step is 1-based.  Hyper-parameters are
