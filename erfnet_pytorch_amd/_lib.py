@@ -107,6 +107,8 @@ SIGNATURES = {
     "erf_adam_advance": (I, [P, P, P, D, D, P]),
     "erf_adam_fused_arena_hyper": (I, [P, P, P, P, LL, P, D, D, D, D, D, P]),
     "erf_dropout2d_mask_many_counter": (I, [P, I, P, P, P, P]),
+    "erf_class_log_probs_fwd": (I, [P, I, LL, I, LL, LL, LL, P, LL, P, P, P, I, P, P, P]),
+    "erf_class_log_probs_bwd": (I, [P, I, LL, I, LL, LL, LL, P, LL, P, P, P, P, I, P, P, P, LL, LL, P]),
     "erf_adamw_chunk_elements": (I, []),
     "erf_adamw_scale_block": (I, []),
     "erf_adamw_set_grads": (I, [P, P, I, P]),

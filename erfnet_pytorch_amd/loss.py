@@ -13,9 +13,11 @@ parameter gradients gives the global-batch gradient.
 """
 from __future__ import annotations
 
+from typing import NamedTuple, Optional
+
 import torch
 
-from . import ops
+from . import ops, train_ops
 from ._lib import call, query
 from .dp import global_weighted_mean
 
@@ -68,3 +70,57 @@ class CrossEntropyLoss2d(torch.nn.Module):
 
     def forward(self, outputs, targets):
         return weighted_cross_entropy(outputs, targets, self.weight, self.group)
+
+
+class ClassLogProbs(NamedTuple):
+    log_prob: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_log_probs: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+class _ClassLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, top_k, ignore_index):
+        log_prob, entropy, stats, top, index = train_ops.class_log_probs_fwd(logits, target, top_k, ignore_index)
+        ctx.save_for_backward(logits, target, stats, entropy, index)
+        ctx.ignore_index = ignore_index
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(index)
+        return log_prob, entropy, top, index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, g_top, _):
+        logits, target, stats, entropy, index = ctx.saved_tensors
+        if target is None:
+            g_log_prob = None
+        if not index.shape[1]:
+            g_top = None
+        if g_log_prob is None and g_entropy is None and g_top is None:
+            return None, None, None, None
+        return train_ops.class_log_probs_bwd(logits, target, stats, entropy, index, g_log_prob, g_entropy, g_top, ctx.ignore_index), None, None, None
+
+
+def class_log_probs(logits, target=None, top_k=0, ignore_index=-100):
+    """Log probability of the target class, entropy and the `top_k` most probable classes at every position, in one pass.
+
+    logits [N, C, ...] fp32 or bf16, classes on axis 1 as in CrossEntropyLoss2d: rows [N, C] (tokens, classifier outputs; rows may
+    lie further apart than C), maps [N, C, H, W] (NCHW or channels-last memory, read where they are; other layouts are copied).
+    target [N, ...] int64 or None.  Returns ClassLogProbs of fp32 tensors:
+      log_prob [N, ...]            log softmax(logits)[target]; 0 where target == ignore_index; NaN for a target outside [0, C)
+                                   (as the weighted cross entropy, which cannot raise from a kernel either); None without a target
+      entropy [N, ...]             -sum p log p, of every position, ignored or not
+      top_log_probs [N, k, ...]    the k <= 32 largest log probabilities in falling order, equal ones by index, NaN before all
+      top_indices [N, k, ...]      their classes (int64); both None for top_k = 0
+    Differentiable in the logits through log_prob, entropy and top_log_probs (once).  A position whose incoming gradients are all 0
+    gets the gradient 0 whatever its logits hold, so padding that is ignored cannot spread NaN.
+    A logit of -inf has probability 0 and takes no part.  A position without any finite logit, or with +inf or NaN among its
+    logits, has no distribution: its log_prob (if not ignored), entropy and top_log_probs are NaN, as log_softmax's.
+    """
+    ops.require_gpu(logits, "class_log_probs")
+    if logits.requires_grad and torch.is_grad_enabled():
+        log_prob, entropy, top, index = _ClassLogProbsFn.apply(logits, target, int(top_k), int(ignore_index))
+    else:
+        log_prob, entropy, _, top, index = train_ops.class_log_probs_fwd(logits, target, int(top_k), int(ignore_index))
+    return ClassLogProbs(None if target is None else log_prob, entropy, top if top_k else None, index if top_k else None)

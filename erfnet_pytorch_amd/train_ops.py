@@ -1,0 +1,182 @@
+"""Operators of training and answering beside the convolution engine's: log probabilities of labels with entropy and top
+alternatives.
+
+Each is a plain function on tensors (one call through the C ABI on the current stream of the tensor's device, outputs from
+torch's allocator) and a registered op of the namespace `erfnet_mi355`, with a fake kernel for shapes and types and no CPU
+kernel, like those of torch_ops.py.  The differentiable entry points are loss.class_log_probs and norm.group_norm_act.
+"""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from ._lib import BF16, F32, call, size_query
+from .torch_ops import LIB, NS
+
+OPS = []                      # names, in registration order (tests walk this list)
+
+_no_guard = contextlib.nullcontext()
+
+
+def _register(schema: str, impl, fake):
+    name = schema.split("(", 1)[0]
+    LIB.define(schema)
+    LIB.impl(name, impl, "CUDA")
+    torch.library.register_fake(f"{NS}::{name}", fake, lib=LIB)
+    OPS.append(name)
+
+
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def on_device_of(t: torch.Tensor):
+    """Launches inside go to the current stream of t's device, whichever device is current outside."""
+    return _no_guard if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def dtype_code(t: torch.Tensor, who: str) -> int:
+    if t.dtype == torch.float32:
+        return F32
+    if t.dtype == torch.bfloat16:
+        return BF16
+    raise TypeError(f"{who}: float32 or bfloat16 tensors, got {t.dtype}")
+
+
+def _p(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _same_device(who, t, **others):
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{who}: {name} is on {o.device}, the input on {t.device}")
+
+
+# ------------------------------------------------------------------------------------------------ label log probabilities
+TOP_MAX = 32
+
+
+def class_layout(z: torch.Tensor):
+    """(tensor, N, C, L, stride of N, stride of C, shape without the class axis, rows) of logits [N, C, ...]: `rows` where the
+    classes of a position lie side by side ([N, C], or a channels-last map), else planes of L positions.  Other layouts are
+    copied into planes."""
+    n, c = z.shape[:2]
+    rest = z.shape[2:]
+    length = rest.numel()
+    if length == 1:
+        z = z if c == 1 or z.stride(1) == 1 else z.contiguous()
+        return z, n, c, 1, z.stride(0) if n > 1 else c, 1, (n, *rest), True
+    if c > 1 and z.stride(1) == 1 and z.movedim(1, -1).is_contiguous():
+        return z, n * length, c, 1, c, 1, (n, *rest), True
+    dense = 1                                               # the map's own axes, innermost last, without gaps
+    for size, stride in zip(reversed(rest), reversed(z.stride()[2:])):
+        dense = dense * size if size == 1 or stride == dense else 0
+    if not dense or not (c == 1 or z.stride(1) >= max(length, 2)):
+        z = z.contiguous()
+    return z, n, c, length, z.stride(0) if n > 1 else c * length, max(z.stride(1) if c > 1 else 0, length, 2), (n, *rest), False
+
+
+def _like_layout(z, rows):
+    """A dense tensor for the gradient: classes side by side for rows (channels-last for maps), else planes."""
+    if rows and z.dim() > 2:
+        return z.new_empty((z.shape[0], *z.shape[2:], z.shape[1])).movedim(-1, 1)
+    return z.new_empty(z.shape)
+
+
+def _top_shape(shape, k, rows):
+    """Memory shape of the alternatives, and the axis order that puts k where the class axis was."""
+    if rows:
+        return (*shape, k), (0, len(shape), *range(1, len(shape)))
+    return (shape[0], k, *shape[1:]), None
+
+
+def _check_target(who, target, shape, z):
+    if target is None:
+        return None
+    if target.dtype != torch.int64:
+        raise TypeError(f"{who}: targets are int64 class indices, got {target.dtype}")
+    if tuple(target.shape) != tuple(shape):
+        raise ValueError(f"{who}: expected targets of shape {tuple(shape)}, got {tuple(target.shape)}")
+    _same_device(who, z, target=target)
+    return target.contiguous()
+
+
+def class_log_probs_fwd(logits, target, top_k=0, ignore_index=-100):
+    """(log_prob, entropy, stats, top_log_probs, top_indices) of logits [N, C, ...]; loss.class_log_probs describes them.  stats
+    [2, ...]: the row maximum and log sum e^{z - max}, for the backward pass.  Without a target log_prob is empty."""
+    who = "class_log_probs"
+    code = dtype_code(logits, who)
+    if logits.dim() < 2 or logits.shape[1] < 1:
+        raise ValueError(f"{who}: logits have shape [N, C, ...] with at least one class, got {tuple(logits.shape)}")
+    if not 0 <= top_k <= min(TOP_MAX, logits.shape[1]):
+        raise ValueError(f"{who}: top_k lies between 0 and min({TOP_MAX}, classes), got {top_k} for {logits.shape[1]} classes")
+    z, n, c, length, sn, sc, shape, rows = class_layout(logits)
+    target = _check_target(who, target, shape, z)
+    new = z.new_empty
+    log_prob = new(shape if target is not None else (0,), dtype=torch.float32)
+    entropy, stats = new(shape, dtype=torch.float32), new((2, *shape), dtype=torch.float32)
+    top_shape, order = _top_shape(shape, top_k, rows)
+    top, index = new(top_shape, dtype=torch.float32), new(top_shape, dtype=torch.int64)
+    if entropy.numel():
+        with on_device_of(z):
+            call("erf_class_log_probs_fwd", z.data_ptr(), code, n, c, length, sn, sc, _p(target), ignore_index,
+                 log_prob.data_ptr() if target is not None else 0, entropy.data_ptr(), stats.data_ptr(), top_k, top.data_ptr() if top_k else 0,
+                 index.data_ptr() if top_k else 0, _stream())
+    if order is not None and top_k:
+        top, index = top.permute(order), index.permute(order)
+    elif not top_k:
+        top, index = top.view(shape[0], 0, *shape[1:]), index.view(shape[0], 0, *shape[1:])
+    return log_prob, entropy, stats, top, index
+
+
+def class_log_probs_bwd(logits, target, stats, entropy, top_indices, g_log_prob, g_entropy, g_top, ignore_index=-100):
+    """d logits, laid out as the logits."""
+    z, n, c, length, sn, sc, shape, rows = class_layout(logits)
+    code = dtype_code(z, "class_log_probs")
+    target = _check_target("class_log_probs", target, shape, z)
+    dz = _like_layout(z, rows)
+    if not dz.numel():
+        return dz
+    if rows:
+        dn, dc = c, 1
+    else:
+        dn, dc = c * length, max(length, 2)              
+    k = top_indices.shape[1] if g_top is not None else 0
+
+    def flat(t, like_top=False):
+        if t is None:
+            return None
+        if like_top and rows and t.dim() > 2:
+            t = t.movedim(1, -1)
+        return t.float().contiguous() if t.dtype != torch.int64 else t.contiguous()
+    g_log_prob, g_entropy = flat(g_log_prob), flat(g_entropy)
+    g_top, top_indices = (flat(g_top, True), flat(top_indices, True)) if k else (None, None)
+    with on_device_of(z):
+        call("erf_class_log_probs_bwd", z.data_ptr(), code, n, c, length, sn, sc, _p(target), ignore_index, stats.data_ptr(), entropy.data_ptr(),
+             _p(g_log_prob), _p(g_entropy), k, _p(top_indices), _p(g_top), dz.data_ptr(), dn, dc, _stream())
+    return dz
+
+
+def _lp_fwd_fake(logits, target, top_k, ignore_index):
+    shape = (logits.shape[0], *logits.shape[2:])
+    new = logits.new_empty
+    top = (shape[0], top_k, *shape[1:])
+    outs = [new(top, dtype=torch.float32), new(top, dtype=torch.int64)]
+    if top_k and len(shape) > 1 and class_layout(logits)[-1]:
+        outs = [new((*shape, top_k), dtype=o.dtype).movedim(-1, 1) for o in outs]
+    return (new(shape if target is not None else (0,), dtype=torch.float32), new(shape, dtype=torch.float32), new((2, *shape), dtype=torch.float32), *outs)
+
+
+_register("class_log_probs_fwd(Tensor logits, Tensor? target, int top_k, int ignore_index) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+          class_log_probs_fwd, _lp_fwd_fake)
+
+
+def _lp_bwd_fake(logits, target, stats, entropy, top_indices, g_log_prob, g_entropy, g_top, ignore_index):
+    z, *_, rows = class_layout(logits)
+    return _like_layout(z, rows)
+
+
+_register("class_log_probs_bwd(Tensor logits, Tensor? target, Tensor stats, Tensor entropy, Tensor top_indices, Tensor? g_log_prob, "
+          "Tensor? g_entropy, Tensor? g_top, int ignore_index) -> Tensor", class_log_probs_bwd, _lp_bwd_fake)

@@ -234,6 +234,24 @@ int erf_weighted_ce_fwd(const void* logits, int dtype, const long long* target, 
 int erf_weighted_ce_bwd(const void* logits, int dtype, const long long* target, const float* weight, int N, int C,
                         long long HW, const float* coef, void* dlogits, void* stream);
 
+/* ---- log probabilities of given labels, entropy and the most probable classes; and the gradient.
+ * Logits of N x L positions and C classes: class c of position (n, l) is logits[n * stride_n + c * stride_c + l].
+ *   rows: L = 1, stride_c = 1 (tokens, classifier outputs, channels-last maps);  planes: stride_c >= max(L, 2) (NCHW maps).
+ * All other arrays are contiguous: [N][L], and [N][k][L] for the alternatives (top_k <= min(ERF_TOP_MAX, C)).
+ * fwd: log_prob = log softmax(z)[target] (0 where target == ignore_index, NaN for a target outside [0, C)); target and log_prob are
+ *   both given or both NULL; entropy = -sum p log p; stats [2][N][L]: max z and log sum e^{z - max}, for bwd; alternatives in falling
+ *   order of their value, equal ones by index, NaN first.
+ * bwd: dlogits (same type, own strides, same kind of layout) = gl ([j = t] - p) - gh p (log p + entropy) + sum_k gk ([j = i_k] - p);
+ *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits hold. */
+#define ERF_TOP_MAX 32
+int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, long long L, long long stride_n, long long stride_c,
+                            const long long* target, long long ignore_index, float* log_prob, float* entropy, float* stats, int top_k,
+                            float* top_log_probs, long long* top_indices, void* stream);
+int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, long long L, long long stride_n, long long stride_c,
+                            const long long* target, long long ignore_index, const float* stats, const float* entropy,
+                            const float* g_log_prob, const float* g_entropy, int top_k, const long long* top_indices, const float* g_top,
+                            void* dlogits, long long dstride_n, long long dstride_c, void* stream);
+
 /* ---- optimiser over many tensors in one launch: AdamW (decoupled weight decay), moments in 32 or 8 bits.
  * m = b1 m + (1-b1) g; v = b2 v + (1-b2) g^2; p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps).
  * table: one device record per tensor; `dtype` (one per launch) is the element type of param and grad.

@@ -1,0 +1,418 @@
+"""loss.class_log_probs (log probability, entropy, top alternatives of labels) against the definition in 64 bits.
+
+Tolerances, U = 2^-24 (half an fp32 step), from the kernel's formula  m = max z, s = sum e^{z - m}, log p = (z - m) - log s,
+H = log s - sum e^{z-m} (z - m) / s:
+  a term e^y is off by 2 |y| U from y's two roundings and by at most 4 U from the exponential and its use; a partial sum of n terms adds
+  U per addition and 4 U per change of its maximum, 5 n in all.  With A = sum p |z - m| and B = sum p (z - m)^2:
+  log s: U (5 n + 4 + 2 A + 2 |log s|) =: E;  log p: E + U (|z - m| + 2 |log p|)
+  H: (log s's) + U (5 n + 8) A + 2 U B + E A + 2 U H
+  dz: with w = G + gh (log p + H): |p w| (off(log p) + 8 U) + p |gh| (off(log p) + off(H) + 4 U (|log p| + H)) + 4 U (|own| + p (|G| + ...)),
+  and half a step of the type.  n: additions one after another, the class count for planes, C / 64 + 32 for rows.
+"""
+import math
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+HALF = {torch.float32: U, torch.bfloat16: 2.0 ** -8}
+
+
+def _ref(z, target, k, ignore=-100):
+    """(log_prob, entropy, top, index) of float64 logits [R, C], differentiable, by torch's own log_softmax on the CPU."""
+    logp = torch.log_softmax(z, 1)
+    t = target.clamp(0, z.shape[1] - 1)
+    lp = torch.where(target == ignore, torch.zeros((), dtype=z.dtype), logp.gather(1, t[:, None])[:, 0])
+    p = logp.exp()
+    ent = -(p * torch.where(p > 0, logp, torch.zeros((), dtype=z.dtype))).sum(1)
+    index = z.detach().sort(dim=1, descending=True, stable=True)[1][:, :k]
+    return lp, ent, logp.gather(1, index), index
+
+
+def _tolerances(z, n):
+    """off(log p) [R, C], off(H) [R] of float64 logits whose rows have a finite logit."""
+    m = z.max(1, keepdim=True)[0]
+    y = (z - m).clamp_min(-1e30)
+    p = torch.softmax(z, 1)
+    logp = torch.log_softmax(z, 1).clamp_min(-1e30)
+    logs = (z - m).exp().sum(1).log()
+    a, b = (p * y.abs()).sum(1), (p * y * y).sum(1)
+    h = -(p * logp).sum(1)                                  # p = 0 where logp was cut off
+    e = U * (5 * n + 4 + 2 * a + 2 * logs.abs())
+    return e[:, None] + U * (y.abs() + 2 * logp.abs()), e + U * (5 * n + 8) * a + 2 * U * b + e * a + 2 * U * h
+
+
+def _close(got, want, tol):
+    return (got == want) | ((got - want).abs() <= tol)
+
+
+def _to_rows(t, k_axis=False):
+    """[N, C, ...] -> [R, C] (class axis last), [N, ...] -> [R]."""
+    if k_axis:
+        return t.movedim(1, -1).reshape(-1, t.shape[1])
+    return t.reshape(-1)
+
+
+def _logits(shape, dtype, layout, seed, spread=3.0, shift=0.0):
+    gen = torch.Generator().manual_seed(seed)
+    z = (spread * torch.randn(shape, generator=gen) + shift).to(dtype)
+    if layout == "channels_last":
+        return z.cuda().contiguous(memory_format=torch.channels_last)
+    if layout == "padded":                                    # rows further apart than C, first one off the 16-byte grid
+        big = torch.full((shape[0], shape[1] + 5), 99.0, dtype=dtype).cuda()
+        big[:, 1:1 + shape[1]] = z.cuda()
+        return big[:, 1:1 + shape[1]]
+    if layout == "sliced":                                    # a run of classes and images of a larger map
+        big = torch.full((shape[0] + 1, shape[1] + 2, *shape[2:]), 99.0, dtype=dtype).cuda()
+        big[1:, 1:-1] = z.cuda()
+        return big[1:, 1:-1]
+    if layout == "transposed":                                # no layout of its own: copied
+        return z.movedim(1, 0).contiguous().cuda().movedim(0, 1)
+    return z.cuda()
+
+
+def _check(z, target, k, grads=True, seed=0):
+    from erfnet_pytorch_amd.loss import class_log_probs
+    c = z.shape[1]
+    rows_layout = z.dim() == 2 or z.is_contiguous(memory_format=torch.channels_last) if z.dim() in (2, 4) else False
+    n = c / 64 + 32 if rows_layout else c
+    z = z.detach().requires_grad_(grads)
+    out = class_log_probs(z, target, top_k=k)
+    zr = _to_rows(z.detach().cpu().double(), True).requires_grad_()
+    tr = _to_rows(target.cpu())
+    lp, ent, top, index = _ref(zr, tr, k)
+    off_lp, off_h = _tolerances(zr.detach(), n)
+    shape = (z.shape[0], *z.shape[2:])
+    assert out.log_prob.shape == shape and out.entropy.shape == shape and out.log_prob.dtype == out.entropy.dtype == torch.float32
+    got = _to_rows(out.log_prob.detach().cpu().double())
+    live = tr != -100
+    assert _close(got, lp.detach(), off_lp.gather(1, tr.clamp_min(0)[:, None])[:, 0])[live].all() and (got[~live] == 0).all()
+    assert ((_to_rows(out.entropy.detach().cpu().double()) - ent.detach()).abs() <= off_h).all()
+    if k:
+        assert out.top_indices.shape == (shape[0], k, *shape[1:]) and out.top_indices.dtype == torch.int64
+        assert torch.equal(_to_rows(out.top_indices.cpu(), True), index)
+        assert _close(_to_rows(out.top_log_probs.detach().cpu().double(), True), top.detach(), off_lp.gather(1, index)).all()
+    else:
+        assert out.top_log_probs is None and out.top_indices is None
+    if not grads:
+        return
+    gen = torch.Generator().manual_seed(seed)
+    r = zr.shape[0]
+    gl, gh, gk = torch.randn(r, generator=gen), torch.randn(r, generator=gen), torch.randn(r, k, generator=gen)
+    back = lambda t: t.reshape(shape).cuda()                                                     # noqa: E731
+    outs, gs = [out.log_prob, out.entropy], [back(gl), back(gh)]
+    if k:
+        outs.append(out.top_log_probs)
+        gs.append(gk.reshape(*shape, k).movedim(-1, 1).cuda())
+    dz, = torch.autograd.grad(outs, z, gs)
+    assert dz.shape == z.shape and dz.dtype == z.dtype
+    heads = (lp * gl.double()).sum() + (ent * gh.double()).sum() + (top * gk.double()).sum()
+    want, = torch.autograd.grad(heads, zr)
+    with torch.no_grad():
+        logp = torch.log_softmax(zr, 1)
+        p = logp.exp()
+        size_lp = logp.abs().clamp_max(1e30)
+        pull = (gl.double() * live)[:, None].abs() + gk.double().abs().sum(1, keepdim=True)
+        w = pull + gh.double()[:, None].abs() * (size_lp + ent[:, None])
+        own = torch.zeros_like(p).scatter_add_(1, tr.clamp_min(0)[:, None], (gl.double().abs() * live)[:, None])
+        if k:
+            own.scatter_add_(1, index, gk.double().abs())
+        tol = p * w * (off_lp + 8 * U) + p * gh.double()[:, None].abs() * (off_lp + off_h[:, None] + 4 * U * (size_lp + ent[:, None])) \
+            + 4 * U * (own + p * w) + 8 * k * U * (own + p * pull)
+        tol = torch.where(p > 0, tol, 4 * U * own) + HALF[z.dtype] * want.abs() + 2.0 ** -125
+        assert ((_to_rows(dz.cpu().double(), True) - want).abs() <= tol).all()
+
+
+def _targets(z, seed, ignored=0.2):
+    gen = torch.Generator().manual_seed(seed)
+    shape = (z.shape[0], *z.shape[2:])
+    t = torch.randint(0, z.shape[1], shape, generator=gen)
+    t[torch.rand(shape, generator=gen) < ignored] = -100
+    return t.cuda()
+
+
+ROWS = [(1, 1), (3, 2), (700, 20), (5, 33), (2, 64), (4, 1000), (1, 2049), (3, 4097), (300, 4096), (2, 70001), (1, 200000)]
+MAPS = [(1, 1, 3, 3), (2, 20, 5, 7), (2, 6, 1, 1), (1, 150, 16, 17), (3, 2, 1, 1000), (2, 20, 32, 64), (1, 33, 128, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["plain", "padded"])
+@pytest.mark.parametrize("shape", ROWS)
+def test_rows(shape, layout, dtype):
+    z = _logits(shape, dtype, layout, 1)
+    t = _targets(z, 2)
+    for k in sorted({0, min(3, shape[1]), min(32, shape[1])}):
+        _check(z, t, k, seed=k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["plain", "channels_last", "sliced", "transposed"])
+@pytest.mark.parametrize("shape", MAPS)
+def test_maps(shape, layout, dtype):
+    z = _logits(shape, dtype, layout, 3)
+    t = _targets(z, 4)
+    for k in sorted({0, 1, min(5, shape[1]), min(32, shape[1])}):
+        _check(z, t, k, seed=k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 20, 9), (2, 20, 2, 3, 4), (0, 7), (2, 7, 0, 3)])
+def test_other_numbers_of_axes_and_empty_batches(shape):
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits(shape, torch.float32, "plain", 5)
+    if z.numel():
+        return _check(z, _targets(z, 6), 2)
+    z.requires_grad_()
+    out = class_log_probs(z, torch.zeros((shape[0], *shape[2:]), dtype=torch.int64, device="cuda"), top_k=3)
+    assert out.log_prob.shape == (shape[0], *shape[2:]) and out.top_indices.shape == (shape[0], 3, *shape[2:])
+    dz, = torch.autograd.grad(out.entropy.sum() + out.log_prob.sum(), z)
+    assert dz.shape == z.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 50), (3, 5000), (2, 20, 6, 8)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_far_from_zero_and_widely_spread_logits(shape, dtype):
+    for spread, shift in ((3.0, 1e4), (3.0, -1e4), (200.0, 0.0), (1e-3, 0.0), (1e30, 0.0)):
+        z = _logits(shape, dtype, "plain", 7, spread, shift)
+        _check(z, _targets(z, 8), 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 50), (2, 5000), (2, 20, 6, 8), (1, 20, 8, 130)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_equal_values_go_by_index(shape, dtype):
+    """All logits equal; a handful of values only; zeros of both signs."""
+    for seed, make in enumerate((lambda z: torch.zeros_like(z), lambda z: (z > 0).to(z.dtype), lambda z: (z * 0.5).round(),
+                                 lambda z: torch.where(z > 0, 0.0, -0.0).to(z.dtype))):
+        z = make(_logits(shape, dtype, "plain", seed))
+        _check(z, _targets(z, 9), 20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(6, 50), (6, 5000), (1, 20, 2, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masked_classes(shape, dtype):
+    """-inf and the type's lowest value in masked places: every second class, all but one, all (-inf: no distribution)."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    low = torch.finfo(dtype).min
+    z = _logits(shape, dtype, "plain", 11)
+    rows = z.movedim(1, -1).reshape(-1, shape[1]).clone()
+    rows[0, ::2] = float("-inf")
+    rows[1, 1:] = float("-inf")
+    rows[2, ::2] = low
+    rows[3, 1:] = low
+    rows[4, :] = low
+    rows[5, :7] = float("-inf")
+    rows[5, 7:14] = low
+    z = rows.reshape(shape[0], *shape[2:], shape[1]).movedim(-1, 1).contiguous()
+    t = torch.ones((shape[0], *shape[2:]), dtype=torch.int64, device="cuda")
+    t.view(-1)[1] = 0
+    _check(z, t, 5)
+    t.view(-1)[1] = 1                                       # a masked target: -inf, and a finite gradient
+    z.requires_grad_()
+    out = class_log_probs(z, t)
+    assert float(out.log_prob.detach().reshape(-1)[1]) == float("-inf") and float(out.entropy.detach().reshape(-1)[1]) == 0.0
+    dz, = torch.autograd.grad(out.log_prob.view(-1)[1], z)
+    dz = dz.movedim(1, -1).reshape(-1, shape[1])
+    assert dz[1, 0] == -1 and dz[1, 1] == 1 and (dz[1, 2:] == 0).all() and (dz[0] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(5, 50), (5, 5000), (1, 20, 1, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_positions_without_a_distribution_and_ignored_ones(shape, dtype):
+    """All -inf, +inf, NaN: NaN as log_softmax's, in that position alone; ignored or without a gradient, they give exactly 0."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits(shape, dtype, "plain", 12)
+    rows = z.movedim(1, -1).reshape(-1, shape[1]).clone()
+    rows[0, :] = float("-inf")
+    rows[1, 5] = float("inf")
+    rows[2, 7] = float("nan")
+    z = rows.reshape(shape[0], *shape[2:], shape[1]).movedim(-1, 1).contiguous().requires_grad_()
+    t = torch.tensor([1, 1, 1, 1, -100], device="cuda").reshape(shape[0], *shape[2:])
+    out = class_log_probs(z, t, top_k=4)
+    lp, ent, top, index = (a.detach() for a in out)
+    lp, ent, top, index = lp.reshape(-1), ent.reshape(-1), top.movedim(1, -1).reshape(-1, 4), index.movedim(1, -1).reshape(-1, 4)
+    assert lp[:3].isnan().all() and ent[:3].isnan().all() and top[:3].isnan().all() and lp[3:].isfinite().all() and lp[4] == 0 and ent[3:].isfinite().all()
+    assert index[0].tolist() == [0, 1, 2, 3] and index[1, 0] == 5 and index[2, 0] == 7
+    t = torch.tensor([-100, -100, -100, 1, -100], device="cuda").reshape(shape[0], *shape[2:])
+    g = torch.tensor([0, 0, 0, 1.0, 1.0], device="cuda").reshape(t.shape)
+    out = class_log_probs(z, t, top_k=4)
+    dz, = torch.autograd.grad([out.log_prob, out.entropy, out.top_log_probs], z,
+                              [torch.ones_like(g), g, g.unsqueeze(1).expand(g.shape[0], 4, *g.shape[1:])])
+    dz = dz.movedim(1, -1).reshape(-1, shape[1])
+    assert (dz[:3] == 0).all() and dz[3:].isfinite().all() and (dz[3] != 0).any() and (dz[4] != 0).any()
+
+
+@pytest.mark.gpu
+def test_targets_outside_the_classes_give_nan_and_another_ignore_index():
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits((4, 9), torch.float32, "plain", 13).requires_grad_()
+    out = class_log_probs(z, torch.tensor([9, -1, 255, 3], device="cuda"), ignore_index=255)
+    assert out.log_prob.detach().isnan().tolist() == [True, True, False, False] and out.log_prob[2] == 0
+    dz, = torch.autograd.grad(out.log_prob.sum(), z)
+    assert dz[:2].isnan().all() and (dz[2] == 0).all() and dz[3].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_without_target_and_partial_gradients():
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits((3, 30), torch.float32, "plain", 14).requires_grad_()
+    out = class_log_probs(z, top_k=2)
+    assert out.log_prob is None
+    d1, = torch.autograd.grad(out.entropy.sum(), z, retain_graph=True)
+    d2, = torch.autograd.grad(out.top_log_probs.sum(), z)
+    zr = z.detach().cpu().double().requires_grad_()
+    _, ent, top, _ = _ref(zr, torch.zeros(3, dtype=torch.int64), 2)
+    w1, = torch.autograd.grad(ent.sum(), zr, retain_graph=True)
+    w2, = torch.autograd.grad(top.sum(), zr)
+    # 32 + 30 / 64 additions, log p and H below 12: every factor within 2000 U of its value
+    assert (d1.cpu() - w1).abs().max() <= 2000 * U * 24 and (d2.cpu() - w2).abs().max() <= 2000 * U * 4
+    with torch.no_grad():
+        assert not class_log_probs(z).entropy.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 11), (1, 11, 1, 3)])
+def test_gradient_against_differences(shape):
+    """(f(z + h) - f(z - h)) / 2h with h = 2^-6: truncated at h^2 / 6 |f'''|, |f'''| <= 40 for log p and H of logits this flat
+    (third derivatives are sums of at most 6 products of numbers up to log 11 + 2), rounded by 2 * 2000 U / 2h."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits(shape, torch.float32, "plain", 15, 0.5)
+    t = _targets(z, 16, 0.0)
+    zz = z.clone().requires_grad_()
+    out = class_log_probs(zz, t)
+    grads = [torch.autograd.grad(f.sum(), zz, retain_graph=True)[0] for f in (out.log_prob, out.entropy)]
+    h = 2.0 ** -6
+    for c in range(shape[1]):
+        ends = []
+        for s in (h, -h):
+            moved = z.clone()
+            moved[:, c] += s
+            o = class_log_probs(moved, t)
+            ends.append((o.log_prob, o.entropy))
+        for f, g in enumerate(grads):
+            diff = (ends[0][f].double() - ends[1][f].double()) / (2 * h)
+            assert (diff - g[:, c].double()).abs().max() <= h * h / 6 * 40 + 4000 * U / (2 * h)
+
+
+@pytest.mark.gpu
+def test_rows_of_the_gradient_do_not_touch_what_lies_between_them():
+    from erfnet_pytorch_amd import _lib, ops
+    from erfnet_pytorch_amd.loss import class_log_probs
+    n, c, s = 5, 37, 48
+    z = torch.randn(n, s, device="cuda")
+    d = torch.full((n, s), 7.0, device="cuda")
+    t = torch.randint(0, c, (n,), device="cuda")
+    zz = z[:, :c].clone().requires_grad_()
+    out = class_log_probs(zz, t)
+    want, = torch.autograd.grad(out.log_prob.sum(), zz)
+    stats = torch.empty(2, n, device="cuda")
+    lp, ent, one = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.ones(n, device="cuda")
+    from erfnet_pytorch_amd import train_ops
+    got = train_ops.class_log_probs_fwd(z[:, :c], t)
+    stats.copy_(got[2])
+    ent.copy_(got[1])
+    _lib.call("erf_class_log_probs_bwd", z.data_ptr(), _lib.F32, n, c, 1, s, 1, t.data_ptr(), -100, stats.data_ptr(), ent.data_ptr(), one.data_ptr(),
+              0, 0, 0, 0, d.data_ptr(), s, 1, ops._stream())
+    assert torch.equal(d[:, :c], want) and (d[:, c:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 70001), (40, 1000), (2, 20, 16, 32)])
+def test_captured_calls_and_another_stream(shape):
+    """Forward and backward captured together, replayed on new inputs with eager calls between; two graphs at once; a side stream."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+
+    def both(z, t, g):
+        out = class_log_probs(z, t, top_k=4)
+        dz, = torch.autograd.grad([out.log_prob, out.entropy], z, [g, g])
+        return [a.detach() for a in out] + [dz]
+    z = [_logits(shape, torch.bfloat16, "plain", 20 + i).requires_grad_() for i in range(2)]
+    t = [_targets(z[i], 30 + i) for i in range(2)]
+    g = torch.randn(t[0].shape, device="cuda")
+    both(z[0], t[0], g)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, capture_error_mode="thread_local"):
+            outs.append(both(z[i], t[i], g))
+        graphs.append(gr)
+    for rep in range(3):
+        for i in range(2):
+            with torch.no_grad():
+                z[i].copy_(_logits(shape, torch.bfloat16, "plain", 40 + 2 * rep + i))
+        for gr in graphs:
+            gr.replay()
+        want = [both(z[i].detach().clone().requires_grad_(), t[i], g) for i in range(2)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = both(z[0].detach().clone().requires_grad_(), t[0], g)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(there, want[0]))
+
+
+# ------------------------------------------------------------------------------------------------ refusals (CPU)
+def test_wrong_arguments_are_refused():
+    from erfnet_pytorch_amd import train_ops
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = torch.zeros(3, 5)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        class_log_probs(z, torch.zeros(3, dtype=torch.int64))
+    f = train_ops.class_log_probs_fwd
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        f(z.half(), None)
+    with pytest.raises(TypeError, match="int64"):
+        f(z, torch.zeros(3, dtype=torch.int32))
+    for bad in (torch.zeros(4, dtype=torch.int64), torch.zeros(3, 5, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="targets of shape"):
+            f(z, bad)
+    with pytest.raises(ValueError, match="device|on meta"):
+        f(z, torch.zeros(3, dtype=torch.int64, device="meta"))
+    for k in (-1, 6):
+        with pytest.raises(ValueError, match="top_k"):
+            f(z, None, k)
+    with pytest.raises(ValueError, match="top_k"):
+        f(torch.zeros(1, 100), None, 33)
+    for bad in (torch.zeros(3), torch.zeros(3, 0)):
+        with pytest.raises(ValueError, match="shape"):
+            f(bad, None)
+
+
+def test_abi_refuses_bad_arguments_without_a_gpu():
+    from erfnet_pytorch_amd import _lib
+    good = [16, 0, 4, 5, 1, 5, 1, 16, -100, 16, 16, 16, 2, 16, 16, 0]
+    for i, bad in ((0, 0), (1, 2), (2, 0), (3, 0), (4, 0), (5, -1), (6, 0), (7, 0), (9, 0), (10, 0), (11, 0), (12, 6), (12, -1), (13, 0), (14, 0)):
+        args = list(good)
+        args[i] = bad
+        assert _lib.query("erf_class_log_probs_fwd", *args) == -1, i
+    good = [16, 0, 4, 5, 6, 30, 6, 16, -100, 16, 16, 16, 16, 2, 16, 16, 16, 30, 6, 0]
+    for i, bad in ((0, 0), (1, 2), (2, 0), (3, 0), (4, 0), (6, 5), (6, 1), (7, 0), (9, 0), (10, 0), (13, 33), (14, 0), (16, 0), (17, -1), (18, 5), (18, 1)):
+        args = list(good)
+        args[i] = bad
+        assert _lib.query("erf_class_log_probs_bwd", *args) == -1, i
+
+
+def test_layouts_are_recognised():
+    from erfnet_pytorch_amd.train_ops import class_layout
+    z = torch.zeros(2, 5, 3, 4)
+    assert class_layout(z)[1:6] == (2, 5, 12, 60, 12)
+    assert class_layout(z.contiguous(memory_format=torch.channels_last))[1:6] == (24, 5, 1, 5, 1)
+    assert class_layout(z[:, 1:3])[1:6] == (2, 2, 12, 60, 12)
+    assert class_layout(z.transpose(2, 3))[0].is_contiguous()
+    assert class_layout(torch.zeros(4, 9)[:, 2:7])[1:6] == (4, 5, 1, 9, 1)
+    assert class_layout(torch.zeros(1, 1, 3, 4))[1:6] == (1, 1, 12, 12, 12)
+    assert class_layout(torch.zeros(2, 5, 1, 1))[1:6] == (2, 5, 1, 5, 1)
+    assert class_layout(torch.zeros(3, 8, 1, 1)[:, 1:7])[1:6] == (3, 6, 1, 8, 1)
+    assert class_layout(torch.zeros(3, 8, 1, 2)[..., :1])[1:6] == (3, 8, 1, 8, 1)
+    assert class_layout(torch.zeros(3, 1, 1, 1))[1:6] == (3, 1, 1, 1, 1)
+    assert class_layout(torch.zeros(4, 3).t())[1:6] == (3, 4, 1, 4, 1)
+    assert math.prod(class_layout(torch.zeros(0, 7, 3, 4))[1:4:2]) == 0
