@@ -1,5 +1,5 @@
 """Operators of training and answering beside the convolution engine's: log probabilities of labels with entropy and top
-alternatives.
+alternatives, group normalisation with an activation on channels-last maps.
 
 Each is a plain function on tensors (one call through the C ABI on the current stream of the tensor's device, outputs from
 torch's allocator) and a registered op of the namespace `erfnet_mi355`, with a fake kernel for shapes and types and no CPU
@@ -180,3 +180,100 @@ def _lp_bwd_fake(logits, target, stats, entropy, top_indices, g_log_prob, g_entr
 
 _register("class_log_probs_bwd(Tensor logits, Tensor? target, Tensor stats, Tensor entropy, Tensor top_indices, Tensor? g_log_prob, "
           "Tensor? g_entropy, Tensor? g_top, int ignore_index) -> Tensor", class_log_probs_bwd, _lp_bwd_fake)
+
+
+# ------------------------------------------------------------------------------------------------ group norm + activation
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+
+
+def channels_last(x: torch.Tensor) -> torch.Tensor:
+    """Logical [N, C, ...] as a contiguous [N, ..., C]; zero-copy where the memory is channels-last."""
+    last = x.movedim(1, -1)
+    if last.is_contiguous():
+        return last
+    if x.dim() == 4 and x.is_contiguous() and x.numel():
+        n, c, h, w = x.shape
+        out = x.new_empty((n, h, w, c))
+        code = dtype_code(x, "group_norm_act")
+        with on_device_of(x):
+            call("erf_nchw_to_nhwc", x.data_ptr(), code, out.data_ptr(), code, n, c, h, w, _stream())
+        return out
+    return last.contiguous()
+
+
+def _gn_check(x, weight, bias, groups, activation):
+    who = "group_norm_act"
+    code = dtype_code(x, who)
+    if x.dim() < 2 or not x.is_contiguous():
+        raise ValueError(f"{who}: a contiguous channels-last tensor [N, ..., C], got shape {tuple(x.shape)} strides {x.stride()}")
+    c = x.shape[-1]
+    if groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"{who}: {c} channels do not split into {groups} groups")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{who}: activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (c,):
+            raise ValueError(f"{who}: {name} has shape [{c}], got {tuple(t.shape)}")
+    _same_device(who, x, weight=weight, bias=bias)
+    return code, x.shape[0], x.numel() // max(1, x.shape[0] * c), c
+
+
+def _f32(t):
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.float().contiguous()
+
+
+def _gn_workspace(x, code, n, hw, c, groups):
+    return torch.empty(size_query("erf_group_norm_workspace_bytes", code, n, hw, c, groups), dtype=torch.uint8, device=x.device)
+
+
+def group_norm_act_fwd(x, weight, bias, groups, eps, activation):
+    """(y, mean [N, groups], rstd [N, groups]) of a contiguous channels-last x [N, ..., C]; norm.group_norm_act describes them."""
+    code, n, hw, c = _gn_check(x, weight, bias, groups, activation)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"group_norm_act: invalid eps {eps}")
+    weight, bias = _f32(weight), _f32(bias)
+    y = torch.empty_like(x)
+    mean, rstd = x.new_empty((n, groups), dtype=torch.float32), x.new_empty((n, groups), dtype=torch.float32)
+    if x.numel():
+        with on_device_of(x):
+            ws = _gn_workspace(x, code, n, hw, c, groups)
+            call("erf_group_norm_fwd", x.data_ptr(), y.data_ptr(), code, n, hw, c, groups, _p(weight), _p(bias), eps, ACTIVATIONS[activation],
+                 mean.data_ptr(), rstd.data_ptr(), ws.data_ptr(), _stream())
+    return y, mean, rstd
+
+
+def group_norm_act_bwd(dy, x, weight, bias, mean, rstd, groups, activation):
+    """(dx, dweight [C], dbias [C]) from a contiguous channels-last dy; the parameter gradients are fp32 whatever the types."""
+    code, n, hw, c = _gn_check(x, weight, bias, groups, activation)
+    if dy.shape != x.shape or dy.dtype != x.dtype or not dy.is_contiguous():
+        raise ValueError(f"group_norm_act: dy is a contiguous {x.dtype} tensor of shape {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)} strides {dy.stride()}")
+    if mean.shape != (n, groups) or rstd.shape != (n, groups) or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise ValueError(f"group_norm_act: mean and rstd are fp32 [{n}, {groups}]")
+    _same_device("group_norm_act", x, dy=dy, mean=mean, rstd=rstd)
+    weight, bias, mean, rstd = _f32(weight), _f32(bias), _f32(mean), _f32(rstd)
+    dx = torch.empty_like(x)
+    if not x.numel():
+        return dx, x.new_zeros(c, dtype=torch.float32), x.new_zeros(c, dtype=torch.float32)
+    dweight, dbias = x.new_empty(c, dtype=torch.float32), x.new_empty(c, dtype=torch.float32)
+    with on_device_of(x):
+        ws = _gn_workspace(x, code, n, hw, c, groups)
+        call("erf_group_norm_bwd", x.data_ptr(), dy.data_ptr(), dx.data_ptr(), code, n, hw, c, groups, _p(weight), _p(bias), ACTIVATIONS[activation],
+             mean.data_ptr(), rstd.data_ptr(), dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), _stream())
+    return dx, dweight, dbias
+
+
+def _gn_fwd_fake(x, weight, bias, groups, eps, activation):
+    stat = (x.shape[0], groups)
+    return torch.empty_like(x), x.new_empty(stat, dtype=torch.float32), x.new_empty(stat, dtype=torch.float32)
+
+
+_register("group_norm_act_fwd(Tensor x, Tensor? weight, Tensor? bias, int groups, float eps, str activation) -> (Tensor, Tensor, Tensor)",
+          group_norm_act_fwd, _gn_fwd_fake)
+
+
+def _gn_bwd_fake(dy, x, weight, bias, mean, rstd, groups, activation):
+    return torch.empty_like(x), x.new_empty(x.shape[-1], dtype=torch.float32), x.new_empty(x.shape[-1], dtype=torch.float32)
+
+
+_register("group_norm_act_bwd(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, int groups, str activation) -> "
+          "(Tensor, Tensor, Tensor)", group_norm_act_bwd, _gn_bwd_fake)

@@ -234,6 +234,21 @@ int erf_weighted_ce_fwd(const void* logits, int dtype, const long long* target, 
 int erf_weighted_ce_bwd(const void* logits, int dtype, const long long* target, const float* weight, int N, int C,
                         long long HW, const float* coef, void* dlogits, void* stream);
 
+/* ---- group normalisation with an activation on channels-last maps x, y [N][HW][C] (contiguous; y and dx may not alias x or dy).
+ * y = act((x - mean) * rstd * gamma + beta), mean / rstd [N][groups] over HW x C / groups values (rstd = 1 / sqrt(var + eps)).
+ * gamma, beta: fp32 [C] or NULL (1, 0).  bwd: dx, and dgamma / dbeta fp32 [C] (each may be NULL), from the forward pass's x, mean
+ * and rstd.  workspace: erf_group_norm_workspace_bytes (0: unsupported arguments), 16-byte aligned, not shared by calls that may
+ * overlap; it need not be cleared. */
+#define ERF_ACT_NONE 0
+#define ERF_ACT_RELU 1
+#define ERF_ACT_SILU 2
+size_t erf_group_norm_workspace_bytes(int dtype, int N, long long HW, int C, int groups);
+int erf_group_norm_fwd(const void* x, void* y, int dtype, int N, long long HW, int C, int groups, const float* gamma, const float* beta,
+                       float eps, int act, float* mean, float* rstd, void* workspace, void* stream);
+int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N, long long HW, int C, int groups, const float* gamma,
+                       const float* beta, int act, const float* mean, const float* rstd, float* dgamma, float* dbeta, void* workspace,
+                       void* stream);
+
 /* ---- log probabilities of given labels, entropy and the most probable classes; and the gradient.
  * Logits of N x L positions and C classes: class c of position (n, l) is logits[n * stride_n + c * stride_c + l].
  *   rows: L = 1, stride_c = 1 (tokens, classifier outputs, channels-last maps);  planes: stride_c >= max(L, 2) (NCHW maps).
