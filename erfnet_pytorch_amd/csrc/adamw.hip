@@ -73,70 +73,165 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+template <typename T> struct Quad;                            // 4 neighbouring values in memory
+template <> struct Quad<float> { typedef f32x4 raw; };
+template <> struct Quad<bf16raw> { typedef i32x2 raw; };
+
+// One lane's 4 elements of a scale block on their way through the update
+template <typename T, int BITS>
+struct Lane4 {
+    f32x4 p, g, m, v;                                         // BITS 8: m and v's codes as words, decoded by update()
+    int cm, cr;
+
+    // VEC: all 4 elements exist and lie on vector boundaries; else n of them, one by one
+    template <bool VEC>
+    __device__ __forceinline__ void load(const erf_adamw_tensor& t, long long i, int n) {
+        if (VEC) {
+            p = load4((const T*)t.param + i);
+            g = load4((const T*)t.grad + i);
+            if (BITS == 32) { m = *(const f32x4*)((const float*)t.exp_avg + i); v = *(const f32x4*)((const float*)t.exp_avg_sq + i); }
+            else { cm = *(const int*)((const char*)t.exp_avg + i); cr = *(const int*)((const char*)t.exp_avg_sq + i); }
+            return;
+        }
+        cm = cr = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = e < n;
+            p[e] = in ? Elem<T>::ld((const T*)t.param + i + e) : 0.f;
+            g[e] = in ? Elem<T>::ld((const T*)t.grad + i + e) : 0.f;
+            if (BITS == 32) {
+                m[e] = in ? ((const float*)t.exp_avg)[i + e] : 0.f;
+                v[e] = in ? ((const float*)t.exp_avg_sq)[i + e] : 0.f;
+            } else if (in) {
+                cm |= ((const unsigned char*)t.exp_avg)[i + e] << (8 * e);
+                cr |= ((const unsigned char*)t.exp_avg_sq)[i + e] << (8 * e);
+            }
+        }
+    }
+
+    template <bool VEC>
+    __device__ __forceinline__ void store(const erf_adamw_tensor& t, long long i, int n) const {
+        if (VEC) {
+            store4((T*)t.param + i, p);
+            if (BITS == 32) { *(f32x4*)((float*)t.exp_avg + i) = m; *(f32x4*)((float*)t.exp_avg_sq + i) = v; }
+            else { *(int*)((char*)t.exp_avg + i) = cm; *(int*)((char*)t.exp_avg_sq + i) = cr; }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e >= n) break;
+            Elem<T>::st((T*)t.param + i + e, p[e]);
+            if (BITS == 32) { ((float*)t.exp_avg)[i + e] = m[e]; ((float*)t.exp_avg_sq)[i + e] = v[e]; }
+            else { ((unsigned char*)t.exp_avg)[i + e] = cm >> (8 * e); ((unsigned char*)t.exp_avg_sq)[i + e] = cr >> (8 * e); }
+        }
+    }
+};
+
+struct AdamwScalars { float step_size, decay, inv_bc2, b1, omb1, b2, omb2, eps; unsigned key; };
+
+// The update of one wave's scale block, QB elements from `first` on; sm, sr: its scales, replaced by the new ones
+template <typename T, int BITS>
+__device__ __forceinline__ void adamw_update(Lane4<T, BITS>& x, const AdamwScalars& k, unsigned counter, float& sm, float& sr) {
+#pragma clang fp contract(off)
+    if (BITS == 8) {
+        const f32x2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cm, true);
+        const f32x2 r0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, true);
+        x.m = f32x4{m0[0], m0[1], m1[0], m1[1]};
+        x.v = f32x4{r0[0], r0[1], r1[0], r1[1]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float r = x.v[e] * sr;
+            x.m[e] *= sm;
+            x.v[e] = r * r;
+        }
+    }
+    float r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x.m[e] = x.m[e] * k.b1 + x.g[e] * k.omb1;
+        x.v[e] = x.v[e] * k.b2 + x.g[e] * x.g[e] * k.omb2;
+        r[e] = sqrtf(x.v[e]);
+        x.p[e] = x.p[e] * k.decay - x.m[e] / (r[e] * k.inv_bc2 + k.eps) * k.step_size;
+    }
+    if (BITS == 8) {
+        // a value that is not finite becomes a NaN code and leaves its neighbours' scale alone
+        float am = 0.f, ar = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            am = fmaxf(am, fabsf(x.m[e]) < INFINITY ? fabsf(x.m[e]) : 0.f);
+            ar = fmaxf(ar, r[e] < INFINITY ? r[e] : 0.f);
+        }
+        const int em = scale_exp(wave_max(am)), er = scale_exp(wave_max(ar));
+        const float im = exp2i(-em), ir = exp2i(-er);
+        sm = exp2i(em);
+        sr = exp2i(er);
+        float qm[4], qr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned h = mix32((counter + e) ^ k.key);
+            qm[e] = round_e4m3(x.m[e] * im, h & 0xFFFFu, false);
+            qr[e] = round_e4m3(r[e] * ir, h >> 16, true);
+        }
+        x.cm = __builtin_amdgcn_cvt_pk_fp8_f32(qm[2], qm[3], __builtin_amdgcn_cvt_pk_fp8_f32(qm[0], qm[1], 0, false), true);
+        x.cr = __builtin_amdgcn_cvt_pk_fp8_f32(qr[2], qr[3], __builtin_amdgcn_cvt_pk_fp8_f32(qr[0], qr[1], 0, false), true);
+    }
+}
+
+// A workgroup takes one chunk; a wave takes every 4th scale block of it, 4 neighbouring elements per lane (16-byte accesses on
+// fp32, 8 on bf16, 4 on codes).  A whole chunk on vector boundaries has all its loads in flight before the first update; what is
+// ragged or lies off the boundaries goes block by block, element by element.
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
-#pragma clang fp contract(off)
+    constexpr int PER_WAVE = CHUNK / QB / 4;
     const int2 ch = a.chunks[blockIdx.x];
     const erf_adamw_tensor t = a.table[ch.x];
     const int step = a.steps[blockIdx.x] + 1;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long start = (long long)ch.y * CHUNK;
+    const unsigned long long at = (unsigned long long)t.param | (unsigned long long)t.grad |
+                                  (BITS == 32 ? (unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq : 0ull);
+    const bool whole = start + CHUNK <= t.count && at % sizeof(typename Quad<T>::raw) == 0 &&
+                       (BITS == 8 ? ((unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq) % 4 == 0
+                                  : ((unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq) % 16 == 0);
+    Lane4<T, BITS> x[PER_WAVE];
+    float sm[PER_WAVE], sr[PER_WAVE];
+    if (whole) {
+#pragma unroll
+        for (int j = 0; j < PER_WAVE; ++j) {
+            const int q = j * 4 + wave;
+            x[j].template load<true>(t, start + q * QB + lane * 4, 4);
+            if (BITS == 8) { sm[j] = t.exp_avg_scale[start / QB + q]; sr[j] = t.root_scale[start / QB + q]; }
+        }
+    }
     __syncthreads();                                          // every wave has read the count
     if (threadIdx.x == 0) a.steps[blockIdx.x] = step;
     const double lr = *a.lr;
-    const float step_size = (float)(lr / (1.0 - ipow(a.b1, step))), decay = (float)(1.0 - lr * a.wd);
-    const float inv_bc2 = (float)(1.0 / sqrt(1.0 - ipow(a.b2, step)));
-    const float b1 = (float)a.b1, omb1 = (float)(1.0 - a.b1), b2 = (float)a.b2, omb2 = (float)(1.0 - a.b2), eps = (float)a.eps;
-    const unsigned key = ((unsigned)step * 0x9E3779B9u) ^ a.seed;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    T* p = (T*)t.param;
-    const T* g = (const T*)t.grad;
+    const AdamwScalars k{(float)(lr / (1.0 - ipow(a.b1, step))), (float)(1.0 - lr * a.wd), (float)(1.0 / sqrt(1.0 - ipow(a.b2, step))),
+                         (float)a.b1, (float)(1.0 - a.b1), (float)a.b2, (float)(1.0 - a.b2), (float)a.eps,
+                         ((unsigned)step * 0x9E3779B9u) ^ a.seed};
+    if (whole) {
+#pragma unroll
+        for (int j = 0; j < PER_WAVE; ++j) {
+            const int q = j * 4 + wave;
+            const long long i = start + q * QB + lane * 4;
+            adamw_update<T, BITS>(x[j], k, (unsigned)(t.base + i), sm[j], sr[j]);
+            x[j].template store<true>(t, i, 4);
+            if (BITS == 8 && lane == 0) { t.exp_avg_scale[start / QB + q] = sm[j]; t.root_scale[start / QB + q] = sr[j]; }
+        }
+        return;
+    }
     for (int q = wave; q < CHUNK / QB; q += 4) {
-        const long long first = (long long)ch.y * CHUNK + q * QB, base = first + lane * 4;
+        const long long first = start + q * QB, i = first + lane * 4;
         if (first >= t.count) break;                          // uniform over the wave
-        float m[4], r[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const long long i = base + e;
-            const bool in = i < t.count;
-            const float gi = in ? Elem<T>::ld(g + i) : 0.f;
-            float mi, vi;
-            if (BITS == 32) {
-                mi = in ? ((const float*)t.exp_avg)[i] : 0.f;
-                vi = in ? ((const float*)t.exp_avg_sq)[i] : 0.f;
-            } else {
-                const int cm = in ? ((const unsigned char*)t.exp_avg)[i] : 0, cr = in ? ((const unsigned char*)t.exp_avg_sq)[i] : 0;
-                mi = __builtin_amdgcn_cvt_f32_fp8(cm, 0) * t.exp_avg_scale[first / QB];
-                vi = __builtin_amdgcn_cvt_f32_fp8(cr, 0) * t.root_scale[first / QB];
-                vi = vi * vi;
-            }
-            mi = mi * b1 + gi * omb1;
-            vi = vi * b2 + gi * gi * omb2;
-            const float ri = sqrtf(vi);
-            if (in) {
-                Elem<T>::st(p + i, Elem<T>::ld(p + i) * decay - mi / (ri * inv_bc2 + eps) * step_size);
-                if (BITS == 32) { ((float*)t.exp_avg)[i] = mi; ((float*)t.exp_avg_sq)[i] = vi; }
-            }
-            m[e] = mi; r[e] = ri;
-        }
-        if (BITS == 8) {
-            // a value that is not finite becomes a NaN code and leaves its neighbours' scale alone
-            float am = 0.f, ar = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                am = fmaxf(am, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.f);
-                ar = fmaxf(ar, r[e] < INFINITY ? r[e] : 0.f);
-            }
-            const int em = scale_exp(wave_max(am)), er = scale_exp(wave_max(ar));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const long long i = base + e;
-                if (i >= t.count) break;
-                const unsigned h = mix32((unsigned)(t.base + i) ^ key);
-                const float qm = round_e4m3(m[e] * exp2i(-em), h & 0xFFFFu, false), qr = round_e4m3(r[e] * exp2i(-er), h >> 16, true);
-                ((unsigned char*)t.exp_avg)[i] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(qm, qm, 0, false);
-                ((unsigned char*)t.exp_avg_sq)[i] = (unsigned char)__builtin_amdgcn_cvt_pk_fp8_f32(qr, qr, 0, false);
-            }
-            if (lane == 0) { t.exp_avg_scale[first / QB] = exp2i(em); t.root_scale[first / QB] = exp2i(er); }
-        }
+        const long long left = t.count - i;
+        const int n = left > 4 ? 4 : left < 0 ? 0 : (int)left;
+        Lane4<T, BITS> y;
+        float ym = 0.f, yr = 0.f;
+        y.template load<false>(t, i, n);
+        if (BITS == 8) { ym = t.exp_avg_scale[first / QB]; yr = t.root_scale[first / QB]; }
+        adamw_update<T, BITS>(y, k, (unsigned)(t.base + i), ym, yr);
+        y.template store<false>(t, i, n);
+        if (BITS == 8 && lane == 0) { t.exp_avg_scale[first / QB] = ym; t.root_scale[first / QB] = yr; }
     }
 }
 
