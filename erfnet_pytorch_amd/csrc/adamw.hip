@@ -14,6 +14,7 @@
 // are rounded.
 #include "../../include/erfnet_mi355.h"
 #include "common.cuh"
+#include <type_traits>
 
 #define CHUNK 4096
 #define QB 256
@@ -46,135 +47,197 @@ __device__ __forceinline__ unsigned mix32(unsigned h) {
     return h ^ (h >> 16);
 }
 
-// x, |x| <= 448, to the e4m3 value below or above it, up with probability (16 random bits) distance / step.
+// x, |x| <= 448, to the e4m3 value below or above it, up with probability (16 random bits) distance / step; the sign is dropped.
 // Values from 2^-6 on have 3 mantissa bits: adding random bits below them and cutting them off is the rounding.  Below 2^-6 the
-// step stays 2^-9, which is the mantissa step of x + 2^-6.  least: what is above 0 stays above 0.
-__device__ __forceinline__ float round_e4m3(float x, unsigned rnd16, bool least) {
-    float a = fabsf(x);
-    const bool low = a < 0.015625f;
-    a = low ? a + 0.015625f : a;
-    a = __uint_as_float((__float_as_uint(a) + (rnd16 << 4)) & 0xFFF00000u);
-    a = low ? a - 0.015625f : a;
-    if (least) a = x > 0.f ? fmaxf(a, 0.001953125f) : a;
-    return fabsf(x) <= 448.f ? copysignf(a, x) : __builtin_nanf("");
+// step stays 2^-9, which is the mantissa step of x + 2^-6.
+__device__ __forceinline__ float round_e4m3(float x, unsigned rnd16) {
+    const float up = fabsf(x) < 0.015625f ? 0.015625f : 0.f;
+    const unsigned b = (__float_as_uint(fabsf(x) + up) + (rnd16 << 4)) & 0xFFF00000u;
+    return __uint_as_float(b) - up;
 }
 
-// 2^e with e the smallest exponent that brings `most` to 448 = 1.75 * 2^8 or below
-__device__ __forceinline__ int scale_exp(float most) {
-    const unsigned b = __float_as_uint(most);
-    const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    return most > 0.f ? min(max(e, -126), 120) : -126;
+// 2^e with e the smallest exponent that brings the value with bits `most` (finite, >= 0) to 448 = 1.75 * 2^8 or below
+__device__ __forceinline__ int scale_exp(unsigned most) {
+    const int e = (int)(most >> 23) - 127 - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return most ? min(max(e, -126), 120) : -126;
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// Largest of the 64 lanes' values, as a scalar: shifts within rows of 16 lanes, then the rows' last lanes are passed on
+template <int CTRL>
+__device__ __forceinline__ unsigned umax_dpp(unsigned v) {
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+    v = umax_dpp<0x111>(v);                                   // row_shr 1, 2, 4, 8
+    v = umax_dpp<0x112>(v);
+    v = umax_dpp<0x114>(v);
+    v = umax_dpp<0x118>(v);
+    v = umax_dpp<0x142>(v);                                   // row_bcast 15, 31
+    v = umax_dpp<0x143>(v);
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-template <typename T> struct Quad;                            // 4 neighbouring values in memory
-template <> struct Quad<float> { typedef f32x4 raw; };
-template <> struct Quad<bf16raw> { typedef i32x2 raw; };
+// Addresses from the table are global memory: said here, the compiler forms scalar base + 32-bit offset accesses
+#define GLOBAL __attribute__((address_space(1)))
 
-// One lane's 4 elements of a scale block on their way through the update
+// One chunk's arrays, at its first element; scales at the chunk's first scale block
+template <typename T, int BITS>
+struct ChunkPtrs {
+    typedef typename std::conditional<BITS == 32, float, unsigned char>::type S;
+    GLOBAL T* p;
+    const GLOBAL T* g;
+    GLOBAL S *m, *v;
+    GLOBAL float *sm, *sr;
+    __device__ __forceinline__ ChunkPtrs(const erf_adamw_tensor& t, long long start)
+        : p((GLOBAL T*)t.param + start), g((const GLOBAL T*)t.grad + start), m((GLOBAL S*)t.exp_avg + start), v((GLOBAL S*)t.exp_avg_sq + start),
+          sm((GLOBAL float*)t.exp_avg_scale + start / QB), sr((GLOBAL float*)t.root_scale + start / QB) {}
+};
+
+__device__ __forceinline__ f32x4 quad(const GLOBAL float* p) { return *(const GLOBAL f32x4*)p; }
+__device__ __forceinline__ f32x4 quad(const GLOBAL bf16raw* p) {
+    const i32x2 r = *(const GLOBAL i32x2*)p;
+    return f32x4{__uint_as_float((unsigned)r[0] << 16), __uint_as_float((unsigned)r[0] & 0xFFFF0000u), __uint_as_float((unsigned)r[1] << 16),
+                 __uint_as_float((unsigned)r[1] & 0xFFFF0000u)};
+}
+__device__ __forceinline__ void put_quad(GLOBAL float* p, const f32x4& v) { *(GLOBAL f32x4*)p = v; }
+__device__ __forceinline__ void put_quad(GLOBAL bf16raw* p, const f32x4& v) { *(GLOBAL i32x2*)p = pack_bf16x4(v); }
+
+// One lane's 4 elements of a scale block on their way through the update; i: their place in the chunk.
+// VEC: all 4 exist and lie on vector boundaries; else the first n of them, one by one.
 template <typename T, int BITS>
 struct Lane4 {
-    f32x4 p, g, m, v;                                         // BITS 8: m and v's codes as words, decoded by update()
+    f32x4 p, g, m, v;                                         // BITS 8: m and v's codes as words, decoded by the update
     int cm, cr;
 
-    // VEC: all 4 elements exist and lie on vector boundaries; else n of them, one by one
     template <bool VEC>
-    __device__ __forceinline__ void load(const erf_adamw_tensor& t, long long i, int n) {
-        if (VEC) {
-            p = load4((const T*)t.param + i);
-            g = load4((const T*)t.grad + i);
-            if (BITS == 32) { m = *(const f32x4*)((const float*)t.exp_avg + i); v = *(const f32x4*)((const float*)t.exp_avg_sq + i); }
-            else { cm = *(const int*)((const char*)t.exp_avg + i); cr = *(const int*)((const char*)t.exp_avg_sq + i); }
-            return;
-        }
-        cm = cr = 0;
+    __device__ __forceinline__ void load(const ChunkPtrs<T, BITS>& t, unsigned i, int n) {
+        if constexpr (VEC) {
+            p = quad(t.p + i);
+            g = quad(t.g + i);
+            if constexpr (BITS == 32) { m = quad(t.m + i); v = quad(t.v + i); }
+            else { cm = *(const GLOBAL int*)(t.m + i); cr = *(const GLOBAL int*)(t.v + i); }
+        } else {
+            cm = cr = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const bool in = e < n;
-            p[e] = in ? Elem<T>::ld((const T*)t.param + i + e) : 0.f;
-            g[e] = in ? Elem<T>::ld((const T*)t.grad + i + e) : 0.f;
-            if (BITS == 32) {
-                m[e] = in ? ((const float*)t.exp_avg)[i + e] : 0.f;
-                v[e] = in ? ((const float*)t.exp_avg_sq)[i + e] : 0.f;
-            } else if (in) {
-                cm |= ((const unsigned char*)t.exp_avg)[i + e] << (8 * e);
-                cr |= ((const unsigned char*)t.exp_avg_sq)[i + e] << (8 * e);
+            for (int e = 0; e < 4; ++e) {
+                const bool in = e < n;
+                p[e] = in ? Elem<T>::to_f32(t.p[i + e]) : 0.f;
+                g[e] = in ? Elem<T>::to_f32(t.g[i + e]) : 0.f;
+                if constexpr (BITS == 32) {
+                    m[e] = in ? t.m[i + e] : 0.f;
+                    v[e] = in ? t.v[i + e] : 0.f;
+                } else if (in) {
+                    cm |= t.m[i + e] << (8 * e);
+                    cr |= t.v[i + e] << (8 * e);
+                }
             }
         }
     }
 
     template <bool VEC>
-    __device__ __forceinline__ void store(const erf_adamw_tensor& t, long long i, int n) const {
-        if (VEC) {
-            store4((T*)t.param + i, p);
-            if (BITS == 32) { *(f32x4*)((float*)t.exp_avg + i) = m; *(f32x4*)((float*)t.exp_avg_sq + i) = v; }
-            else { *(int*)((char*)t.exp_avg + i) = cm; *(int*)((char*)t.exp_avg_sq + i) = cr; }
-            return;
-        }
+    __device__ __forceinline__ void store(const ChunkPtrs<T, BITS>& t, unsigned i, int n) const {
+        if constexpr (VEC) {
+            put_quad(t.p + i, p);
+            if constexpr (BITS == 32) { put_quad(t.m + i, m); put_quad(t.v + i, v); }
+            else { *(GLOBAL int*)(t.m + i) = cm; *(GLOBAL int*)(t.v + i) = cr; }
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e >= n) break;
-            Elem<T>::st((T*)t.param + i + e, p[e]);
-            if (BITS == 32) { ((float*)t.exp_avg)[i + e] = m[e]; ((float*)t.exp_avg_sq)[i + e] = v[e]; }
-            else { ((unsigned char*)t.exp_avg)[i + e] = cm >> (8 * e); ((unsigned char*)t.exp_avg_sq)[i + e] = cr >> (8 * e); }
+            for (int e = 0; e < 4; ++e) {
+                if (e >= n) break;
+                t.p[i + e] = Elem<T>::from_f32(p[e]);
+                if constexpr (BITS == 32) { t.m[i + e] = m[e]; t.v[i + e] = v[e]; }
+                else { t.m[i + e] = (unsigned char)(cm >> (8 * e)); t.v[i + e] = (unsigned char)(cr >> (8 * e)); }
+            }
         }
     }
 };
 
 struct AdamwScalars { float step_size, decay, inv_bc2, b1, omb1, b2, omb2, eps; unsigned key; };
 
-// The update of one wave's scale block, QB elements from `first` on; sm, sr: its scales, replaced by the new ones
-template <typename T, int BITS>
-__device__ __forceinline__ void adamw_update(Lane4<T, BITS>& x, const AdamwScalars& k, unsigned counter, float& sm, float& sr) {
+// sqrt(v), v >= 0, to half a step but for one case in a million: y = v / sqrt(v) from the hardware's reciprocal root, then
+// y + (v - y^2) / (2 sqrt(v)).  A v below the smallest normal number has no digits left and loses some more.
+__device__ __forceinline__ float fast_sqrt(float v) {
+    const float s = __builtin_amdgcn_rsqf(fmaxf(v, 1.17549435e-38f)), y = v * s;
+    return fmaf(fmaf(-y, y, v), 0.5f * s, y);
+}
+// m / d, d finite and not 0, in the same way
+__device__ __forceinline__ float fast_div(float m, float d) {
+    const float r = __builtin_amdgcn_rcpf(d), q = m * r;
+    return fmaf(fmaf(-q, d, m), r, q);
+}
+
+// The update with moments in 32 bits.  Multiplications and additions round one by one (no fused ones), so that a plain program
+// gives the same bits.
+template <typename T>
+__device__ __forceinline__ void adamw_update(Lane4<T, 32>& x, const AdamwScalars& k, unsigned, float&, float&) {
 #pragma clang fp contract(off)
-    if (BITS == 8) {
-        const f32x2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cm, true);
-        const f32x2 r0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, true);
-        x.m = f32x4{m0[0], m0[1], m1[0], m1[1]};
-        x.v = f32x4{r0[0], r0[1], r1[0], r1[1]};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float r = x.v[e] * sr;
-            x.m[e] *= sm;
-            x.v[e] = r * r;
-        }
-    }
-    float r[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         x.m[e] = x.m[e] * k.b1 + x.g[e] * k.omb1;
         x.v[e] = x.v[e] * k.b2 + x.g[e] * x.g[e] * k.omb2;
-        r[e] = sqrtf(x.v[e]);
-        x.p[e] = x.p[e] * k.decay - x.m[e] / (r[e] * k.inv_bc2 + k.eps) * k.step_size;
+        x.p[e] = x.p[e] * k.decay - x.m[e] / (sqrtf(x.v[e]) * k.inv_bc2 + k.eps) * k.step_size;
     }
-    if (BITS == 8) {
+}
+
+// ... in 8 bits, of one wave's scale block; sm, sr: its scales, replaced by the new ones.  The arithmetic, not the memory, bounds
+// this kernel: what handles values that are not finite stands in a branch of its own that a wave takes when it has met one (bits
+// of NaN and infinity, as integers, are above all others, so the maximum finds them).
+template <typename T>
+__device__ __forceinline__ void adamw_update(Lane4<T, 8>& x, const AdamwScalars& k, unsigned counter, float& sm, float& sr) {
+#pragma clang fp contract(off)
+    const f32x2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cm, true);
+    const f32x2 r0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, true);
+    float m[4] = {m0[0], m0[1], m1[0], m1[1]}, r[4] = {r0[0], r0[1], r1[0], r1[1]}, v[4];
+    unsigned bm[4], br[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float old = r[e] * sr;
+        m[e] = m[e] * sm * k.b1 + x.g[e] * k.omb1;
+        v[e] = old * old * k.b2 + x.g[e] * x.g[e] * k.omb2;
+        r[e] = fast_sqrt(v[e]);
+        bm[e] = __float_as_uint(m[e]) & 0x7FFFFFFFu;
+        br[e] = __float_as_uint(r[e]);
+    }
+    unsigned most_m = wave_umax(max(max(bm[0], bm[1]), max(bm[2], bm[3]))), most_r = wave_umax(max(max(br[0], br[1]), max(br[2], br[3])));
+    const bool odd = most_m >= 0x7F800000u || most_r >= 0x7F800000u || k.eps == 0.f;
+    if (!odd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.p[e] = x.p[e] * k.decay - fast_div(m[e], r[e] * k.inv_bc2 + k.eps) * k.step_size;
+    } else {
         // a value that is not finite becomes a NaN code and leaves its neighbours' scale alone
-        float am = 0.f, ar = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            am = fmaxf(am, fabsf(x.m[e]) < INFINITY ? fabsf(x.m[e]) : 0.f);
-            ar = fmaxf(ar, r[e] < INFINITY ? r[e] : 0.f);
+            r[e] = sqrtf(v[e]);
+            x.p[e] = x.p[e] * k.decay - m[e] / (r[e] * k.inv_bc2 + k.eps) * k.step_size;
+            br[e] = __float_as_uint(r[e]) < 0x7F800000u ? __float_as_uint(r[e]) : 0u;
+            bm[e] = bm[e] < 0x7F800000u ? bm[e] : 0u;
         }
-        const int em = scale_exp(wave_max(am)), er = scale_exp(wave_max(ar));
-        const float im = exp2i(-em), ir = exp2i(-er);
-        sm = exp2i(em);
-        sr = exp2i(er);
-        float qm[4], qr[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const unsigned h = mix32((counter + e) ^ k.key);
-            qm[e] = round_e4m3(x.m[e] * im, h & 0xFFFFu, false);
-            qr[e] = round_e4m3(r[e] * ir, h >> 16, true);
-        }
-        x.cm = __builtin_amdgcn_cvt_pk_fp8_f32(qm[2], qm[3], __builtin_amdgcn_cvt_pk_fp8_f32(qm[0], qm[1], 0, false), true);
-        x.cr = __builtin_amdgcn_cvt_pk_fp8_f32(qr[2], qr[3], __builtin_amdgcn_cvt_pk_fp8_f32(qr[0], qr[1], 0, false), true);
+        most_m = wave_umax(max(max(bm[0], bm[1]), max(bm[2], bm[3])));
+        most_r = wave_umax(max(max(br[0], br[1]), max(br[2], br[3])));
     }
+    const int em = scale_exp(most_m), er = scale_exp(most_r);
+    const float im = exp2i(-em), ir = exp2i(-er);
+    sm = exp2i(em);
+    sr = exp2i(er);
+    float qm[4], qr[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned h = mix32((counter + e) ^ k.key);
+        const float tm = m[e] * im, tr = r[e] * ir;
+        qm[e] = copysignf(round_e4m3(tm, h & 0xFFFFu), tm);
+        qr[e] = tr > 0.f ? fmaxf(round_e4m3(tr, h >> 16), 0.001953125f) : 0.f;        // above 0 stays above 0
+    }
+    if (odd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            qm[e] = fabsf(m[e]) < INFINITY ? qm[e] : __builtin_nanf("");
+            qr[e] = r[e] < INFINITY ? qr[e] : __builtin_nanf("");
+        }
+    }
+    x.cm = __builtin_amdgcn_cvt_pk_fp8_f32(qm[2], qm[3], __builtin_amdgcn_cvt_pk_fp8_f32(qm[0], qm[1], 0, false), true);
+    x.cr = __builtin_amdgcn_cvt_pk_fp8_f32(qr[2], qr[3], __builtin_amdgcn_cvt_pk_fp8_f32(qr[0], qr[1], 0, false), true);
 }
 
 // A workgroup takes one chunk; a wave takes every 4th scale block of it, 4 neighbouring elements per lane (16-byte accesses on
@@ -186,21 +249,20 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
     const int2 ch = a.chunks[blockIdx.x];
     const erf_adamw_tensor t = a.table[ch.x];
     const int step = a.steps[blockIdx.x] + 1;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const long long start = (long long)ch.y * CHUNK;
-    const unsigned long long at = (unsigned long long)t.param | (unsigned long long)t.grad |
-                                  (BITS == 32 ? (unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq : 0ull);
-    const bool whole = start + CHUNK <= t.count && at % sizeof(typename Quad<T>::raw) == 0 &&
-                       (BITS == 8 ? ((unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq) % 4 == 0
-                                  : ((unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq) % 16 == 0);
+    const ChunkPtrs<T, BITS> ptr(t, start);
+    constexpr unsigned long long VT = sizeof(T) * 4 - 1, VS = BITS == 32 ? 15 : 3;
+    const bool whole = start + CHUNK <= t.count && (((unsigned long long)t.param | (unsigned long long)t.grad) & VT) == 0 &&
+                       (((unsigned long long)t.exp_avg | (unsigned long long)t.exp_avg_sq) & VS) == 0;
     Lane4<T, BITS> x[PER_WAVE];
     float sm[PER_WAVE], sr[PER_WAVE];
     if (whole) {
 #pragma unroll
         for (int j = 0; j < PER_WAVE; ++j) {
-            const int q = j * 4 + wave;
-            x[j].template load<true>(t, start + q * QB + lane * 4, 4);
-            if (BITS == 8) { sm[j] = t.exp_avg_scale[start / QB + q]; sr[j] = t.root_scale[start / QB + q]; }
+            const unsigned q = j * 4 + wave;
+            x[j].template load<true>(ptr, q * QB + lane * 4, 4);
+            if (BITS == 8) { sm[j] = ptr.sm[q]; sr[j] = ptr.sr[q]; }
         }
     }
     __syncthreads();                                          // every wave has read the count
@@ -209,29 +271,29 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
     const AdamwScalars k{(float)(lr / (1.0 - ipow(a.b1, step))), (float)(1.0 - lr * a.wd), (float)(1.0 / sqrt(1.0 - ipow(a.b2, step))),
                          (float)a.b1, (float)(1.0 - a.b1), (float)a.b2, (float)(1.0 - a.b2), (float)a.eps,
                          ((unsigned)step * 0x9E3779B9u) ^ a.seed};
+    const unsigned counter = (unsigned)(t.base + start);
     if (whole) {
 #pragma unroll
         for (int j = 0; j < PER_WAVE; ++j) {
-            const int q = j * 4 + wave;
-            const long long i = start + q * QB + lane * 4;
-            adamw_update<T, BITS>(x[j], k, (unsigned)(t.base + i), sm[j], sr[j]);
-            x[j].template store<true>(t, i, 4);
-            if (BITS == 8 && lane == 0) { t.exp_avg_scale[start / QB + q] = sm[j]; t.root_scale[start / QB + q] = sr[j]; }
+            const unsigned q = j * 4 + wave, i = q * QB + lane * 4;
+            adamw_update<T>(x[j], k, counter + i, sm[j], sr[j]);
+            x[j].template store<true>(ptr, i, 4);
+            if (BITS == 8 && lane == 0) { ptr.sm[q] = sm[j]; ptr.sr[q] = sr[j]; }
         }
         return;
     }
-    for (int q = wave; q < CHUNK / QB; q += 4) {
-        const long long first = start + q * QB, i = first + lane * 4;
-        if (first >= t.count) break;                          // uniform over the wave
-        const long long left = t.count - i;
-        const int n = left > 4 ? 4 : left < 0 ? 0 : (int)left;
+    const int count = (int)(t.count - start < CHUNK ? t.count - start : CHUNK);
+    for (unsigned q = wave; q < CHUNK / QB; q += 4) {
+        if ((int)(q * QB) >= count) break;                    // uniform over the wave
+        const unsigned i = q * QB + lane * 4;
+        const int n = min(max(count - (int)i, 0), 4);
         Lane4<T, BITS> y;
         float ym = 0.f, yr = 0.f;
-        y.template load<false>(t, i, n);
-        if (BITS == 8) { ym = t.exp_avg_scale[first / QB]; yr = t.root_scale[first / QB]; }
-        adamw_update<T, BITS>(y, k, (unsigned)(t.base + i), ym, yr);
-        y.template store<false>(t, i, n);
-        if (BITS == 8 && lane == 0) { t.exp_avg_scale[first / QB] = ym; t.root_scale[first / QB] = yr; }
+        y.template load<false>(ptr, i, n);
+        if (BITS == 8) { ym = ptr.sm[q]; yr = ptr.sr[q]; }
+        adamw_update<T>(y, k, counter + i, ym, yr);
+        y.template store<false>(ptr, i, n);
+        if (BITS == 8 && lane == 0) { ptr.sm[q] = ym; ptr.sr[q] = yr; }
     }
 }
 
