@@ -110,7 +110,8 @@ SIGNATURES = {
     "erf_group_norm_workspace_bytes": (c_size_t, [I, I, LL, I, I]),
     "erf_group_norm_fwd": (I, [P, P, I, I, LL, I, I, P, P, F, I, P, P, P, P]),
     "erf_group_norm_bwd": (I, [P, P, P, I, I, LL, I, I, P, P, I, P, P, P, P, P, P]),
-    "erf_class_log_probs_fwd": (I, [P, I, LL, I, LL, LL, LL, P, LL, P, P, P, I, P, P, P]),
+    "erf_class_log_probs_workspace_bytes": (c_size_t, [I, LL, I, LL, LL, I]),
+    "erf_class_log_probs_fwd": (I, [P, I, LL, I, LL, LL, LL, P, LL, P, P, P, I, P, P, P, P]),
     "erf_class_log_probs_bwd": (I, [P, I, LL, I, LL, LL, LL, P, LL, P, P, P, P, I, P, P, P, LL, LL, P]),
     "erf_adamw_chunk_elements": (I, []),
     "erf_adamw_scale_block": (I, []),

@@ -19,31 +19,51 @@
 struct Stat { float m, s, t; };
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 __device__ __forceinline__ void stat_move(Stat& a, float m) {          // a's sums about the larger maximum m
-    const float d = fmaxf((a.m - base_of(m)) * LOG2E, -200.f), f = exp2f(d);
+    const float d = fmaxf((a.m - base_of(m)) * LOG2E, -200.f), f = __builtin_amdgcn_exp2f(d);
     a.t = f * (a.t + a.s * d);
     a.s = f * a.s;
     a.m = m;
 }
-__device__ __forceinline__ void stat_add(Stat& a, float z) {           // z <= a.m, or NaN
-    const float y = (z - base_of(a.m)) * LOG2E, e = exp2f(y);
+__device__ __forceinline__ void stat_add(Stat& a, float base, float z) {          // base = base_of(a.m), z <= a.m or NaN
+    const float y = (z - base) * LOG2E, e = __builtin_amdgcn_exp2f(y);
     a.s += e;
-    a.t += e * fmaxf(y, -200.f);                                       // 0 * -inf
-}
-__device__ __forceinline__ void stat_join(Stat& a, Stat b) {
-    const float m = fmaxf(a.m, b.m);
-    stat_move(a, m);
-    stat_move(b, m);
-    a.s += b.s;
-    a.t += b.t;
+    a.t += e * fmaxf(y, -200.f);                                       // 0 * -inf; NaN comes through e
 }
 
-// Order of the alternatives as one integer: larger value first, then lower index; NaN before everything, -0 as 0
-__device__ __forceinline__ unsigned long long rank_of(float z, unsigned j) {
+// Order of the alternatives as one integer: larger value first, then lower index; NaN before everything, -0 as 0.  No rank
+// is 0 or ~0: these stand for nothing and for a bound above all.
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 rank_of(float z, unsigned j) {
     const unsigned b = __float_as_uint(z == 0.f ? 0.f : z);
-    const unsigned k = z != z ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    return ((unsigned long long)k << 32) | (0xFFFFFFFFu - j);
+    const unsigned k = z != z ? 0xFFFFFFFEu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return ((u64)k << 32) | (0xFFFFFFFFu - j);
 }
-__device__ __forceinline__ unsigned rank_index(unsigned long long r) { return 0xFFFFFFFFu - (unsigned)r; }
+__device__ __forceinline__ unsigned rank_index(u64 r) { return 0xFFFFFFFFu - (unsigned)r; }
+__device__ __forceinline__ float rank_value(u64 r) {
+    const unsigned k = (unsigned)(r >> 32);
+    return k > 0xFF800000u ? __builtin_nanf("") : __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+}
+
+// Reductions over the 64 lanes: shifts within rows of 16 lanes, then the rows' last lanes are passed on; lane 63 has the result
+template <int CTRL> __device__ __forceinline__ int dpp0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true); }
+template <int CTRL> __device__ __forceinline__ void sum_step(float& v) { v += __int_as_float(dpp0<CTRL>(__float_as_int(v))); }
+__device__ __forceinline__ float wave_total(float v) {
+    sum_step<0x111>(v); sum_step<0x112>(v); sum_step<0x114>(v); sum_step<0x118>(v); sum_step<0x142>(v); sum_step<0x143>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+template <int CTRL> __device__ __forceinline__ void max_step(u64& v) {
+    const u64 o = ((u64)(unsigned)dpp0<CTRL>((int)(v >> 32)) << 32) | (unsigned)dpp0<CTRL>((int)v);
+    v = o > v ? o : v;
+}
+__device__ __forceinline__ u64 wave_best(u64 v) {
+    max_step<0x111>(v); max_step<0x112>(v); max_step<0x114>(v); max_step<0x118>(v); max_step<0x142>(v); max_step<0x143>(v);
+    return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ float wave_largest(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
 
 struct LpArgs {
     const void* z;
@@ -53,12 +73,14 @@ struct LpArgs {
     long long ignore;
     float *log_prob, *entropy, *stats, *top;
     long long* top_index;
+    int segments;                      // rows: workgroups per row
+    u64* parts;                        // [N][segments][2 + k]: (m, s), (t, -), the segment's best ranks
 };
 
-// log p of the target, entropy and the saved pair of row i from its statistics
+// log p of the target, entropy and the saved pair of position i from its statistics
 template <typename T>
-__device__ __forceinline__ void lp_finish(const LpArgs& a, const T* row, long long i, const Stat& st, long long rows) {
-    const float base = base_of(st.m), logs = logf(st.s);
+__device__ __forceinline__ void lp_finish(const LpArgs& a, const T* row, long long i, const Stat& st, float logs) {
+    const float base = base_of(st.m);
     if (a.log_prob) {
         const long long t = a.target[i];
         float v = __builtin_nanf("");                                  // a target outside [0, C): as in the weighted cross entropy
@@ -68,12 +90,13 @@ __device__ __forceinline__ void lp_finish(const LpArgs& a, const T* row, long lo
     }
     a.entropy[i] = logs - st.t * LN2 / st.s;
     a.stats[i] = base;
-    a.stats[rows + i] = logs;
+    a.stats[a.N * a.L + i] = logs;
 }
 
-// planes: one thread per pixel
+// ------------------------------------------------------------------------------------------------ one thread per position
+// Planes, and rows of few classes.  The alternatives by k rounds over the classes.
 template <typename T>
-__global__ __launch_bounds__(256) void lp_planes_kernel(const LpArgs a) {
+__global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
     const long long rows = a.N * a.L;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows; i += (long long)gridDim.x * 256) {
         const long long n = i / a.L, l = i % a.L;
@@ -82,65 +105,263 @@ __global__ __launch_bounds__(256) void lp_planes_kernel(const LpArgs a) {
         for (int c = 0; c < a.C; ++c) {
             const float z = Elem<T>::ld(row + c * a.sc);
             if (z > st.m) stat_move(st, z);
-            stat_add(st, z);
+            stat_add(st, base_of(st.m), z);
         }
-        lp_finish(a, row, i, st, rows);
-        unsigned long long last = ~0ull;
+        const float logs = logf(st.s);
+        lp_finish(a, row, i, st, logs);
+        u64 last = ~0ull;
         for (int k = 0; k < a.k; ++k) {
-            unsigned long long best = 0;
+            u64 best = 0;
             for (int c = 0; c < a.C; ++c) {
-                const unsigned long long r = rank_of(Elem<T>::ld(row + c * a.sc), c);
+                const u64 r = rank_of(Elem<T>::ld(row + c * a.sc), c);
                 if ((r < last || k == 0) && r > best) best = r;
             }
             last = best;
-            const unsigned j = rank_index(best);
-            a.top[(n * a.k + k) * a.L + l] = (Elem<T>::ld(row + j * a.sc) - base_of(st.m)) - logf(st.s);
-            a.top_index[(n * a.k + k) * a.L + l] = j;
+            a.top[(n * a.k + k) * a.L + l] = (rank_value(best) - base_of(st.m)) - logs;
+            a.top_index[(n * a.k + k) * a.L + l] = rank_index(best);
         }
     }
 }
 
-// rows: one workgroup per row
-template <typename T>
-__global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
-    __shared__ Stat part[4];
-    __shared__ unsigned long long ranks[4];
-    const long long i = blockIdx.x;
-    const T* row = (const T*)a.z + i * a.sn;
-    Stat st{-INFINITY, 0.f, 0.f};
-    for (int c = threadIdx.x; c < a.C; c += 256) {
-        const float z = Elem<T>::ld(row + c);
-        if (z > st.m) stat_move(st, z);
-        stat_add(st, z);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) stat_join(st, Stat{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)});
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
-    __syncthreads();
-    st = part[0];
-    for (int w = 1; w < 4; ++w) stat_join(st, part[w]);
-    if (threadIdx.x == 0) lp_finish(a, row, i, st, a.N);
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < a.k; ++k) {
-        unsigned long long best = 0;
-        for (int c = threadIdx.x; c < a.C; c += 256) {
-            const unsigned long long r = rank_of(Elem<T>::ld(row + c), c);
-            if ((r < last || k == 0) && r > best) best = r;
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const unsigned long long r = __shfl_xor(best, o, 64);
-            best = r > best ? r : best;
-        }
-        __syncthreads();                                               // the previous round's ranks have been read
-        if ((threadIdx.x & 63) == 0) ranks[threadIdx.x >> 6] = best;
+// ------------------------------------------------------------------------------------------------ a team of threads per row
+// A row is cut at the 16-byte boundaries of memory into chunks of EPC classes, the first and the last possibly partial; thread r of
+// the team takes chunks r, r + TEAM, ...  UNROLL of them are in flight and share one change of the maximum.
+//
+// Alternatives: each thread keeps its largest value and the first chunk it stood in.  Ordered by (value, chunk), the k best threads
+// hold the k best classes -- any class of another thread has k before it -- so only their chunks are read again, 1/TEAM of the row
+// each.  What reaches the k-th thread's value is collected and the k best of it taken.  Rows with NaN, and rows where more values tie
+// than the collection holds, go through k rounds over the row.
+#define CAND 512
+#define UNROLL 4
+
+template <int TEAM> struct TeamShared {
+    float m[4], s[4], t[4];
+    u64 key[TEAM], cand[CAND];
+    int winner[ERF_TOP_MAX];
+    int winners, ncand;
+    float least;
+};
+
+template <int TEAM> __device__ __forceinline__ void team_sync() {
+    if (TEAM == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
         __syncthreads();
-        for (int w = 0; w < 4; ++w) best = ranks[w] > best ? ranks[w] : best;
-        last = best;
+    }
+}
+
+// Classes of chunk q of a row whose first class lies `off` classes behind a boundary; what is not part of the row reads -inf
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* row, int off, int C, int q, float* f) {
+    constexpr int E = Elem<T>::EPC;
+    const int c0 = q * E - off;
+    if (c0 >= 0 && c0 + E <= C) {
+        const i32x4 r = *(const i32x4*)(row + c0);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (E == 4) f[e] = __int_as_float(r[e & 3]);
+            else f[e] = (e & 1) ? __uint_as_float((unsigned)r[(e >> 1) & 3] & 0xFFFF0000u) : __uint_as_float((unsigned)r[(e >> 1) & 3] << 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = c0 + e >= 0 && c0 + e < C ? Elem<T>::ld(row + c0 + e) : -INFINITY;
+    }
+}
+
+// Best rank below `last` among the classes of chunks [q0, q1), by the whole team
+template <typename T, int TEAM>
+__device__ __forceinline__ u64 team_round(TeamShared<TEAM>& sh, const T* row, int off, int C, int q0, int q1, int tid, u64 last) {
+    constexpr int E = Elem<T>::EPC;
+    u64 best = 0;
+    const int c1 = min(q1 * E - off, C);
+    for (int c = max(q0 * E - off, 0) + tid; c < c1; c += TEAM) {
+        const u64 r = rank_of(Elem<T>::ld(row + c), c);
+        if (r < last && r > best) best = r;
+    }
+    best = wave_best(best);
+    if (TEAM == 64) return best;
+    __syncthreads();                                                   // the previous round's keys have been read
+    if ((tid & 63) == 0) sh.key[tid >> 6] = best;
+    __syncthreads();
+    best = sh.key[0];
+    for (int w = 1; w < TEAM / 64; ++w) best = sh.key[w] > best ? sh.key[w] : best;
+    return best;
+}
+
+template <typename T, int TEAM, bool TOP>
+__global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
+    constexpr int E = Elem<T>::EPC;
+    __shared__ TeamShared<TEAM> shared[256 / TEAM];
+    const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
+    TeamShared<TEAM>& sh = shared[team];
+    const long long i = (long long)blockIdx.x * (256 / TEAM) + team;
+    if (TEAM == 64 && i >= a.N) return;                                // no barrier of the workgroup below for teams of one wave
+    const T* row = (const T*)a.z + i * a.sn;
+    const int off = (int)(((unsigned long long)row / sizeof(T)) % E);
+    const int chunks = (a.C + off + E - 1) / E, per = (chunks + a.segments - 1) / a.segments;
+    const int seg = blockIdx.y, q0 = min(seg * per, chunks), q1 = min(q0 + per, chunks);
+
+    Stat st{-INFINITY, 0.f, 0.f};
+    float best = -INFINITY;
+    int bestq = -1;
+    for (int q = q0 + tid; q < q1; q += TEAM * UNROLL) {
+        float f[UNROLL][E], cm[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            if (q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
+            else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[u][e] = -INFINITY;
+            }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            cm[u] = f[u][0];
+#pragma unroll
+            for (int e = 1; e < E; ++e) cm[u] = fmaxf(cm[u], f[u][e]);
+            most = fmaxf(most, cm[u]);
+            if (TOP && (cm[u] > best || bestq < 0) && q + u * TEAM < q1) { best = cm[u]; bestq = q + u * TEAM; }
+        }
+        if (most > st.m) stat_move(st, most);
+        const float base = base_of(st.m);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) stat_add(st, base, f[u][e]);
+    }
+    const float wm = wave_largest(st.m);
+    stat_move(st, wm);
+    st.s = wave_total(st.s);
+    st.t = wave_total(st.t);
+    if (TEAM > 64) {
+        if ((tid & 63) == 0) { sh.m[tid >> 6] = st.m; sh.s[tid >> 6] = st.s; sh.t[tid >> 6] = st.t; }
+        __syncthreads();
+        float m = sh.m[0];
+        for (int w = 1; w < TEAM / 64; ++w) m = fmaxf(m, sh.m[w]);
+        Stat sum{m, 0.f, 0.f};
+        for (int w = 0; w < TEAM / 64; ++w) {
+            Stat p{sh.m[w], sh.s[w], sh.t[w]};
+            stat_move(p, m);
+            sum.s += p.s;
+            sum.t += p.t;
+        }
+        st = sum;
+    }
+    const bool whole = a.segments == 1;
+    u64* part = whole ? nullptr : a.parts + (i * a.segments + seg) * (2 + a.k);
+    const float base = base_of(st.m), logs = logf(st.s);
+    if (tid == 0) {
+        if (whole) lp_finish(a, row, i, st, logs);
+        else {
+            part[0] = ((u64)__float_as_uint(st.s) << 32) | __float_as_uint(st.m);
+            part[1] = __float_as_uint(st.t);
+        }
+    }
+    if (!TOP) return;
+
+    auto put = [&](int k, u64 r) {                                     // alternative k, by one thread
+        if (whole) {
+            a.top[i * a.k + k] = (rank_value(r) - base) - logs;
+            a.top_index[i * a.k + k] = rank_index(r);
+        } else {
+            part[2 + k] = r;
+        }
+    };
+    bool slow = st.s != st.s;                                          // the same for the whole team, as all that follows
+    if (!slow) {
+        sh.key[tid] = bestq >= 0 ? rank_of(best, bestq) : 0;
+        if (tid == 0) sh.ncand = 0;
+        team_sync<TEAM>();
+        if (tid < 64) {
+            u64 key[TEAM / 64], last = ~0ull;
+#pragma unroll
+            for (int w = 0; w < TEAM / 64; ++w) key[w] = sh.key[w * 64 + tid];
+            int n = 0;
+            for (; n < a.k; ++n) {
+                u64 r = 0;
+#pragma unroll
+                for (int w = 0; w < TEAM / 64; ++w) r = key[w] < last && key[w] > r ? key[w] : r;
+                r = wave_best(r);
+                if (!r) break;                                         // fewer threads than k have a chunk
+                last = r;
+                if (tid == 0) sh.winner[n] = (int)(rank_index(r) - q0) % TEAM;
+            }
+            if (tid == 0) { sh.winners = n; sh.least = n == a.k ? rank_value(last) : -INFINITY; }
+        }
+        team_sync<TEAM>();
+        const int each = (q1 - q0 + TEAM - 1) / TEAM, winners = sh.winners;
+        const float least = sh.least;
+        for (int p = tid; p < winners * each; p += TEAM) {
+            const int q = q0 + sh.winner[p / each] + p % each * TEAM;
+            if (q >= q1) continue;
+            float f[E];
+            load_chunk(row, off, a.C, q, f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int c = q * E - off + e;
+                if (f[e] >= least && c >= 0 && c < a.C) {
+                    const int at = atomicAdd(&sh.ncand, 1);            // their order has no effect: the ranks decide
+                    if (at < CAND) sh.cand[at] = rank_of(f[e], c);
+                }
+            }
+        }
+        team_sync<TEAM>();
+        const int n = sh.ncand;
+        slow = n > CAND;
+        if (!slow && tid < 64) {
+            u64 last = ~0ull;
+            for (int k = 0; k < a.k; ++k) {
+                u64 r = 0;
+                for (int c = tid; c < n; c += 64) r = sh.cand[c] < last && sh.cand[c] > r ? sh.cand[c] : r;
+                last = wave_best(r);
+                if (tid == 0) put(k, last);
+            }
+        }
+    }
+    if (slow) {
+        u64 last = ~0ull;
+        for (int k = 0; k < a.k; ++k) {
+            last = team_round<T, TEAM>(sh, row, off, a.C, q0, q1, tid, last);
+            if (tid == 0) put(k, last);
+        }
+    }
+}
+
+// The segments of a row joined by one wave
+template <typename T>
+__global__ __launch_bounds__(64) void lp_join_kernel(const LpArgs a) {
+    const long long i = blockIdx.x;
+    const int step = 2 + a.k;
+    const u64* part = a.parts + i * a.segments * step;
+    Stat st{-INFINITY, 0.f, 0.f};
+    for (int g = threadIdx.x; g < a.segments; g += 64) {
+        const u64 ms = part[(long long)g * step];
+        Stat p{__uint_as_float((unsigned)ms), __uint_as_float((unsigned)(ms >> 32)), __uint_as_float((unsigned)part[(long long)g * step + 1])};
+        const float m = fmaxf(p.m, st.m);
+        stat_move(st, m);
+        stat_move(p, m);
+        st.s += p.s;
+        st.t += p.t;
+    }
+    stat_move(st, wave_largest(st.m));
+    st.s = wave_total(st.s);
+    st.t = wave_total(st.t);
+    const float logs = logf(st.s);
+    if (threadIdx.x == 0) lp_finish(a, (const T*)a.z + i * a.sn, i, st, logs);
+    u64 last = ~0ull;
+    const int n = a.segments * a.k;
+    for (int k = 0; k < a.k; ++k) {
+        u64 r = 0;
+        for (int c = threadIdx.x; c < n; c += 64) {
+            const u64 o = part[(long long)(c / a.k) * step + 2 + c % a.k];
+            r = o < last && o > r ? o : r;
+        }
+        last = wave_best(r);
         if (threadIdx.x == 0) {
-            const unsigned j = rank_index(best);
-            a.top[i * a.k + k] = (Elem<T>::ld(row + j) - base_of(st.m)) - logf(st.s);
-            a.top_index[i * a.k + k] = j;
+            a.top[i * a.k + k] = (rank_value(last) - base_of(st.m)) - logs;
+            a.top_index[i * a.k + k] = rank_index(last);
         }
     }
 }
@@ -189,9 +410,9 @@ __global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdArgs a) {
 }
 
 static inline bool lp_shape_ok(int dtype, long long N, int C, long long L, long long sn, long long sc, int k) {
-    if ((dtype != ERF_F32 && dtype != ERF_BF16) || N <= 0 || C <= 0 || L <= 0 || sn < 0 || k < 0 || k > C || k > ERF_TOP_MAX) return false;
+    if ((dtype != ERF_F32 && dtype != ERF_BF16) || N <= 0 || C <= 0 || C > (1 << 28) || L <= 0 || sn < 0 || k < 0 || k > C || k > ERF_TOP_MAX) return false;
     if (N > 0x7FFFFFFFll || L > 0x7FFFFFFFll || N * L > (1ll << 40)) return false;
-    return (sc == 1 && L == 1) || (sc >= L);
+    return (sc == 1 && L == 1) || (sc >= L && sc >= 2);
 }
 
 static inline unsigned lp_grid(long long total) {
@@ -199,22 +420,48 @@ static inline unsigned lp_grid(long long total) {
     return (unsigned)(g > 65536 ? 65536 : g);
 }
 
+// Rows of more classes than a thread walks through by itself are taken by teams: a wave, or a workgroup where that gives each of its
+// threads a full set of loads; few rows of very many classes are split so that about 1024 workgroups have work.
+#define POSITION_CLASSES 64
+static inline int lp_epc(int dtype) { return dtype == ERF_BF16 ? 8 : 4; }
+static inline bool lp_wave_rows(int dtype, int C) { return C <= 64 * UNROLL * lp_epc(dtype); }
+static inline int lp_segments(int dtype, long long N, int C) {
+    if (lp_wave_rows(dtype, C)) return 1;
+    const long long most = ((long long)C + 256 * UNROLL * lp_epc(dtype) - 1) / (256 * UNROLL * lp_epc(dtype)), want = (1024 + N - 1) / N;
+    return (int)(want < most ? want : most);
+}
+
+template <typename T, bool TOP>
+static void lp_rows_launch(const LpArgs& a, int dtype, hipStream_t s) {
+    if (lp_wave_rows(dtype, a.C)) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), dim3((unsigned)((a.N + 3) / 4)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), dim3((unsigned)a.N, (unsigned)a.segments), dim3(256), 0, s, a);
+    if (a.segments > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)a.N), dim3(64), 0, s, a);
+}
+
 extern "C" {
+
+size_t erf_class_log_probs_workspace_bytes(int dtype, long long N, int C, long long L, long long stride_c, int top_k) {
+    if (!lp_shape_ok(dtype, N, C, L, 0, stride_c, top_k) || stride_c != 1 || C <= POSITION_CLASSES) return 0;
+    const int segments = lp_segments(dtype, N, C);
+    return segments > 1 ? (size_t)N * segments * (2 + top_k) * sizeof(u64) : 0;
+}
 
 int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, long long L, long long stride_n, long long stride_c,
                             const long long* target, long long ignore_index, float* log_prob, float* entropy, float* stats, int top_k,
-                            float* top_log_probs, long long* top_indices, void* stream) {
+                            float* top_log_probs, long long* top_indices, void* workspace, void* stream) {
     if (!logits || !entropy || !stats || (!target != !log_prob) || !lp_shape_ok(dtype, N, C, L, stride_n, stride_c, top_k) ||
-        (top_k && (!top_log_probs || !top_indices)))
+        (top_k && (!top_log_probs || !top_indices)) ||
+        (!workspace && erf_class_log_probs_workspace_bytes(dtype, N, C, L, stride_c, top_k)))
         return ERF_EINVAL;
-    const LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices};
+    LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, (u64*)workspace};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && L == 1) {
-        if (dtype == ERF_BF16) hipLaunchKernelGGL(lp_rows_kernel<bf16raw>, dim3((unsigned)N), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(lp_rows_kernel<float>, dim3((unsigned)N), dim3(256), 0, s, a);
+    if (stride_c == 1 && C > POSITION_CLASSES) {
+        a.segments = lp_segments(dtype, N, C);
+        if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
+        else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
     } else {
-        if (dtype == ERF_BF16) hipLaunchKernelGGL(lp_planes_kernel<bf16raw>, dim3(lp_grid(N * L)), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(lp_planes_kernel<float>, dim3(lp_grid(N * L)), dim3(256), 0, s, a);
+        if (dtype == ERF_BF16) hipLaunchKernelGGL(lp_position_kernel<bf16raw>, dim3(lp_grid(N * L)), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(lp_position_kernel<float>, dim3(lp_grid(N * L)), dim3(256), 0, s, a);
     }
     return erf_check_launch();
 }

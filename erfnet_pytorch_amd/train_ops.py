@@ -121,9 +121,11 @@ def class_log_probs_fwd(logits, target, top_k=0, ignore_index=-100):
     top, index = new(top_shape, dtype=torch.float32), new(top_shape, dtype=torch.int64)
     if entropy.numel():
         with on_device_of(z):
+            nbytes = size_query("erf_class_log_probs_workspace_bytes", code, n, c, length, sc, top_k)
+            ws = new(nbytes, dtype=torch.uint8) if nbytes else None
             call("erf_class_log_probs_fwd", z.data_ptr(), code, n, c, length, sn, sc, _p(target), ignore_index,
                  log_prob.data_ptr() if target is not None else 0, entropy.data_ptr(), stats.data_ptr(), top_k, top.data_ptr() if top_k else 0,
-                 index.data_ptr() if top_k else 0, _stream())
+                 index.data_ptr() if top_k else 0, _p(ws), _stream())
     if order is not None and top_k:
         top, index = top.permute(order), index.permute(order)
     elif not top_k:

@@ -259,9 +259,12 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
  * bwd: dlogits (same type, own strides, same kind of layout) = gl ([j = t] - p) - gh p (log p + entropy) + sum_k gk ([j = i_k] - p);
  *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits hold. */
 #define ERF_TOP_MAX 32
+/* workspace of fwd: erf_class_log_probs_workspace_bytes (0: none needed, NULL is fine), 16-byte aligned, not shared by calls that may
+ * overlap; it need not be cleared. */
+size_t erf_class_log_probs_workspace_bytes(int dtype, long long N, int C, long long L, long long stride_c, int top_k);
 int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, long long L, long long stride_n, long long stride_c,
                             const long long* target, long long ignore_index, float* log_prob, float* entropy, float* stats, int top_k,
-                            float* top_log_probs, long long* top_indices, void* stream);
+                            float* top_log_probs, long long* top_indices, void* workspace, void* stream);
 int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, long long L, long long stride_n, long long stride_c,
                             const long long* target, long long ignore_index, const float* stats, const float* entropy,
                             const float* g_log_prob, const float* g_entropy, int top_k, const long long* top_indices, const float* g_top,

@@ -389,11 +389,13 @@ def test_wrong_arguments_are_refused():
 
 def test_abi_refuses_bad_arguments_without_a_gpu():
     from erfnet_pytorch_amd import _lib
-    good = [16, 0, 4, 5, 1, 5, 1, 16, -100, 16, 16, 16, 2, 16, 16, 0]
+    good = [16, 0, 4, 5, 1, 5, 1, 16, -100, 16, 16, 16, 2, 16, 16, 0, 0]
     for i, bad in ((0, 0), (1, 2), (2, 0), (3, 0), (4, 0), (5, -1), (6, 0), (7, 0), (9, 0), (10, 0), (11, 0), (12, 6), (12, -1), (13, 0), (14, 0)):
         args = list(good)
         args[i] = bad
         assert _lib.query("erf_class_log_probs_fwd", *args) == -1, i
+    assert _lib.query("erf_class_log_probs_workspace_bytes", 1, 1, 200000, 1, 1, 4) > 0
+    assert _lib.query("erf_class_log_probs_fwd", 16, 1, 1, 200000, 1, 200000, 1, 16, -100, 16, 16, 16, 2, 16, 16, 0, 0) == -1      # no workspace
     good = [16, 0, 4, 5, 6, 30, 6, 16, -100, 16, 16, 16, 16, 2, 16, 16, 16, 30, 6, 0]
     for i, bad in ((0, 0), (1, 2), (2, 0), (3, 0), (4, 0), (6, 5), (6, 1), (7, 0), (9, 0), (10, 0), (13, 33), (14, 0), (16, 0), (17, -1), (18, 5), (18, 1)):
         args = list(good)
