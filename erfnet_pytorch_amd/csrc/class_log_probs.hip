@@ -94,31 +94,127 @@ __device__ __forceinline__ void lp_finish(const LpArgs& a, const T* row, long lo
 }
 
 // ------------------------------------------------------------------------------------------------ one thread per position
-// Planes, and rows of few classes.  The alternatives by k rounds over the classes.
-template <typename T>
+// Planes, and rows of few classes.  A thread takes P neighbouring positions (P > 1: planes, whole vectors) and BATCH classes at a
+// time, all of whose loads are in flight together and which share one change of the maximum.  Up to KT alternatives are kept in
+// registers, sorted; more (KT < 0) are found by rounds over the classes, as they are where NaN or too few finite values upset the order.
+#define BATCH 8
+
+template <typename T, int P>
+__device__ __forceinline__ void load_positions(const T* p, float* f) {
+    if constexpr (P == 1) f[0] = Elem<T>::ld(p);
+    else if constexpr (sizeof(T) * P == 16) {
+        const f32x4 v = *(const f32x4*)p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = v[i];
+    } else if constexpr (sizeof(T) == 4) {
+        const f32x2 v = *(const f32x2*)p;
+        f[0] = v[0]; f[1] = v[1];
+    } else if constexpr (P == 4) {
+        const i32x2 r = *(const i32x2*)p;
+        f[0] = __uint_as_float((unsigned)r[0] << 16); f[1] = __uint_as_float((unsigned)r[0] & 0xFFFF0000u);
+        f[2] = __uint_as_float((unsigned)r[1] << 16); f[3] = __uint_as_float((unsigned)r[1] & 0xFFFF0000u);
+    } else {
+        const unsigned r = *(const unsigned*)p;
+        f[0] = __uint_as_float(r << 16); f[1] = __uint_as_float(r & 0xFFFF0000u);
+    }
+}
+
+template <typename T, int P>
+__device__ __forceinline__ void store_positions(T* p, const float* f) {
+    if constexpr (P == 1) Elem<T>::st(p, f[0]);
+    else if constexpr (sizeof(T) * P == 16) *(f32x4*)p = f32x4{f[0], f[1], f[2], f[3]};
+    else if constexpr (sizeof(T) == 4) *(f32x2*)p = f32x2{f[0], f[1]};
+    else if constexpr (P == 4) *(i32x2*)p = pack_bf16x4(f32x4{f[0], f[1], f[2], f[3]});
+    else *(int*)p = pack_bf16x2(f[0], f[1]);
+}
+
+// image and place in the image of position i: one division, of 32 bits where that does
+__device__ __forceinline__ void split_position(long long i, long long L, long long& n, long long& l) {
+    if (L == 1) { n = i; l = 0; }
+    else if (i <= 0xFFFFFFFFll) { n = (unsigned)i / (unsigned)L; l = i - n * L; }
+    else { n = i / L; l = i - n * L; }
+}
+
+template <typename T, int P, int KT>
 __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
+    constexpr int K = KT > 0 ? KT : 1;
     const long long rows = a.N * a.L;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows; i += (long long)gridDim.x * 256) {
-        const long long n = i / a.L, l = i % a.L;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * P; i < rows; i += (long long)gridDim.x * 256 * P) {
+        long long n, l;
+        split_position(i, a.L, n, l);
         const T* row = (const T*)a.z + n * a.sn + l;
-        Stat st{-INFINITY, 0.f, 0.f};
-        for (int c = 0; c < a.C; ++c) {
-            const float z = Elem<T>::ld(row + c * a.sc);
-            if (z > st.m) stat_move(st, z);
-            stat_add(st, base_of(st.m), z);
+        Stat st[P];
+        float tv[P][K];
+        int tc[P][K];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            st[p] = Stat{-INFINITY, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < K; ++k) { tv[p][k] = -INFINITY; tc[p][k] = -1; }
         }
-        const float logs = logf(st.s);
-        lp_finish(a, row, i, st, logs);
-        u64 last = ~0ull;
-        for (int k = 0; k < a.k; ++k) {
-            u64 best = 0;
-            for (int c = 0; c < a.C; ++c) {
-                const u64 r = rank_of(Elem<T>::ld(row + c * a.sc), c);
-                if ((r < last || k == 0) && r > best) best = r;
+        for (int c0 = 0; c0 < a.C; c0 += BATCH) {
+            float f[BATCH][P];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (c0 + b < a.C) load_positions<T, P>(row + (c0 + b) * a.sc, f[b]);
+                else {
+#pragma unroll
+                    for (int p = 0; p < P; ++p) f[b][p] = -INFINITY;
+                }
             }
-            last = best;
-            a.top[(n * a.k + k) * a.L + l] = (rank_value(best) - base_of(st.m)) - logs;
-            a.top_index[(n * a.k + k) * a.L + l] = rank_index(best);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                float most = f[0][p];
+#pragma unroll
+                for (int b = 1; b < BATCH; ++b) most = fmaxf(most, f[b][p]);
+                if (most > st[p].m) stat_move(st[p], most);
+                const float base = base_of(st[p].m);
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b) {
+                    stat_add(st[p], base, f[b][p]);
+                    if (KT > 0) {
+                        const float z = f[b][p];
+                        bool up[K];                                    // slots that are sorted behind z; equal values stay before it
+#pragma unroll
+                        for (int k = 0; k < K; ++k) up[k] = z > tv[p][k];
+#pragma unroll
+                        for (int k = K - 1; k >= 0; --k) {
+                            const bool from_above = k > 0 && up[k > 0 ? k - 1 : 0];
+                            tv[p][k] = from_above ? tv[p][k > 0 ? k - 1 : 0] : up[k] ? z : tv[p][k];
+                            tc[p][k] = from_above ? tc[p][k > 0 ? k - 1 : 0] : up[k] ? c0 + b : tc[p][k];
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const float logs = logf(st[p].s), base = base_of(st[p].m);
+            lp_finish(a, row + p, i + p, st[p], logs);
+            if (KT == 0) continue;
+            bool rounds = KT < 0 || logs != logs;
+#pragma unroll
+            for (int k = 0; k < K; ++k) rounds = rounds || (k < a.k && tc[p][k] < 0);
+            if (!rounds) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k < a.k) {
+                        a.top[(n * a.k + k) * a.L + l + p] = (tv[p][k] - base) - logs;
+                        a.top_index[(n * a.k + k) * a.L + l + p] = tc[p][k];
+                    }
+                continue;
+            }
+            u64 last = ~0ull;
+            for (int k = 0; k < a.k; ++k) {
+                u64 best = 0;
+                for (int c = 0; c < a.C; ++c) {
+                    const u64 r = rank_of(Elem<T>::ld(row + p + c * a.sc), c);
+                    best = r < last && r > best ? r : best;
+                }
+                last = best;
+                a.top[(n * a.k + k) * a.L + l + p] = (rank_value(best) - base) - logs;
+                a.top_index[(n * a.k + k) * a.L + l + p] = rank_index(best);
+            }
         }
     }
 }
@@ -377,35 +473,138 @@ struct LpBwdArgs {
     void* dz;
 };
 
-// One element per thread; rows whose gradients are all 0 get 0 whatever their logits hold
-template <typename T>
-__global__ __launch_bounds__(256) void lp_bwd_kernel(const LpBwdArgs a) {
-    const long long rows = a.N * a.L, total = rows * a.C;
-    const bool planes = a.sc != 1;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-        long long n, l, c;
-        if (planes) { l = e % a.L; c = e / a.L % a.C; n = e / a.L / a.C; }
-        else { l = 0; c = e % a.C; n = e / a.C; }
-        const long long i = n * a.L + l;
-        const long long t = a.g_log_prob ? a.target[i] : a.ignore;
-        const float gl = t == a.ignore ? 0.f : t >= 0 && t < a.C ? a.g_log_prob[i] : __builtin_nanf("");
-        const float gh = a.g_entropy ? a.g_entropy[i] : 0.f;
-        float pull = gl, own = c == t ? gl : 0.f;
-        bool any = gl != 0.f || gh != 0.f;
-        for (int k = 0; k < a.k && a.g_top; ++k) {
-            const long long at = (n * a.k + k) * a.L + l;
-            const float gk = a.g_top[at];
-            any = any || gk != 0.f;
+// What a position's gradient takes besides the logits.  dz_j = -p_j (pull + gh (log p_j + H)) for every class, and the target and the
+// alternatives get their own terms added; a position whose gradients are all 0 gets 0 whatever its logits hold.
+struct LpPull {
+    float base, logs, a, gh, gl;       // a = pull + gh H
+    long long t;
+    bool any;
+};
+__device__ __forceinline__ LpPull lp_pull(const LpBwdArgs& a, long long n, long long l) {
+    const long long i = n * a.L + l;
+    LpPull q;
+    q.t = a.g_log_prob ? a.target[i] : a.ignore;
+    q.gl = q.t == a.ignore ? 0.f : q.t >= 0 && q.t < a.C ? a.g_log_prob[i] : __builtin_nanf("");
+    q.gh = a.g_entropy ? a.g_entropy[i] : 0.f;
+    q.any = q.gl != 0.f || q.gh != 0.f;
+    float pull = q.gl;
+    if (a.g_top)
+        for (int k = 0; k < a.k; ++k) {
+            const float gk = a.g_top[(n * a.k + k) * a.L + l];
+            q.any = q.any || gk != 0.f;
             pull += gk;
-            if (a.top_index[at] == c) own += gk;
         }
-        float d = 0.f;
-        if (any) {
-            const float lp = (Elem<T>::ld((const T*)a.z + n * a.sn + c * a.sc + l) - a.stats[i]) - a.stats[rows + i];
-            const float p = exp2f(lp * LOG2E);
-            d = own - p * (pull + (gh != 0.f ? gh * (fmaxf(lp, -200.f) + a.entropy[i]) : 0.f));
+    q.base = a.stats[i];
+    q.logs = a.stats[a.N * a.L + i];
+    q.a = q.gh != 0.f ? fmaf(q.gh, a.entropy[i], pull) : pull;
+    return q;
+}
+__device__ __forceinline__ float lp_grad(const LpPull& q, float z) {
+    const float lp = (z - q.base) - q.logs;
+    return -__builtin_amdgcn_exp2f(lp * LOG2E) * fmaf(q.gh, fmaxf(lp, -200.f), q.a);          // p = 0: 0 * -inf
+}
+// own term of class j: its share as the target and as each alternative
+__device__ __forceinline__ float lp_own(const LpBwdArgs& a, const LpPull& q, long long n, long long l, long long j) {
+    float own = j == q.t ? q.gl : 0.f;
+    for (int k = 0; k < a.k; ++k) {
+        const long long at = (n * a.k + k) * a.L + l;
+        if (a.top_index[at] == j) own += a.g_top[at];
+    }
+    return own;
+}
+
+// One thread per P positions, as in the forward pass.  The target's term is added on the way; classes that are alternatives are
+// written once more.
+template <typename T, int P>
+__global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a) {
+    const long long rows = a.N * a.L;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * P; i < rows; i += (long long)gridDim.x * 256 * P) {
+        long long n, l;
+        split_position(i, a.L, n, l);
+        const T* row = (const T*)a.z + n * a.sn + l;
+        T* out = (T*)a.dz + n * a.dn + l;
+        LpPull q[P];
+        bool any = false;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            q[p] = lp_pull(a, n, l + p);
+            any = any || q[p].any;
         }
-        Elem<T>::st((T*)a.dz + n * a.dn + c * a.dc + l, d);
+        for (int c0 = 0; c0 < a.C; c0 += BATCH) {
+            float f[BATCH][P];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (any && c0 + b < a.C) load_positions<T, P>(row + (c0 + b) * a.sc, f[b]);
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (c0 + b < a.C) {
+                    float d[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) d[p] = q[p].any ? lp_grad(q[p], f[b][p]) + ((int)q[p].t == c0 + b ? q[p].gl : 0.f) : 0.f;
+                    store_positions<T, P>(out + (c0 + b) * a.dc, d);
+                }
+        }
+        if (!a.g_top) continue;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            if (!q[p].any) continue;
+            for (int k = 0; k < a.k; ++k) {
+                const long long j = a.top_index[(n * a.k + k) * a.L + l + p];
+                Elem<T>::st(out + p + j * a.dc, lp_grad(q[p], Elem<T>::ld(row + p + j * a.sc)) + lp_own(a, q[p], n, l + p, j));
+            }
+        }
+    }
+}
+
+// Rows by teams: chunks at the 16-byte boundaries as in the forward pass; the target and the alternatives are written once more
+// after the rest.  A gradient row that lies differently to the boundaries than the logits' row is stored class by class.
+#define BWD_UNROLL 4
+template <typename T, int TEAM>
+__global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
+    constexpr int E = Elem<T>::EPC;
+    const int tid = threadIdx.x % TEAM;
+    const long long i = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    if (TEAM == 64 && i >= a.N) return;                                // no barrier of the workgroup below for teams of one wave
+    const T* row = (const T*)a.z + i * a.sn;
+    T* out = (T*)a.dz + i * a.dn;
+    const int off = (int)(((unsigned long long)row / sizeof(T)) % E), dist = (int)(((unsigned long long)out / sizeof(T)) % E);
+    const int chunks = (a.C + off + E - 1) / E, q0 = blockIdx.y * TEAM * BWD_UNROLL, q1 = TEAM == 64 ? chunks : min(q0 + TEAM * BWD_UNROLL, chunks);
+    const LpPull pull = lp_pull(a, i, 0);
+    for (int q = q0 + tid; q < q1; q += TEAM * BWD_UNROLL) {
+        float f[BWD_UNROLL][E];
+#pragma unroll
+        for (int u = 0; u < BWD_UNROLL; ++u)
+            if (pull.any && q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
+#pragma unroll
+        for (int u = 0; u < BWD_UNROLL; ++u) {
+            if (q + u * TEAM >= q1) break;
+            const int c0 = (q + u * TEAM) * E - off;
+            float d[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) d[e] = pull.any ? lp_grad(pull, f[u][e]) : 0.f;
+            if (c0 >= 0 && c0 + E <= a.C && off == dist) {
+                if constexpr (E == 4) *(f32x4*)(out + c0) = f32x4{d[0], d[1], d[2], d[3]};
+                else *(i32x4*)(out + c0) = i32x4{pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]), pack_bf16x2(d[6], d[7])};
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (c0 + e >= 0 && c0 + e < a.C) Elem<T>::st(out + c0 + e, d[e]);
+            }
+        }
+    }
+    if (!pull.any) return;                                             // the same for the whole team
+    if (TEAM == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();                                               // the stores above are done before a class is written again
+    }
+    const int own = 1 + (a.g_top ? a.k : 0);
+    if (tid < own) {
+        const long long j = tid ? a.top_index[i * a.k + tid - 1] : pull.t;
+        const long long c = j + off;
+        if (j >= 0 && j < a.C && c >= (long long)q0 * E && c < (long long)q1 * E)
+            Elem<T>::st(out + j, lp_grad(pull, Elem<T>::ld(row + j)) + lp_own(a, pull, i, 0, j));
     }
 }
 
@@ -418,6 +617,12 @@ static inline bool lp_shape_ok(int dtype, long long N, int C, long long L, long 
 static inline unsigned lp_grid(long long total) {
     const long long g = (total + 255) / 256;
     return (unsigned)(g > 65536 ? 65536 : g);
+}
+
+// Positions per thread: 4 where whole vectors lie on their boundaries and enough threads are left to fill the chip
+static inline int lp_positions(int dtype, long long N, long long L, long long sc, unsigned long long addresses, unsigned long long strides) {
+    const int size = dtype == ERF_BF16 ? 2 : 4;
+    return sc != 1 && L % 4 == 0 && strides % 4 == 0 && addresses % (4 * size) == 0 && N * L >= (1ll << 19) ? 4 : 1;
 }
 
 // Rows of more classes than a thread walks through by itself are taken by teams: a wave, or a workgroup where that gives each of its
@@ -460,8 +665,19 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
         else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
     } else {
-        if (dtype == ERF_BF16) hipLaunchKernelGGL(lp_position_kernel<bf16raw>, dim3(lp_grid(N * L)), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(lp_position_kernel<float>, dim3(lp_grid(N * L)), dim3(256), 0, s, a);
+        const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits, (unsigned long long)(stride_n | stride_c));
+        const dim3 grid(lp_grid(N * L / p)), block(256);
+#define LP_KT(T, P)                                                                                          \
+    do {                                                                                                     \
+        if (top_k == 0) hipLaunchKernelGGL((lp_position_kernel<T, P, 0>), grid, block, 0, s, a);             \
+        else if (top_k == 1) hipLaunchKernelGGL((lp_position_kernel<T, P, 1>), grid, block, 0, s, a);        \
+        else if (top_k == 2) hipLaunchKernelGGL((lp_position_kernel<T, P, 2>), grid, block, 0, s, a);        \
+        else if (top_k <= 4) hipLaunchKernelGGL((lp_position_kernel<T, P, 4>), grid, block, 0, s, a);        \
+        else hipLaunchKernelGGL((lp_position_kernel<T, P, -1>), grid, block, 0, s, a);                       \
+    } while (0)
+        if (dtype == ERF_BF16) { if (p == 4) LP_KT(bf16raw, 4); else LP_KT(bf16raw, 1); }
+        else { if (p == 4) LP_KT(float, 4); else LP_KT(float, 1); }
+#undef LP_KT
     }
     return erf_check_launch();
 }
@@ -475,9 +691,31 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
         return ERF_EINVAL;
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
                       g_log_prob, g_entropy, g_top, top_indices, dlogits};
-    const unsigned g = lp_grid(N * L * C);
-    if (dtype == ERF_BF16) hipLaunchKernelGGL(lp_bwd_kernel<bf16raw>, dim3(g), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(lp_bwd_kernel<float>, dim3(g), dim3(256), 0, (hipStream_t)stream, a);
+    hipStream_t s = (hipStream_t)stream;
+    if (stride_c == 1 && C > POSITION_CLASSES) {
+        const int per = 256 * BWD_UNROLL * lp_epc(dtype);
+        const bool wave = lp_wave_rows(dtype, C);
+        // one chunk more than C / EPC where a row starts off the boundaries
+        const dim3 grid(wave ? (unsigned)((N + 3) / 4) : (unsigned)N, wave ? 1u : (unsigned)((C + lp_epc(dtype) - 1 + per - 1) / per)), block(256);
+        if (dtype == ERF_BF16) {
+            if (wave) hipLaunchKernelGGL((lp_rows_bwd_kernel<bf16raw, 64>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((lp_rows_bwd_kernel<bf16raw, 256>), grid, block, 0, s, a);
+        } else {
+            if (wave) hipLaunchKernelGGL((lp_rows_bwd_kernel<float, 64>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((lp_rows_bwd_kernel<float, 256>), grid, block, 0, s, a);
+        }
+    } else {
+        const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits | (unsigned long long)dlogits,
+                                   (unsigned long long)(stride_n | stride_c | dstride_n | dstride_c));
+        const dim3 grid(lp_grid(N * L / p)), block(256);
+        if (dtype == ERF_BF16) {
+            if (p == 4) hipLaunchKernelGGL((lp_position_bwd_kernel<bf16raw, 4>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((lp_position_bwd_kernel<bf16raw, 1>), grid, block, 0, s, a);
+        } else {
+            if (p == 4) hipLaunchKernelGGL((lp_position_bwd_kernel<float, 4>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((lp_position_bwd_kernel<float, 1>), grid, block, 0, s, a);
+        }
+    }
     return erf_check_launch();
 }
 
