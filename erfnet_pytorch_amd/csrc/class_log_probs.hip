@@ -128,6 +128,25 @@ __device__ __forceinline__ void store_positions(T* p, const float* f) {
     else *(int*)p = pack_bf16x2(f[0], f[1]);
 }
 
+template <int P>
+__device__ __forceinline__ void load_indices(const long long* p, int* t) {         // classes fit 32 bits; others become -1
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const long long v = p[i];
+        t[i] = v >= 0 && v <= 0x7FFFFFFF ? (int)v : -1;
+    }
+}
+template <int P>
+__device__ __forceinline__ void store_indices(long long* p, const int* t) {
+    if constexpr (P == 4) {
+        *(i32x4*)p = i32x4{t[0], t[0] >> 31, t[1], t[1] >> 31};
+        *(i32x4*)(p + 2) = i32x4{t[2], t[2] >> 31, t[3], t[3] >> 31};
+    } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) p[i] = t[i];
+    }
+}
+
 // image and place in the image of position i: one division, of 32 bits where that does
 __device__ __forceinline__ void split_position(long long i, long long L, long long& n, long long& l) {
     if (L == 1) { n = i; l = 0; }
@@ -144,11 +163,20 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
         split_position(i, a.L, n, l);
         const T* row = (const T*)a.z + n * a.sn + l;
         Stat st[P];
-        float tv[P][K];
-        int tc[P][K];
+        float tv[P][K], zt[P];
+        int tc[P][K], t[P], ignored = 0;
+        if (a.log_prob) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const long long v = a.target[i + p];
+                t[p] = v >= 0 && v < a.C ? (int)v : -1;
+                ignored |= (v == a.ignore) << p;
+            }
+        }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             st[p] = Stat{-INFINITY, 0.f, 0.f};
+            zt[p] = __builtin_nanf("");                                // a target outside [0, C): as in the weighted cross entropy
 #pragma unroll
             for (int k = 0; k < K; ++k) { tv[p][k] = -INFINITY; tc[p][k] = -1; }
         }
@@ -172,6 +200,7 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b) {
                     stat_add(st[p], base, f[b][p]);
+                    if (a.log_prob) zt[p] = t[p] == c0 + b ? f[b][p] : zt[p];
                     if (KT > 0) {
                         const float z = f[b][p];
                         bool up[K];                                    // slots that are sorted behind z; equal values stay before it
@@ -187,23 +216,44 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
                 }
             }
         }
+        float logs[P], base[P], v[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const float logs = logf(st[p].s), base = base_of(st[p].m);
-            lp_finish(a, row + p, i + p, st[p], logs);
-            if (KT == 0) continue;
-            bool rounds = KT < 0 || logs != logs;
+            logs[p] = logf(st[p].s);
+            base[p] = base_of(st[p].m);
+        }
+        if (a.log_prob) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) v[p] = ignored >> p & 1 ? 0.f : (zt[p] - base[p]) - logs[p];
+            store_positions<float, P>(a.log_prob + i, v);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) v[p] = logs[p] - st[p].t * LN2 / st[p].s;
+        store_positions<float, P>(a.entropy + i, v);
+        store_positions<float, P>(a.stats + i, base);
+        store_positions<float, P>(a.stats + rows + i, logs);
+        if (KT == 0) continue;
+        bool rounds = KT < 0;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            rounds = rounds || logs[p] != logs[p];
 #pragma unroll
             for (int k = 0; k < K; ++k) rounds = rounds || (k < a.k && tc[p][k] < 0);
-            if (!rounds) {
+        }
+        if (!rounds) {
 #pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k < a.k) {
-                        a.top[(n * a.k + k) * a.L + l + p] = (tv[p][k] - base) - logs;
-                        a.top_index[(n * a.k + k) * a.L + l + p] = tc[p][k];
-                    }
-                continue;
-            }
+            for (int k = 0; k < K; ++k)
+                if (k < a.k) {
+                    int j[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) { v[p] = (tv[p][k] - base[p]) - logs[p]; j[p] = tc[p][k]; }
+                    store_positions<float, P>(a.top + (n * a.k + k) * a.L + l, v);
+                    store_indices<P>(a.top_index + (n * a.k + k) * a.L + l, j);
+                }
+            continue;
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
             u64 last = ~0ull;
             for (int k = 0; k < a.k; ++k) {
                 u64 best = 0;
@@ -212,7 +262,7 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
                     best = r < last && r > best ? r : best;
                 }
                 last = best;
-                a.top[(n * a.k + k) * a.L + l + p] = (rank_value(best) - base) - logs;
+                a.top[(n * a.k + k) * a.L + l + p] = (rank_value(best) - base[p]) - logs[p];
                 a.top_index[(n * a.k + k) * a.L + l + p] = rank_index(best);
             }
         }
@@ -473,84 +523,108 @@ struct LpBwdArgs {
     void* dz;
 };
 
-// What a position's gradient takes besides the logits.  dz_j = -p_j (pull + gh (log p_j + H)) for every class, and the target and the
-// alternatives get their own terms added; a position whose gradients are all 0 gets 0 whatever its logits hold.
-struct LpPull {
-    float base, logs, a, gh, gl;       // a = pull + gh H
-    long long t;
-    bool any;
-};
-__device__ __forceinline__ LpPull lp_pull(const LpBwdArgs& a, long long n, long long l) {
-    const long long i = n * a.L + l;
-    LpPull q;
-    q.t = a.g_log_prob ? a.target[i] : a.ignore;
-    q.gl = q.t == a.ignore ? 0.f : q.t >= 0 && q.t < a.C ? a.g_log_prob[i] : __builtin_nanf("");
-    q.gh = a.g_entropy ? a.g_entropy[i] : 0.f;
-    q.any = q.gl != 0.f || q.gh != 0.f;
-    float pull = q.gl;
-    if (a.g_top)
-        for (int k = 0; k < a.k; ++k) {
-            const float gk = a.g_top[(n * a.k + k) * a.L + l];
-            q.any = q.any || gk != 0.f;
-            pull += gk;
-        }
-    q.base = a.stats[i];
-    q.logs = a.stats[a.N * a.L + i];
-    q.a = q.gh != 0.f ? fmaf(q.gh, a.entropy[i], pull) : pull;
-    return q;
-}
-__device__ __forceinline__ float lp_grad(const LpPull& q, float z) {
-    const float lp = (z - q.base) - q.logs;
-    return -__builtin_amdgcn_exp2f(lp * LOG2E) * fmaf(q.gh, fmaxf(lp, -200.f), q.a);          // p = 0: 0 * -inf
-}
-// own term of class j: its share as the target and as each alternative
-__device__ __forceinline__ float lp_own(const LpBwdArgs& a, const LpPull& q, long long n, long long l, long long j) {
-    float own = j == q.t ? q.gl : 0.f;
-    for (int k = 0; k < a.k; ++k) {
-        const long long at = (n * a.k + k) * a.L + l;
-        if (a.top_index[at] == j) own += a.g_top[at];
-    }
-    return own;
+// dz_j = -p_j (pull + gh log p_j) for every class, pull = gl + sum gk + gh H; the target and the alternatives get their own terms
+// added.  A position whose gradients are all 0 gets 0 whatever its logits hold.
+__device__ __forceinline__ float lp_grad(float z, float base, float logs, float gh, float pull) {
+    const float lp = (z - base) - logs;
+    return -__builtin_amdgcn_exp2f(lp * LOG2E) * fmaf(gh, fmaxf(lp, -200.f), pull);          // p = 0: 0 * -inf
 }
 
-// One thread per P positions, as in the forward pass.  The target's term is added on the way; classes that are alternatives are
-// written once more.
-template <typename T, int P>
+// One thread per P positions, as in the forward pass.  The target's term and those of up to KT alternatives are added on the way;
+// where there are more (KT < 0), the classes that are alternatives are written once more.
+template <typename T, int P, int KT>
 __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a) {
+    constexpr int K = KT > 0 ? KT : 1;
     const long long rows = a.N * a.L;
     for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * P; i < rows; i += (long long)gridDim.x * 256 * P) {
         long long n, l;
         split_position(i, a.L, n, l);
         const T* row = (const T*)a.z + n * a.sn + l;
         T* out = (T*)a.dz + n * a.dn + l;
-        LpPull q[P];
-        bool any = false;
+        float gl[P], gh[P], pull[P], base[P], logs[P], gk[K][P];
+        int t[P], jk[K][P];
+        bool any[P], some = false;
+#pragma unroll
+        for (int p = 0; p < P; ++p) { gl[p] = gh[p] = 0.f; t[p] = -1; }
+        if (a.g_log_prob) {
+            load_positions<float, P>(a.g_log_prob + i, gl);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const long long v = a.target[i + p];
+                t[p] = v >= 0 && v < a.C ? (int)v : -1;
+                gl[p] = v == a.ignore ? 0.f : t[p] >= 0 ? gl[p] : __builtin_nanf("");
+            }
+        }
+        if (a.g_entropy) load_positions<float, P>(a.g_entropy + i, gh);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            q[p] = lp_pull(a, n, l + p);
-            any = any || q[p].any;
+            pull[p] = gl[p];
+            any[p] = gl[p] != 0.f || gh[p] != 0.f;
         }
+        if (KT > 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int p = 0; p < P; ++p) { gk[k][p] = 0.f; jk[k][p] = -1; }
+                if (k < a.k) {
+                    load_positions<float, P>(a.g_top + (n * a.k + k) * a.L + l, gk[k]);
+                    load_indices<P>(a.top_index + (n * a.k + k) * a.L + l, jk[k]);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) { pull[p] += gk[k][p]; any[p] = any[p] || gk[k][p] != 0.f; }
+                }
+            }
+        }
+        if (KT < 0)
+            for (int k = 0; k < a.k; ++k)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const float g = a.g_top[(n * a.k + k) * a.L + l + p];
+                    pull[p] += g;
+                    any[p] = any[p] || g != 0.f;
+                }
+        load_positions<float, P>(a.stats + i, base);
+        load_positions<float, P>(a.stats + rows + i, logs);
+        if (a.g_entropy) {
+            float h[P];
+            load_positions<float, P>(a.entropy + i, h);
+#pragma unroll
+            for (int p = 0; p < P; ++p) pull[p] = gh[p] != 0.f ? fmaf(gh[p], h[p], pull[p]) : pull[p];
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) some = some || any[p];
         for (int c0 = 0; c0 < a.C; c0 += BATCH) {
             float f[BATCH][P];
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
-                if (any && c0 + b < a.C) load_positions<T, P>(row + (c0 + b) * a.sc, f[b]);
+                if (some && c0 + b < a.C) load_positions<T, P>(row + (c0 + b) * a.sc, f[b]);
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
                 if (c0 + b < a.C) {
                     float d[P];
 #pragma unroll
-                    for (int p = 0; p < P; ++p) d[p] = q[p].any ? lp_grad(q[p], f[b][p]) + ((int)q[p].t == c0 + b ? q[p].gl : 0.f) : 0.f;
+                    for (int p = 0; p < P; ++p) {
+                        float own = t[p] == c0 + b ? gl[p] : 0.f;
+                        if (KT > 0) {
+#pragma unroll
+                            for (int k = 0; k < K; ++k) own += jk[k][p] == c0 + b ? gk[k][p] : 0.f;
+                        }
+                        d[p] = any[p] ? lp_grad(f[b][p], base[p], logs[p], gh[p], pull[p]) + own : 0.f;
+                    }
                     store_positions<T, P>(out + (c0 + b) * a.dc, d);
                 }
         }
-        if (!a.g_top) continue;
+        if (KT >= 0) continue;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            if (!q[p].any) continue;
+            if (!any[p]) continue;
             for (int k = 0; k < a.k; ++k) {
                 const long long j = a.top_index[(n * a.k + k) * a.L + l + p];
-                Elem<T>::st(out + p + j * a.dc, lp_grad(q[p], Elem<T>::ld(row + p + j * a.sc)) + lp_own(a, q[p], n, l + p, j));
+                float own = j == t[p] ? gl[p] : 0.f;
+                for (int o = 0; o < a.k; ++o) {
+                    const long long at = (n * a.k + o) * a.L + l + p;
+                    if (a.top_index[at] == j) own += a.g_top[at];
+                }
+                Elem<T>::st(out + p + j * a.dc, lp_grad(Elem<T>::ld(row + p + j * a.sc), base[p], logs[p], gh[p], pull[p]) + own);
             }
         }
     }
@@ -569,19 +643,29 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     T* out = (T*)a.dz + i * a.dn;
     const int off = (int)(((unsigned long long)row / sizeof(T)) % E), dist = (int)(((unsigned long long)out / sizeof(T)) % E);
     const int chunks = (a.C + off + E - 1) / E, q0 = blockIdx.y * TEAM * BWD_UNROLL, q1 = TEAM == 64 ? chunks : min(q0 + TEAM * BWD_UNROLL, chunks);
-    const LpPull pull = lp_pull(a, i, 0);
+    const long long t = a.g_log_prob ? a.target[i] : a.ignore;
+    const float gl = t == a.ignore ? 0.f : t >= 0 && t < a.C ? a.g_log_prob[i] : __builtin_nanf(""), gh = a.g_entropy ? a.g_entropy[i] : 0.f;
+    float pull = gl;
+    bool any = gl != 0.f || gh != 0.f;
+    for (int k = 0; k < a.k; ++k) {
+        const float gk = a.g_top[i * a.k + k];
+        any = any || gk != 0.f;
+        pull += gk;
+    }
+    const float base = a.stats[i], logs = a.stats[a.N + i];
+    if (gh != 0.f) pull = fmaf(gh, a.entropy[i], pull);
     for (int q = q0 + tid; q < q1; q += TEAM * BWD_UNROLL) {
         float f[BWD_UNROLL][E];
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u)
-            if (pull.any && q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
+            if (any && q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u) {
             if (q + u * TEAM >= q1) break;
             const int c0 = (q + u * TEAM) * E - off;
             float d[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) d[e] = pull.any ? lp_grad(pull, f[u][e]) : 0.f;
+            for (int e = 0; e < E; ++e) d[e] = any ? lp_grad(f[u][e], base, logs, gh, pull) : 0.f;
             if (c0 >= 0 && c0 + E <= a.C && off == dist) {
                 if constexpr (E == 4) *(f32x4*)(out + c0) = f32x4{d[0], d[1], d[2], d[3]};
                 else *(i32x4*)(out + c0) = i32x4{pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]), pack_bf16x2(d[6], d[7])};
@@ -592,19 +676,21 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
             }
         }
     }
-    if (!pull.any) return;                                             // the same for the whole team
+    if (!any) return;                                             // the same for the whole team
     if (TEAM == 64) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     } else {
         __syncthreads();                                               // the stores above are done before a class is written again
     }
-    const int own = 1 + (a.g_top ? a.k : 0);
-    if (tid < own) {
-        const long long j = tid ? a.top_index[i * a.k + tid - 1] : pull.t;
-        const long long c = j + off;
-        if (j >= 0 && j < a.C && c >= (long long)q0 * E && c < (long long)q1 * E)
-            Elem<T>::st(out + j, lp_grad(pull, Elem<T>::ld(row + j)) + lp_own(a, pull, i, 0, j));
+    if (tid <= a.k) {
+        const long long j = tid ? a.top_index[i * a.k + tid - 1] : t, c = j + off;
+        if (j >= 0 && j < a.C && c >= (long long)q0 * E && c < (long long)q1 * E) {
+            float own = j == t ? gl : 0.f;
+            for (int k = 0; k < a.k; ++k)
+                if (a.top_index[i * a.k + k] == j) own += a.g_top[i * a.k + k];
+            Elem<T>::st(out + j, lp_grad(Elem<T>::ld(row + j), base, logs, gh, pull) + own);
+        }
     }
 }
 
@@ -619,10 +705,12 @@ static inline unsigned lp_grid(long long total) {
     return (unsigned)(g > 65536 ? 65536 : g);
 }
 
-// Positions per thread: 4 where whole vectors lie on their boundaries and enough threads are left to fill the chip
-static inline int lp_positions(int dtype, long long N, long long L, long long sc, unsigned long long addresses, unsigned long long strides) {
+// Positions per thread: 4 where whole vectors lie on their boundaries, enough threads are left to fill the chip and the alternatives
+// leave registers (most_k).  6 x 20 x 512 x 1024, 4 positions against 1: bf16 52 / 75 us forward, 83 / 128 us backward; fp32 alike.
+static inline int lp_positions(int dtype, long long N, long long L, long long sc, unsigned long long addresses, unsigned long long strides,
+                               unsigned long long per_position, int k, int most_k) {
     const int size = dtype == ERF_BF16 ? 2 : 4;
-    return sc != 1 && L % 4 == 0 && strides % 4 == 0 && addresses % (4 * size) == 0 && N * L >= (1ll << 19) ? 4 : 1;
+    return sc != 1 && L % 4 == 0 && strides % 4 == 0 && addresses % (4 * size) == 0 && per_position % 16 == 0 && N * L >= (1ll << 19) && k <= most_k ? 4 : 1;
 }
 
 // Rows of more classes than a thread walks through by itself are taken by teams: a wave, or a workgroup where that gives each of its
@@ -665,7 +753,9 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
         else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
     } else {
-        const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits, (unsigned long long)(stride_n | stride_c));
+        const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits, (unsigned long long)(stride_n | stride_c),
+                                   (unsigned long long)log_prob | (unsigned long long)entropy | (unsigned long long)stats |
+                                       (unsigned long long)top_log_probs | (unsigned long long)top_indices, top_k, 4);
         const dim3 grid(lp_grid(N * L / p)), block(256);
 #define LP_KT(T, P)                                                                                          \
     do {                                                                                                     \
@@ -673,7 +763,8 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         else if (top_k == 1) hipLaunchKernelGGL((lp_position_kernel<T, P, 1>), grid, block, 0, s, a);        \
         else if (top_k == 2) hipLaunchKernelGGL((lp_position_kernel<T, P, 2>), grid, block, 0, s, a);        \
         else if (top_k <= 4) hipLaunchKernelGGL((lp_position_kernel<T, P, 4>), grid, block, 0, s, a);        \
-        else hipLaunchKernelGGL((lp_position_kernel<T, P, -1>), grid, block, 0, s, a);                       \
+        else if (top_k <= 8) hipLaunchKernelGGL((lp_position_kernel<T, 1, 8>), grid, block, 0, s, a);        \
+        else hipLaunchKernelGGL((lp_position_kernel<T, 1, -1>), grid, block, 0, s, a);                       \
     } while (0)
         if (dtype == ERF_BF16) { if (p == 4) LP_KT(bf16raw, 4); else LP_KT(bf16raw, 1); }
         else { if (p == 4) LP_KT(float, 4); else LP_KT(float, 1); }
@@ -706,15 +797,21 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
         }
     } else {
         const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits | (unsigned long long)dlogits,
-                                   (unsigned long long)(stride_n | stride_c | dstride_n | dstride_c));
+                                   (unsigned long long)(stride_n | stride_c | dstride_n | dstride_c),
+                                   (unsigned long long)stats | (unsigned long long)entropy | (unsigned long long)g_log_prob |
+                                       (unsigned long long)g_entropy | (unsigned long long)g_top, a.k, 2);
         const dim3 grid(lp_grid(N * L / p)), block(256);
-        if (dtype == ERF_BF16) {
-            if (p == 4) hipLaunchKernelGGL((lp_position_bwd_kernel<bf16raw, 4>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((lp_position_bwd_kernel<bf16raw, 1>), grid, block, 0, s, a);
-        } else {
-            if (p == 4) hipLaunchKernelGGL((lp_position_bwd_kernel<float, 4>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((lp_position_bwd_kernel<float, 1>), grid, block, 0, s, a);
-        }
+#define LP_KT(T, P)                                                                                          \
+    do {                                                                                                     \
+        if (a.k == 0) hipLaunchKernelGGL((lp_position_bwd_kernel<T, P, 0>), grid, block, 0, s, a);           \
+        else if (a.k <= 2) hipLaunchKernelGGL((lp_position_bwd_kernel<T, P, 2>), grid, block, 0, s, a);      \
+        else if (a.k <= 4) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 4>), grid, block, 0, s, a);      \
+        else if (a.k <= 8) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 8>), grid, block, 0, s, a);      \
+        else hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, -1>), grid, block, 0, s, a);                   \
+    } while (0)
+        if (dtype == ERF_BF16) { if (p == 4) LP_KT(bf16raw, 4); else LP_KT(bf16raw, 1); }
+        else { if (p == 4) LP_KT(float, 4); else LP_KT(float, 1); }
+#undef LP_KT
     }
     return erf_check_launch();
 }

@@ -154,7 +154,7 @@ def test_rows(shape, layout, dtype):
 def test_maps(shape, layout, dtype):
     z = _logits(shape, dtype, layout, 3)
     t = _targets(z, 4)
-    for k in sorted({0, 1, min(5, shape[1]), min(32, shape[1])}):
+    for k in sorted({0, 1, *(min(j, shape[1]) for j in (2, 3, 5, 32))}):
         _check(z, t, k, seed=k)
 
 
