@@ -44,24 +44,45 @@ __device__ __forceinline__ float rank_value(u64 r) {
     return k > 0xFF800000u ? __builtin_nanf("") : __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
 }
 
-// Reductions over the 64 lanes: shifts within rows of 16 lanes, then the rows' last lanes are passed on; lane 63 has the result
+// Reductions over teams of 8, 16 or 64 lanes; every lane of the team gets the result.  8 and 16 lanes: exchanges within a row of 16
+// (across 1, 2 and 4 lanes, then 8); 64: shifts within rows, then the rows' last lanes are passed on and lane 63 has the result.
+// Lanes without a partner read 0, which is below every rank and adds nothing.
 template <int CTRL> __device__ __forceinline__ int dpp0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true); }
-template <int CTRL> __device__ __forceinline__ void sum_step(float& v) { v += __int_as_float(dpp0<CTRL>(__float_as_int(v))); }
-__device__ __forceinline__ float wave_total(float v) {
-    sum_step<0x111>(v); sum_step<0x112>(v); sum_step<0x114>(v); sum_step<0x118>(v); sum_step<0x142>(v); sum_step<0x143>(v);
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+template <int CTRL> __device__ __forceinline__ float dpp_f(float v) { return __int_as_float(dpp0<CTRL>(__float_as_int(v))); }
+template <int CTRL> __device__ __forceinline__ u64 dpp_u(u64 v) {
+    return ((u64)(unsigned)dpp0<CTRL>((int)(v >> 32)) << 32) | (unsigned)dpp0<CTRL>((int)v);
 }
-template <int CTRL> __device__ __forceinline__ void max_step(u64& v) {
-    const u64 o = ((u64)(unsigned)dpp0<CTRL>((int)(v >> 32)) << 32) | (unsigned)dpp0<CTRL>((int)v);
-    v = o > v ? o : v;
+#define SWAP1 0xB1       // quad_perm 1,0,3,2
+#define SWAP2 0x4E       // quad_perm 2,3,0,1
+#define MIRROR8 0x141    // row_half_mirror: after the first two, lane and mirror image stand for the two quads
+#define ROTATE8 0x128    // row_ror 8
+template <int TEAM> __device__ __forceinline__ float team_sum(float v) {
+    if (TEAM == 64) {
+        v += dpp_f<0x111>(v); v += dpp_f<0x112>(v); v += dpp_f<0x114>(v); v += dpp_f<0x118>(v); v += dpp_f<0x142>(v); v += dpp_f<0x143>(v);
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+    }
+    v += dpp_f<SWAP1>(v); v += dpp_f<SWAP2>(v); v += dpp_f<MIRROR8>(v);
+    if (TEAM == 16) v += dpp_f<ROTATE8>(v);
+    return v;
 }
-__device__ __forceinline__ u64 wave_best(u64 v) {
-    max_step<0x111>(v); max_step<0x112>(v); max_step<0x114>(v); max_step<0x118>(v); max_step<0x142>(v); max_step<0x143>(v);
-    return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+template <int TEAM> __device__ __forceinline__ u64 team_best(u64 v) {
+    auto up = [&](u64 o) { v = o > v ? o : v; };
+    if (TEAM == 64) {
+        up(dpp_u<0x111>(v)); up(dpp_u<0x112>(v)); up(dpp_u<0x114>(v)); up(dpp_u<0x118>(v)); up(dpp_u<0x142>(v)); up(dpp_u<0x143>(v));
+        return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+    }
+    up(dpp_u<SWAP1>(v)); up(dpp_u<SWAP2>(v)); up(dpp_u<MIRROR8>(v));
+    if (TEAM == 16) up(dpp_u<ROTATE8>(v));
+    return v;
 }
-__device__ __forceinline__ float wave_largest(float v) {
+template <int TEAM> __device__ __forceinline__ float team_largest(float v) {
+    if (TEAM == 64) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+        for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+        return v;
+    }
+    v = fmaxf(v, dpp_f<SWAP1>(v)); v = fmaxf(v, dpp_f<SWAP2>(v)); v = fmaxf(v, dpp_f<MIRROR8>(v));
+    if (TEAM == 16) v = fmaxf(v, dpp_f<ROTATE8>(v));
     return v;
 }
 
@@ -89,8 +110,10 @@ __device__ __forceinline__ void lp_finish(const LpArgs& a, const T* row, long lo
         a.log_prob[i] = v;
     }
     a.entropy[i] = logs - st.t * LN2 / st.s;
-    a.stats[i] = base;
-    a.stats[a.N * a.L + i] = logs;
+    if (a.stats) {
+        a.stats[i] = base;
+        a.stats[a.N * a.L + i] = logs;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ one thread per position
@@ -230,8 +253,10 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
 #pragma unroll
         for (int p = 0; p < P; ++p) v[p] = logs[p] - st[p].t * LN2 / st[p].s;
         store_positions<float, P>(a.entropy + i, v);
-        store_positions<float, P>(a.stats + i, base);
-        store_positions<float, P>(a.stats + rows + i, logs);
+        if (a.stats) {
+            store_positions<float, P>(a.stats + i, base);
+            store_positions<float, P>(a.stats + rows + i, logs);
+        }
         if (KT == 0) continue;
         bool rounds = KT < 0;
 #pragma unroll
@@ -271,25 +296,27 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
 
 // ------------------------------------------------------------------------------------------------ a team of threads per row
 // A row is cut at the 16-byte boundaries of memory into chunks of EPC classes, the first and the last possibly partial; thread r of
-// the team takes chunks r, r + TEAM, ...  UNROLL of them are in flight and share one change of the maximum.
+// the team takes chunks r, r + TEAM, ...  UNROLL of them are in flight and share one change of the maximum.  Teams of 8, 16 or 64
+// lanes have the whole row in registers then; a workgroup goes on along a longer row.
 //
-// Alternatives: each thread keeps its largest value and the first chunk it stood in.  Ordered by (value, chunk), the k best threads
-// hold the k best classes -- any class of another thread has k before it -- so only their chunks are read again, 1/TEAM of the row
-// each.  What reaches the k-th thread's value is collected and the k best of it taken.  Rows with NaN, and rows where more values tie
-// than the collection holds, go through k rounds over the row.
-#define CAND 512
+// Alternatives: the k-th largest of the threads' own maxima is a bound that the k best classes reach, and few others do.  What
+// reaches it is collected -- from the registers, or by the whole workgroup from the chunks of the threads whose maximum reaches it --
+// and put in its place by counting.  Rows with NaN, and rows where more values tie than the collection holds, go through k rounds
+// over the row.
 #define UNROLL 4
 
 template <int TEAM> struct TeamShared {
+    enum { CAND = TEAM == 256 ? 512 : TEAM == 64 ? 256 : 64 };
     float m[4], s[4], t[4];
-    u64 key[TEAM], cand[CAND];
-    int winner[ERF_TOP_MAX];
+    u64 cand[CAND];
+    float max[TEAM == 256 ? 256 : 1];
+    int winner[TEAM == 256 ? 256 : 1];
     int winners, ncand;
     float least;
 };
 
 template <int TEAM> __device__ __forceinline__ void team_sync() {
-    if (TEAM == 64) {
+    if (TEAM < 256) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     } else {
@@ -325,34 +352,57 @@ __device__ __forceinline__ u64 team_round(TeamShared<TEAM>& sh, const T* row, in
         const u64 r = rank_of(Elem<T>::ld(row + c), c);
         if (r < last && r > best) best = r;
     }
-    best = wave_best(best);
-    if (TEAM == 64) return best;
-    __syncthreads();                                                   // the previous round's keys have been read
-    if ((tid & 63) == 0) sh.key[tid >> 6] = best;
+    if constexpr (TEAM < 256) return team_best<TEAM>(best);
+    best = team_best<64>(best);
+    __syncthreads();                                                   // the previous round's ranks have been read
+    if ((tid & 63) == 0) sh.cand[tid >> 6] = best;
     __syncthreads();
-    best = sh.key[0];
-    for (int w = 1; w < TEAM / 64; ++w) best = sh.key[w] > best ? sh.key[w] : best;
+    best = sh.cand[0];
+    for (int w = 1; w < 4; ++w) best = sh.cand[w] > best ? sh.cand[w] : best;
     return best;
+}
+
+// The k-th largest of the wave's or sub-wave team's PER values a lane; -inf where there are fewer
+template <int TEAM, int PER>
+__device__ __forceinline__ float kth_largest(float* v, int k, int tid) {
+    float m = INFINITY;
+    for (int n = 0; n < k; ++n) {
+        float mine = v[0];
+#pragma unroll
+        for (int w = 1; w < PER; ++w) mine = fmaxf(mine, v[w]);
+        m = team_largest<TEAM>(mine);
+        if (m == -INFINITY) break;
+        // one of the lanes that have it gives it up
+        const u64 have = __ballot(mine == m) & (TEAM == 64 ? ~0ull : ((1ull << (TEAM & 63)) - 1) << ((threadIdx.x & 63) - tid));
+        if ((int)(threadIdx.x & 63) == __ffsll((long long)have) - 1) {
+            bool gone = false;
+#pragma unroll
+            for (int w = 0; w < PER; ++w) {
+                const bool it = !gone && v[w] == m;
+                v[w] = it ? -INFINITY : v[w];
+                gone = gone || it;
+            }
+        }
+    }
+    return m;
 }
 
 template <typename T, int TEAM, bool TOP>
 __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     constexpr int E = Elem<T>::EPC;
-    __shared__ TeamShared<TEAM> shared[256 / TEAM];
+    __shared__ TeamShared<TOP || TEAM == 256 ? TEAM : 8> shared[TOP || TEAM == 256 ? 256 / TEAM : 1];
     const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
-    TeamShared<TEAM>& sh = shared[team];
     const long long i = (long long)blockIdx.x * (256 / TEAM) + team;
-    if (TEAM == 64 && i >= a.N) return;                                // no barrier of the workgroup below for teams of one wave
+    if (TEAM < 256 && i >= a.N) return;                                // no barrier of the workgroup below for teams within a wave
+    auto& sh = shared[TOP ? team : 0];
     const T* row = (const T*)a.z + i * a.sn;
     const int off = (int)(((unsigned long long)row / sizeof(T)) % E);
     const int chunks = (a.C + off + E - 1) / E, per = (chunks + a.segments - 1) / a.segments;
     const int seg = blockIdx.y, q0 = min(seg * per, chunks), q1 = min(q0 + per, chunks);
 
     Stat st{-INFINITY, 0.f, 0.f};
-    float best = -INFINITY;
-    int bestq = -1;
-    for (int q = q0 + tid; q < q1; q += TEAM * UNROLL) {
-        float f[UNROLL][E], cm[UNROLL];
+    float f[UNROLL][E];
+    for (int q = q0 + tid; q < (TEAM < 256 ? q0 + TEAM : q1); q += TEAM * UNROLL) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             if (q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
@@ -363,13 +413,9 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
         }
         float most = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            cm[u] = f[u][0];
+        for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-            for (int e = 1; e < E; ++e) cm[u] = fmaxf(cm[u], f[u][e]);
-            most = fmaxf(most, cm[u]);
-            if (TOP && (cm[u] > best || bestq < 0) && q + u * TEAM < q1) { best = cm[u]; bestq = q + u * TEAM; }
-        }
+            for (int e = 0; e < E; ++e) most = fmaxf(most, f[u][e]);
         if (most > st.m) stat_move(st, most);
         const float base = base_of(st.m);
 #pragma unroll
@@ -377,17 +423,18 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) stat_add(st, base, f[u][e]);
     }
-    const float wm = wave_largest(st.m);
-    stat_move(st, wm);
-    st.s = wave_total(st.s);
-    st.t = wave_total(st.t);
-    if (TEAM > 64) {
+    float own[1] = {st.m};                                             // this thread's largest value
+    constexpr int WAVE = TEAM < 256 ? TEAM : 64;
+    stat_move(st, team_largest<WAVE>(st.m));
+    st.s = team_sum<WAVE>(st.s);
+    st.t = team_sum<WAVE>(st.t);
+    if constexpr (TEAM == 256) {
         if ((tid & 63) == 0) { sh.m[tid >> 6] = st.m; sh.s[tid >> 6] = st.s; sh.t[tid >> 6] = st.t; }
         __syncthreads();
         float m = sh.m[0];
-        for (int w = 1; w < TEAM / 64; ++w) m = fmaxf(m, sh.m[w]);
+        for (int w = 1; w < 4; ++w) m = fmaxf(m, sh.m[w]);
         Stat sum{m, 0.f, 0.f};
-        for (int w = 0; w < TEAM / 64; ++w) {
+        for (int w = 0; w < 4; ++w) {
             Stat p{sh.m[w], sh.s[w], sh.t[w]};
             stat_move(p, m);
             sum.s += p.s;
@@ -405,72 +452,77 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
             part[1] = __float_as_uint(st.t);
         }
     }
-    if (!TOP) return;
-
-    auto put = [&](int k, u64 r) {                                     // alternative k, by one thread
-        if (whole) {
-            a.top[i * a.k + k] = (rank_value(r) - base) - logs;
-            a.top_index[i * a.k + k] = rank_index(r);
-        } else {
-            part[2 + k] = r;
-        }
-    };
-    bool slow = st.s != st.s;                                          // the same for the whole team, as all that follows
-    if (!slow) {
-        sh.key[tid] = bestq >= 0 ? rank_of(best, bestq) : 0;
-        if (tid == 0) sh.ncand = 0;
-        team_sync<TEAM>();
-        if (tid < 64) {
-            u64 key[TEAM / 64], last = ~0ull;
-#pragma unroll
-            for (int w = 0; w < TEAM / 64; ++w) key[w] = sh.key[w * 64 + tid];
-            int n = 0;
-            for (; n < a.k; ++n) {
-                u64 r = 0;
-#pragma unroll
-                for (int w = 0; w < TEAM / 64; ++w) r = key[w] < last && key[w] > r ? key[w] : r;
-                r = wave_best(r);
-                if (!r) break;                                         // fewer threads than k have a chunk
-                last = r;
-                if (tid == 0) sh.winner[n] = (int)(rank_index(r) - q0) % TEAM;
+    if constexpr (TOP) {
+        auto put = [&](int k, u64 r) {                                 // alternative k, by one thread
+            if (whole) {
+                a.top[i * a.k + k] = (rank_value(r) - base) - logs;
+                a.top_index[i * a.k + k] = rank_index(r);
+            } else {
+                part[2 + k] = r;
             }
-            if (tid == 0) { sh.winners = n; sh.least = n == a.k ? rank_value(last) : -INFINITY; }
-        }
-        team_sync<TEAM>();
-        const int each = (q1 - q0 + TEAM - 1) / TEAM, winners = sh.winners;
-        const float least = sh.least;
-        for (int p = tid; p < winners * each; p += TEAM) {
-            const int q = q0 + sh.winner[p / each] + p % each * TEAM;
-            if (q >= q1) continue;
-            float f[E];
-            load_chunk(row, off, a.C, q, f);
+        };
+        bool slow = st.s != st.s;                                      // the same for the whole team, as all that follows
+        if (!slow) {
+            if (tid == 0) sh.ncand = 0;
+            auto collect = [&](const float* v, int q, float least) {   // the order has no effect: the ranks decide
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int c = q * E - off + e;
-                if (f[e] >= least && c >= 0 && c < a.C) {
-                    const int at = atomicAdd(&sh.ncand, 1);            // their order has no effect: the ranks decide
-                    if (at < CAND) sh.cand[at] = rank_of(f[e], c);
+                for (int e = 0; e < E; ++e) {
+                    const int c = q * E - off + e;
+                    if (v[e] >= least && c >= 0 && c < a.C) {
+                        const int at = atomicAdd(&sh.ncand, 1);
+                        if (at < TeamShared<TEAM>::CAND) sh.cand[at] = rank_of(v[e], c);
+                    }
+                }
+            };
+            if constexpr (TEAM < 256) {
+                const float least = kth_largest<TEAM, 1>(own, a.k, tid);
+                team_sync<TEAM>();
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u)
+                    if (q0 + tid + u * TEAM < q1) collect(f[u], q0 + tid + u * TEAM, least);
+            } else {
+                sh.max[tid] = own[0];
+                if (tid == 0) sh.winners = 0;
+                __syncthreads();
+                if (tid < 64) {
+                    float v[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) v[w] = sh.max[w * 64 + tid];
+                    const float least = kth_largest<64, 4>(v, a.k, tid);
+                    if (tid == 0) sh.least = least;
+                }
+                __syncthreads();
+                const float least = sh.least;
+                if (own[0] >= least && q0 + tid < q1) sh.winner[atomicAdd(&sh.winners, 1)] = tid;
+                __syncthreads();
+                const int each = (q1 - q0 + TEAM - 1) / TEAM, n = sh.winners;
+                for (int p = tid; p < n * each; p += TEAM) {
+                    const int q = q0 + sh.winner[p / each] + p % each * TEAM;
+                    if (q >= q1) continue;
+                    float v[E];
+                    load_chunk(row, off, a.C, q, v);
+                    collect(v, q, least);
                 }
             }
-        }
-        team_sync<TEAM>();
-        const int n = sh.ncand;
-        slow = n > CAND;
-        if (!slow && tid < 64) {
-            u64 last = ~0ull;
-            for (int k = 0; k < a.k; ++k) {
-                u64 r = 0;
-                for (int c = tid; c < n; c += 64) r = sh.cand[c] < last && sh.cand[c] > r ? sh.cand[c] : r;
-                last = wave_best(r);
-                if (tid == 0) put(k, last);
+            team_sync<TEAM>();
+            const int n = sh.ncand;
+            slow = n > TeamShared<TEAM>::CAND;
+            if (!slow) {
+                for (int c = tid; c < n; c += TEAM) {
+                    const u64 r = sh.cand[c];
+                    int before = 0;
+                    for (int o = 0; o < n && before < a.k; ++o) before += sh.cand[o] > r;
+                    if (before < a.k) put(before, r);
+                }
+                for (int k = n + tid; k < a.k; k += TEAM) put(k, 0);   // a segment of fewer classes
             }
         }
-    }
-    if (slow) {
-        u64 last = ~0ull;
-        for (int k = 0; k < a.k; ++k) {
-            last = team_round<T, TEAM>(sh, row, off, a.C, q0, q1, tid, last);
-            if (tid == 0) put(k, last);
+        if (slow) {
+            u64 last = ~0ull;
+            for (int k = 0; k < a.k; ++k) {
+                last = team_round<T, TEAM>(sh, row, off, a.C, q0, q1, tid, last);
+                if (tid == 0) put(k, last);
+            }
         }
     }
 }
@@ -491,9 +543,9 @@ __global__ __launch_bounds__(64) void lp_join_kernel(const LpArgs a) {
         st.s += p.s;
         st.t += p.t;
     }
-    stat_move(st, wave_largest(st.m));
-    st.s = wave_total(st.s);
-    st.t = wave_total(st.t);
+    stat_move(st, team_largest<64>(st.m));
+    st.s = team_sum<64>(st.s);
+    st.t = team_sum<64>(st.t);
     const float logs = logf(st.s);
     if (threadIdx.x == 0) lp_finish(a, (const T*)a.z + i * a.sn, i, st, logs);
     u64 last = ~0ull;
@@ -504,7 +556,7 @@ __global__ __launch_bounds__(64) void lp_join_kernel(const LpArgs a) {
             const u64 o = part[(long long)(c / a.k) * step + 2 + c % a.k];
             r = o < last && o > r ? o : r;
         }
-        last = wave_best(r);
+        last = team_best<64>(r);
         if (threadIdx.x == 0) {
             a.top[i * a.k + k] = (rank_value(last) - base_of(st.m)) - logs;
             a.top_index[i * a.k + k] = rank_index(last);
@@ -638,11 +690,11 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     constexpr int E = Elem<T>::EPC;
     const int tid = threadIdx.x % TEAM;
     const long long i = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
-    if (TEAM == 64 && i >= a.N) return;                                // no barrier of the workgroup below for teams of one wave
+    if (TEAM < 256 && i >= a.N) return;                                // no barrier of the workgroup below for teams within a wave
     const T* row = (const T*)a.z + i * a.sn;
     T* out = (T*)a.dz + i * a.dn;
     const int off = (int)(((unsigned long long)row / sizeof(T)) % E), dist = (int)(((unsigned long long)out / sizeof(T)) % E);
-    const int chunks = (a.C + off + E - 1) / E, q0 = blockIdx.y * TEAM * BWD_UNROLL, q1 = TEAM == 64 ? chunks : min(q0 + TEAM * BWD_UNROLL, chunks);
+    const int chunks = (a.C + off + E - 1) / E, q0 = blockIdx.y * TEAM * BWD_UNROLL, q1 = min(q0 + TEAM * BWD_UNROLL, chunks);
     const long long t = a.g_log_prob ? a.target[i] : a.ignore;
     const float gl = t == a.ignore ? 0.f : t >= 0 && t < a.C ? a.g_log_prob[i] : __builtin_nanf(""), gh = a.g_entropy ? a.g_entropy[i] : 0.f;
     float pull = gl;
@@ -654,7 +706,8 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     }
     const float base = a.stats[i], logs = a.stats[a.N + i];
     if (gh != 0.f) pull = fmaf(gh, a.entropy[i], pull);
-    for (int q = q0 + tid; q < q1; q += TEAM * BWD_UNROLL) {
+    {
+        const int q = q0 + tid;
         float f[BWD_UNROLL][E];
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u)
@@ -677,18 +730,15 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
         }
     }
     if (!any) return;                                             // the same for the whole team
-    if (TEAM == 64) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    } else {
-        __syncthreads();                                               // the stores above are done before a class is written again
-    }
-    if (tid <= a.k) {
-        const long long j = tid ? a.top_index[i * a.k + tid - 1] : t, c = j + off;
+    // the stores above are done before a class is written again
+    if (TEAM < 256) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    else __syncthreads();
+    for (int k = tid; k <= a.k; k += TEAM) {
+        const long long j = k ? a.top_index[i * a.k + k - 1] : t, c = j + off;
         if (j >= 0 && j < a.C && c >= (long long)q0 * E && c < (long long)q1 * E) {
             float own = j == t ? gl : 0.f;
-            for (int k = 0; k < a.k; ++k)
-                if (a.top_index[i * a.k + k] == j) own += a.g_top[i * a.k + k];
+            for (int o = 0; o < a.k; ++o)
+                if (a.top_index[i * a.k + o] == j) own += a.g_top[i * a.k + o];
             Elem<T>::st(out + j, lp_grad(Elem<T>::ld(row + j), base, logs, gh, pull) + own);
         }
     }
@@ -713,43 +763,66 @@ static inline int lp_positions(int dtype, long long N, long long L, long long sc
     return sc != 1 && L % 4 == 0 && strides % 4 == 0 && addresses % (4 * size) == 0 && per_position % 16 == 0 && N * L >= (1ll << 19) && k <= most_k ? 4 : 1;
 }
 
-// Rows of more classes than a thread walks through by itself are taken by teams: a wave, or a workgroup where that gives each of its
-// threads a full set of loads; few rows of very many classes are split so that about 1024 workgroups have work.
-#define POSITION_CLASSES 64
+// Rows of more classes than a thread walks through by itself are taken by the smallest team that has the whole row in registers
+// wherever it starts (and lanes for the alternatives), or by a workgroup; few rows of very many classes are split so that about 1024 workgroups have work.
 static inline int lp_epc(int dtype) { return dtype == ERF_BF16 ? 8 : 4; }
-static inline bool lp_wave_rows(int dtype, int C) { return C <= 64 * UNROLL * lp_epc(dtype); }
-static inline int lp_segments(int dtype, long long N, int C) {
-    if (lp_wave_rows(dtype, C)) return 1;
+// A thread takes a whole row of up to `alone` classes.  Forward, 1000000 rows of 24 / 40 classes: 51 / 126 us by threads and 47 / 55 us by
+// teams in fp32, 40 / 133 and 69 / 70 us in bf16; backward, 12 / 24 classes: 49 / 146 and 46 / 71 us, 32 / 105 and 74 / 48 us.
+#define ALONE_FWD 24
+#define ALONE_BWD 12
+static inline int lp_team(int dtype, int C, int k, int alone) {
+    if (C <= alone) return 1;
+    for (int team = 8; team <= 64; team = team == 16 ? 64 : 2 * team)
+        if (k <= team && C <= (team * UNROLL - 1) * lp_epc(dtype) + 1) return team;
+    return 256;
+}
+static inline int lp_segments(int dtype, long long N, int C, int k) {
+    if (lp_team(dtype, C, k, ALONE_FWD) < 256) return 1;
     const long long most = ((long long)C + 256 * UNROLL * lp_epc(dtype) - 1) / (256 * UNROLL * lp_epc(dtype)), want = (1024 + N - 1) / N;
     return (int)(want < most ? want : most);
 }
 
 template <typename T, bool TOP>
 static void lp_rows_launch(const LpArgs& a, int dtype, hipStream_t s) {
-    if (lp_wave_rows(dtype, a.C)) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), dim3((unsigned)((a.N + 3) / 4)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), dim3((unsigned)a.N, (unsigned)a.segments), dim3(256), 0, s, a);
+    const int team = lp_team(dtype, a.C, a.k, ALONE_FWD);
+    const dim3 grid((unsigned)((a.N * team + 255) / 256), (unsigned)a.segments), block(256);
+    if (team == 8) hipLaunchKernelGGL((lp_rows_kernel<T, 8, TOP>), grid, block, 0, s, a);
+    else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, TOP>), grid, block, 0, s, a);
+    else if (team == 64) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), grid, block, 0, s, a);
     if (a.segments > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)a.N), dim3(64), 0, s, a);
+}
+
+template <typename T>
+static void lp_rows_bwd_launch(const LpBwdArgs& a, int dtype, hipStream_t s) {
+    const int team = lp_team(dtype, a.C, 0, ALONE_BWD), per = 256 * BWD_UNROLL;
+    const int chunks = (a.C + 2 * (lp_epc(dtype) - 1)) / lp_epc(dtype);              // of a row that starts just before a boundary
+    const dim3 grid((unsigned)((a.N * team + 255) / 256), team < 256 ? 1u : (unsigned)((chunks + per - 1) / per)), block(256);
+    if (team == 8) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 8>), grid, block, 0, s, a);
+    else if (team == 16) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 16>), grid, block, 0, s, a);
+    else if (team == 64) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 64>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 256>), grid, block, 0, s, a);
 }
 
 extern "C" {
 
 size_t erf_class_log_probs_workspace_bytes(int dtype, long long N, int C, long long L, long long stride_c, int top_k) {
-    if (!lp_shape_ok(dtype, N, C, L, 0, stride_c, top_k) || stride_c != 1 || C <= POSITION_CLASSES) return 0;
-    const int segments = lp_segments(dtype, N, C);
+    if (!lp_shape_ok(dtype, N, C, L, 0, stride_c, top_k) || stride_c != 1) return 0;
+    const int segments = lp_segments(dtype, N, C, top_k);
     return segments > 1 ? (size_t)N * segments * (2 + top_k) * sizeof(u64) : 0;
 }
 
 int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, long long L, long long stride_n, long long stride_c,
                             const long long* target, long long ignore_index, float* log_prob, float* entropy, float* stats, int top_k,
                             float* top_log_probs, long long* top_indices, void* workspace, void* stream) {
-    if (!logits || !entropy || !stats || (!target != !log_prob) || !lp_shape_ok(dtype, N, C, L, stride_n, stride_c, top_k) ||
+    if (!logits || !entropy || (!target != !log_prob) || !lp_shape_ok(dtype, N, C, L, stride_n, stride_c, top_k) ||
         (top_k && (!top_log_probs || !top_indices)) ||
         (!workspace && erf_class_log_probs_workspace_bytes(dtype, N, C, L, stride_c, top_k)))
         return ERF_EINVAL;
     LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, (u64*)workspace};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && C > POSITION_CLASSES) {
-        a.segments = lp_segments(dtype, N, C);
+    if (stride_c == 1 && lp_team(dtype, C, top_k, ALONE_FWD) > 1) {
+        a.segments = lp_segments(dtype, N, C, top_k);
         if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
         else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
     } else {
@@ -783,18 +856,9 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
                       g_log_prob, g_entropy, g_top, top_indices, dlogits};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && C > POSITION_CLASSES) {
-        const int per = 256 * BWD_UNROLL * lp_epc(dtype);
-        const bool wave = lp_wave_rows(dtype, C);
-        // one chunk more than C / EPC where a row starts off the boundaries
-        const dim3 grid(wave ? (unsigned)((N + 3) / 4) : (unsigned)N, wave ? 1u : (unsigned)((C + lp_epc(dtype) - 1 + per - 1) / per)), block(256);
-        if (dtype == ERF_BF16) {
-            if (wave) hipLaunchKernelGGL((lp_rows_bwd_kernel<bf16raw, 64>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((lp_rows_bwd_kernel<bf16raw, 256>), grid, block, 0, s, a);
-        } else {
-            if (wave) hipLaunchKernelGGL((lp_rows_bwd_kernel<float, 64>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((lp_rows_bwd_kernel<float, 256>), grid, block, 0, s, a);
-        }
+    if (stride_c == 1 && lp_team(dtype, C, 0, ALONE_BWD) > 1) {
+        if (dtype == ERF_BF16) lp_rows_bwd_launch<bf16raw>(a, dtype, s);
+        else lp_rows_bwd_launch<float>(a, dtype, s);
     } else {
         const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits | (unsigned long long)dlogits,
                                    (unsigned long long)(stride_n | stride_c | dstride_n | dstride_c),

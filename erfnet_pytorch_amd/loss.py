@@ -122,5 +122,5 @@ def class_log_probs(logits, target=None, top_k=0, ignore_index=-100):
     if logits.requires_grad and torch.is_grad_enabled():
         log_prob, entropy, top, index = _ClassLogProbsFn.apply(logits, target, int(top_k), int(ignore_index))
     else:
-        log_prob, entropy, _, top, index = train_ops.class_log_probs_fwd(logits, target, int(top_k), int(ignore_index))
+        log_prob, entropy, _, top, index = train_ops.class_log_probs_fwd(logits, target, int(top_k), int(ignore_index), False)
     return ClassLogProbs(None if target is None else log_prob, entropy, top if top_k else None, index if top_k else None)

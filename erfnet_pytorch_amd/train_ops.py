@@ -97,15 +97,17 @@ def _check_target(who, target, shape, z):
         return None
     if target.dtype != torch.int64:
         raise TypeError(f"{who}: targets are int64 class indices, got {target.dtype}")
-    if tuple(target.shape) != tuple(shape):
+    if target.shape != shape:
         raise ValueError(f"{who}: expected targets of shape {tuple(shape)}, got {tuple(target.shape)}")
-    _same_device(who, z, target=target)
+    if target.device != z.device:
+        raise ValueError(f"{who}: target is on {target.device}, the input on {z.device}")
     return target.contiguous()
 
 
-def class_log_probs_fwd(logits, target, top_k=0, ignore_index=-100):
+def class_log_probs_fwd(logits, target, top_k=0, ignore_index=-100, with_stats=True):
     """(log_prob, entropy, stats, top_log_probs, top_indices) of logits [N, C, ...]; loss.class_log_probs describes them.  stats
-    [2, ...]: the row maximum and log sum e^{z - max}, for the backward pass.  Without a target log_prob is empty."""
+    [2, ...]: the row maximum and log sum e^{z - max}, for the backward pass (None without `with_stats`).  Without a target
+    log_prob is empty."""
     who = "class_log_probs"
     code = dtype_code(logits, who)
     if logits.dim() < 2 or logits.shape[1] < 1:
@@ -116,7 +118,8 @@ def class_log_probs_fwd(logits, target, top_k=0, ignore_index=-100):
     target = _check_target(who, target, shape, z)
     new = z.new_empty
     log_prob = new(shape if target is not None else (0,), dtype=torch.float32)
-    entropy, stats = new(shape, dtype=torch.float32), new((2, *shape), dtype=torch.float32)
+    entropy = new(shape, dtype=torch.float32)
+    stats = new((2, *shape), dtype=torch.float32) if with_stats else None
     top_shape, order = _top_shape(shape, top_k, rows)
     top, index = new(top_shape, dtype=torch.float32), new(top_shape, dtype=torch.int64)
     if entropy.numel():
@@ -124,7 +127,7 @@ def class_log_probs_fwd(logits, target, top_k=0, ignore_index=-100):
             nbytes = size_query("erf_class_log_probs_workspace_bytes", code, n, c, length, sc, top_k)
             ws = new(nbytes, dtype=torch.uint8) if nbytes else None
             call("erf_class_log_probs_fwd", z.data_ptr(), code, n, c, length, sn, sc, _p(target), ignore_index,
-                 log_prob.data_ptr() if target is not None else 0, entropy.data_ptr(), stats.data_ptr(), top_k, top.data_ptr() if top_k else 0,
+                 log_prob.data_ptr() if target is not None else 0, entropy.data_ptr(), _p(stats), top_k, top.data_ptr() if top_k else 0,
                  index.data_ptr() if top_k else 0, _p(ws), _stream())
     if order is not None and top_k:
         top, index = top.permute(order), index.permute(order)
@@ -172,7 +175,7 @@ def _lp_fwd_fake(logits, target, top_k, ignore_index):
 
 
 _register("class_log_probs_fwd(Tensor logits, Tensor? target, int top_k, int ignore_index) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
-          class_log_probs_fwd, _lp_fwd_fake)
+          lambda logits, target, top_k, ignore_index: class_log_probs_fwd(logits, target, top_k, ignore_index), _lp_fwd_fake)
 
 
 def _lp_bwd_fake(logits, target, stats, entropy, top_indices, g_log_prob, g_entropy, g_top, ignore_index):

@@ -254,7 +254,7 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
  *   rows: L = 1, stride_c = 1 (tokens, classifier outputs, channels-last maps);  planes: stride_c >= max(L, 2) (NCHW maps).
  * All other arrays are contiguous: [N][L], and [N][k][L] for the alternatives (top_k <= min(ERF_TOP_MAX, C)).
  * fwd: log_prob = log softmax(z)[target] (0 where target == ignore_index, NaN for a target outside [0, C)); target and log_prob are
- *   both given or both NULL; entropy = -sum p log p; stats [2][N][L]: max z and log sum e^{z - max}, for bwd; alternatives in falling
+ *   both given or both NULL; entropy = -sum p log p; stats [2][N][L]: max z and log sum e^{z - max}, for bwd (NULL where none follows); alternatives in falling
  *   order of their value, equal ones by index, NaN first.
  * bwd: dlogits (same type, own strides, same kind of layout) = gl ([j = t] - p) - gh p (log p + entropy) + sum_k gk ([j = i_k] - p);
  *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits hold. */
