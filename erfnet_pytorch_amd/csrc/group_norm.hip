@@ -14,15 +14,15 @@ __device__ __forceinline__ float gn_u(float x, float mean, float a, float beta) 
 template <int ACT>
 __device__ __forceinline__ float gn_act(float u) {
     if (ACT == ERF_ACT_RELU) return u < 0.f ? 0.f : u;                  // NaN stays
-    if (ACT == ERF_ACT_SILU) return u / (1.f + __expf(-u));
+    if (ACT == ERF_ACT_SILU) return u * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
     return u;
 }
 template <int ACT>
 __device__ __forceinline__ float gn_slope(float u) {
     if (ACT == ERF_ACT_RELU) return u > 0.f ? 1.f : 0.f;
     if (ACT == ERF_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-u));
-        return s * (1.f + u * (1.f - s));
+        const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
+        return s * fmaf(u, 1.f - s, 1.f);
     }
     return 1.f;
 }
@@ -31,120 +31,473 @@ struct GnArgs {
     const void *x, *dy;
     void *y, *dx;
     const float *gamma, *beta;
-    float *mean, *rstd, *dgamma, *dbeta, *sums;       // sums: [N][C][2] of A, B
+    float *mean, *rstd, *dgamma, *dbeta;
+    float* parts;                      // [N][P][C][2]: forward mean and sum of squares about it, backward A and B, of a run of pixels
+    float* sums;                       // [N][C][2]: A, B;  then [N][G][2]: s1 / M, s2 / M
     long long HW;
-    int N, C, G;
+    int N, C, G, P;
+    int chunks, lanes;                 // a pixel's chunks of VEC channels in one workgroup, and the pixels side by side in it
     float eps;
 };
 
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
-}
-
-// One workgroup per (image, group): three passes over the group's values.
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void gn_fwd_group_kernel(const GnArgs a) {
-    __shared__ float sh[4];
-    const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
-    const T* x = (const T*)a.x + (long long)n * a.HW * a.C + g * cpg;
-    T* y = (T*)a.y + (long long)n * a.HW * a.C + g * cpg;
-    const long long m = a.HW * cpg;
-    float s = 0.f;
-    for (long long i = threadIdx.x; i < m; i += 256) s += Elem<T>::ld(x + i / cpg * a.C + i % cpg);
-    const float mean = block_sum(s, sh) / (float)m;
-    s = 0.f;
-    for (long long i = threadIdx.x; i < m; i += 256) {
-        const float d = Elem<T>::ld(x + i / cpg * a.C + i % cpg) - mean;
-        s += d * d;
-    }
-    const float rstd = 1.f / sqrtf(block_sum(s, sh) / (float)m + a.eps);
-    if (threadIdx.x == 0) { a.mean[blockIdx.x] = mean; a.rstd[blockIdx.x] = rstd; }
-    for (long long i = threadIdx.x; i < m; i += 256) {
-        const int c = g * cpg + (int)(i % cpg);
-        const long long at = i / cpg * a.C + i % cpg;
-        const float u = gn_u(Elem<T>::ld(x + at), mean, rstd * (a.gamma ? a.gamma[c] : 1.f), a.beta ? a.beta[c] : 0.f);
-        Elem<T>::st(y + at, gn_act<ACT>(u));
-    }
-}
-
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void gn_bwd_group_kernel(const GnArgs a) {
-    __shared__ float sh[4];
-    const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
-    const T* x = (const T*)a.x + (long long)n * a.HW * a.C;
-    const T* dy = (const T*)a.dy + (long long)n * a.HW * a.C;
-    T* dx = (T*)a.dx + (long long)n * a.HW * a.C;
-    const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x], m = (float)(a.HW * cpg);
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = g * cpg; c < (g + 1) * cpg; ++c) {
-        const float gamma = a.gamma ? a.gamma[c] : 1.f, beta = a.beta ? a.beta[c] : 0.f;
-        float p = 0.f, q = 0.f;
-        for (long long i = threadIdx.x; i < a.HW; i += 256) {
-            const float v = Elem<T>::ld(x + i * a.C + c);
-            const float du = Elem<T>::ld(dy + i * a.C + c) * gn_slope<ACT>(gn_u(v, mean, rstd * gamma, beta));
-            p += du;
-            q += du * ((v - mean) * rstd);
-        }
-        p = block_sum(p, sh);
-        q = block_sum(q, sh);
-        if (threadIdx.x == 0) { a.sums[2 * ((long long)n * a.C + c)] = p; a.sums[2 * ((long long)n * a.C + c) + 1] = q; }
-        s1 += gamma * p;
-        s2 += gamma * q;
-    }
-    s1 /= m;
-    s2 /= m;
-    for (int c = g * cpg; c < (g + 1) * cpg; ++c) {
-        const float gamma = a.gamma ? a.gamma[c] : 1.f, beta = a.beta ? a.beta[c] : 0.f;
-        for (long long i = threadIdx.x; i < a.HW; i += 256) {
-            const float v = Elem<T>::ld(x + i * a.C + c);
-            const float du = Elem<T>::ld(dy + i * a.C + c) * gn_slope<ACT>(gn_u(v, mean, rstd * gamma, beta));
-            Elem<T>::st(dx + i * a.C + c, rstd * (gamma * du - s1 - (v - mean) * rstd * s2));
+// VEC neighbouring channels of one pixel
+template <typename T, int VEC> __device__ __forceinline__ void vec_load(const T* p, float* f) {
+    if constexpr (VEC == 1) f[0] = Elem<T>::ld(p);
+    else if constexpr (sizeof(T) == 4) {
+        typedef __attribute__((ext_vector_type(VEC))) float V;
+        const V v = *(const V*)p;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = v[e];
+    } else if constexpr (VEC == 2) {
+        const unsigned r = *(const unsigned*)p;
+        f[0] = __uint_as_float(r << 16);
+        f[1] = __uint_as_float(r & 0xFFFF0000u);
+    } else {
+        typedef __attribute__((ext_vector_type(VEC / 2))) int V;
+        const V v = *(const V*)p;
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+            f[2 * e] = __uint_as_float((unsigned)v[e] << 16);
+            f[2 * e + 1] = __uint_as_float((unsigned)v[e] & 0xFFFF0000u);
         }
     }
 }
-
-// dbeta = sum_n A, dgamma = sum_n B
-__global__ void gn_param_grads_kernel(const GnArgs a) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= a.C) return;
-    double p = 0, q = 0;
-    for (int n = 0; n < a.N; ++n) {
-        p += a.sums[2 * ((long long)n * a.C + c)];
-        q += a.sums[2 * ((long long)n * a.C + c) + 1];
+template <typename T, int VEC> __device__ __forceinline__ void vec_store(T* p, const float* f) {
+    if constexpr (VEC == 1) Elem<T>::st(p, f[0]);
+    else if constexpr (sizeof(T) == 4) {
+        typedef __attribute__((ext_vector_type(VEC))) float V;
+        V v;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = f[e];
+        *(V*)p = v;
+    } else if constexpr (VEC == 2) {
+        *(int*)p = pack_bf16x2(f[0], f[1]);
+    } else {
+        typedef __attribute__((ext_vector_type(VEC / 2))) int V;
+        V v;
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) v[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+        *(V*)p = v;
     }
-    if (a.dbeta) a.dbeta[c] = (float)p;
-    if (a.dgamma) a.dgamma[c] = (float)q;
+}
+
+// A workgroup takes a run of pixels of one image (and, where a pixel has more than 256 chunks, 256 of them): thread = (pixel lane,
+// chunk), so that a thread keeps its channels and the workgroup reads whole pixels side by side.
+#define GN_THREADS 256
+#define GN_UNROLL 8
+struct GnPlace { int n, run, chunk, lane, c; long long first, last; bool on; };        // c: first channel; pixels [first, last) of image n
+template <int VEC> __device__ __forceinline__ GnPlace gn_place(const GnArgs& a) {
+    GnPlace q;
+    q.n = blockIdx.x / (unsigned)a.P;
+    q.run = blockIdx.x - q.n * a.P;
+    q.lane = threadIdx.x / a.chunks;
+    q.chunk = threadIdx.x - q.lane * a.chunks;
+    q.c = (blockIdx.y * a.chunks + q.chunk) * VEC;
+    q.on = q.lane < a.lanes && q.c < a.C;
+    const long long per = (a.HW + a.P - 1) / a.P;
+    q.first = q.run * per;
+    q.last = q.first + per < a.HW ? q.first + per : a.HW;
+    return q;
+}
+
+// Mean, sum of squares about it and count of two sets of values as those of their union
+__device__ __forceinline__ void gn_join(float& mean, float& m2, float& n, float omean, float om2, float on) {
+    const float all = n + on;
+    if (all > 0.f) {
+        const float d = omean - mean, w = on / all;
+        mean = fmaf(d, w, mean);
+        m2 += om2 + d * d * (n * w);
+        n = all;
+    }
+}
+
+// Forward statistics of a run of pixels.  A thread sums UNROLL pixels of a channel, then their squares about their own mean, and joins
+// that to what it has: no shift has to be guessed and no large squares cancel.
+template <typename T, int VEC>
+__global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnArgs a) {
+    __shared__ float sh[2][VEC][GN_THREADS], shn[GN_THREADS];
+    const GnPlace q = gn_place<VEC>(a);
+    const T* x = (const T*)a.x + (long long)q.n * a.HW * a.C + q.c;
+    float mean[VEC], m2[VEC], n = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) mean[e] = m2[e] = 0.f;
+    if (q.on) {
+        long long p = q.first + q.lane;
+        for (; p + (GN_UNROLL - 1) * a.lanes < q.last; p += GN_UNROLL * a.lanes) {
+            float f[GN_UNROLL][VEC];
+#pragma unroll
+            for (int u = 0; u < GN_UNROLL; ++u) vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+            const float all = n + GN_UNROLL, w = GN_UNROLL / all, nw = n * w;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float s = 0.f, r = 0.f;
+#pragma unroll
+                for (int u = 0; u < GN_UNROLL; ++u) s += f[u][e];
+                s *= 1.f / GN_UNROLL;
+#pragma unroll
+                for (int u = 0; u < GN_UNROLL; ++u) r = fmaf(f[u][e] - s, f[u][e] - s, r);
+                const float d = s - mean[e];
+                mean[e] = fmaf(d, w, mean[e]);
+                m2[e] += r + d * d * nw;
+            }
+            n = all;
+        }
+        for (; p < q.last; p += a.lanes) {
+            float f[VEC];
+            vec_load<T, VEC>(x + p * a.C, f);
+            const float w = 1.f / (n + 1.f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = f[e] - mean[e];
+                mean[e] = fmaf(d, w, mean[e]);
+                m2[e] = fmaf(d * d, n * w, m2[e]);
+            }
+            n += 1.f;
+        }
+    }
+    // the pixel lanes in halves
+    for (int have = a.lanes; have > 1;) {
+        const int keep = (have + 1) / 2;
+        __syncthreads();
+        if (q.on && q.lane >= keep && q.lane < have) {
+            shn[threadIdx.x] = n;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { sh[0][e][threadIdx.x] = mean[e]; sh[1][e][threadIdx.x] = m2[e]; }
+        }
+        __syncthreads();
+        if (q.on && q.lane + keep < have) {
+            const int o = threadIdx.x + keep * a.chunks;
+            const float on = shn[o], all = n + on, w = all > 0.f ? on / all : 0.f, nw = n * w;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = sh[0][e][o] - mean[e];
+                mean[e] = fmaf(d, w, mean[e]);
+                m2[e] += sh[1][e][o] + d * d * nw;
+            }
+            n = all;
+        }
+        have = keep;
+    }
+    if (q.on && q.lane == 0) {
+        float* out = a.parts + 2 * (((long long)q.n * a.P + q.run) * a.C + q.c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { out[2 * e] = mean[e]; out[2 * e + 1] = m2[e]; }
+    }
+}
+
+// One workgroup per (image, group): the group's channels and runs of pixels joined to its mean and 1 / sqrt(var + eps)
+__global__ __launch_bounds__(1024) void gn_finalize_kernel(const GnArgs a) {
+    __shared__ float sh[3][16];
+    const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
+    const long long per = (a.HW + a.P - 1) / a.P;
+    float mean = 0.f, m2 = 0.f, count = 0.f;
+    for (long long i = threadIdx.x; i < (long long)a.P * cpg; i += 1024) {
+        const long long p = i / cpg, c = g * cpg + (i - p * cpg), left = a.HW - p * per;
+        const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.P + p) * a.C + c));
+        gn_join(mean, m2, count, v.x, v.y, left <= 0 ? 0.f : (float)(left < per ? left : per));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) gn_join(mean, m2, count, __shfl_xor(mean, o, 64), __shfl_xor(m2, o, 64), __shfl_xor(count, o, 64));
+    if ((threadIdx.x & 63) == 0) { sh[0][threadIdx.x >> 6] = mean; sh[1][threadIdx.x >> 6] = m2; sh[2][threadIdx.x >> 6] = count; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) gn_join(mean, m2, count, sh[0][w], sh[1][w], sh[2][w]);
+        a.mean[blockIdx.x] = mean;
+        a.rstd[blockIdx.x] = 1.f / sqrtf(m2 / ((float)a.HW * cpg) + a.eps);
+    }
+}
+
+// A thread's channels: mean, rstd gamma and beta of each
+template <int VEC>
+__device__ __forceinline__ void gn_channels(const GnArgs& a, const GnPlace& q, float* mean, float* scale, float* beta) {
+    const int cpg = a.C / a.G;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const int c = q.c + e, g = c / cpg;
+        mean[e] = a.mean[(long long)q.n * a.G + g];
+        scale[e] = a.rstd[(long long)q.n * a.G + g] * (a.gamma ? a.gamma[c] : 1.f);
+        beta[e] = a.beta ? a.beta[c] : 0.f;
+    }
+}
+
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnArgs a) {
+    constexpr int U = 4;
+    const GnPlace q = gn_place<VEC>(a);
+    if (!q.on) return;
+    const T* x = (const T*)a.x + (long long)q.n * a.HW * a.C + q.c;
+    T* y = (T*)a.y + (long long)q.n * a.HW * a.C + q.c;
+    float mean[VEC], scale[VEC], beta[VEC];
+    gn_channels<VEC>(a, q, mean, scale, beta);
+    for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
+        float f[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (p + u * a.lanes < q.last) vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (p + u * a.lanes < q.last) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f[u][e] = gn_act<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
+                vec_store<T, VEC>(y + (p + u * a.lanes) * a.C, f[u]);
+            }
+    }
+}
+
+// Backward sums A, B of a run of pixels
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const GnArgs a) {
+    constexpr int U = 4;
+    __shared__ float sh[2][VEC][GN_THREADS];
+    const GnPlace q = gn_place<VEC>(a);
+    const long long at = (long long)q.n * a.HW * a.C + q.c;
+    const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
+    float s[VEC], r[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s[e] = r[e] = 0.f;
+    if (q.on) {
+        float mean[VEC], scale[VEC], beta[VEC];
+        gn_channels<VEC>(a, q, mean, scale, beta);
+        for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
+            float f[U][VEC], d[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p + u * a.lanes < q.last) {
+                    vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+                    vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
+                }
+            float ls[VEC], lr[VEC];                                    // these few first: shorter chains of roundings
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) ls[e] = lr[e] = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (p + u * a.lanes < q.last) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
+                        ls[e] += du;
+                        lr[e] = fmaf(du, f[u][e] - mean[e], lr[e]);
+                    }
+                }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { s[e] += ls[e]; r[e] += lr[e]; }
+        }
+        const int cpg = a.C / a.G;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) r[e] *= a.rstd[(long long)q.n * a.G + (q.c + e) / cpg];
+    }
+    for (int have = a.lanes; have > 1;) {
+        const int keep = (have + 1) / 2;
+        __syncthreads();
+        if (q.on && q.lane >= keep && q.lane < have) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { sh[0][e][threadIdx.x] = s[e]; sh[1][e][threadIdx.x] = r[e]; }
+        }
+        __syncthreads();
+        if (q.on && q.lane + keep < have) {
+            const int o = threadIdx.x + keep * a.chunks;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { s[e] += sh[0][e][o]; r[e] += sh[1][e][o]; }
+        }
+        have = keep;
+    }
+    if (q.on && q.lane == 0) {
+        float* out = a.parts + 2 * (((long long)q.n * a.P + q.run) * a.C + q.c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { out[2 * e] = s[e]; out[2 * e + 1] = r[e]; }
+    }
+}
+
+// One workgroup per (image, group): A and B of its channels over the runs of pixels, s1 / M and s2 / M over the channels.  Threads are
+// (run lane, channel) with the channels side by side in memory; 1024 channels at a time.
+__global__ __launch_bounds__(1024) void gn_bwd_finalize_kernel(const GnArgs a) {
+    __shared__ double sh[2][1024];
+    const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
+    const int side = cpg < 1024 ? cpg : 1024, lanes = 1024 / side, lane = threadIdx.x / side, j = threadIdx.x - lane * side;
+    double s1 = 0, s2 = 0;
+    for (int c0 = 0; c0 < cpg; c0 += side) {
+        const int c = g * cpg + c0 + j;
+        const bool on = lane < lanes && c0 + j < cpg;
+        double p = 0, r = 0;
+        if (on)
+            for (int i = lane; i < a.P; i += lanes) {
+                const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.P + i) * a.C + c));
+                p += v.x;
+                r += v.y;
+            }
+        for (int have = lanes; have > 1;) {
+            const int keep = (have + 1) / 2;
+            __syncthreads();
+            if (lane >= keep && lane < have) { sh[0][threadIdx.x] = p; sh[1][threadIdx.x] = r; }
+            __syncthreads();
+            if (lane + keep < have) { p += sh[0][threadIdx.x + keep * side]; r += sh[1][threadIdx.x + keep * side]; }
+            have = keep;
+        }
+        if (on && lane == 0) {
+            a.sums[2 * ((long long)n * a.C + c)] = (float)p;
+            a.sums[2 * ((long long)n * a.C + c) + 1] = (float)r;
+            const double gamma = a.gamma ? a.gamma[c] : 1.f;
+            s1 += gamma * p;
+            s2 += gamma * r;
+        }
+    }
+    __syncthreads();
+    sh[0][threadIdx.x] = s1;
+    sh[1][threadIdx.x] = s2;
+    for (int o = 512; o > 0; o >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < o) { sh[0][threadIdx.x] += sh[0][threadIdx.x + o]; sh[1][threadIdx.x] += sh[1][threadIdx.x + o]; }
+    }
+    if (threadIdx.x == 0) {
+        const double m = (double)a.HW * cpg;
+        float* out = a.sums + 2 * (long long)a.N * a.C + 2 * (long long)blockIdx.x;
+        out[0] = (float)(sh[0][0] / m);
+        out[1] = (float)(sh[1][0] / m);
+    }
+}
+
+// dx; and, by the workgroups behind those of the last run, dbeta = sum_n A and dgamma = sum_n B: 64 channels each, four image lanes
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnArgs a) {
+    constexpr int U = 4;
+    if (blockIdx.x >= (unsigned)(a.N * a.P)) {
+        __shared__ double sh[2][GN_THREADS];
+        if (blockIdx.y) return;
+        const int c = (int)(blockIdx.x - (unsigned)(a.N * a.P)) * 64 + (threadIdx.x & 63);
+        double p = 0, r = 0;
+        if (c < a.C)
+            for (int n = threadIdx.x >> 6; n < a.N; n += 4) {
+                const float2 v = *(const float2*)(a.sums + 2 * ((long long)n * a.C + c));
+                p += v.x;
+                r += v.y;
+            }
+        sh[0][threadIdx.x] = p;
+        sh[1][threadIdx.x] = r;
+        __syncthreads();
+        if (threadIdx.x < 64 && c < a.C) {
+            for (int w = 1; w < 4; ++w) { p += sh[0][threadIdx.x + 64 * w]; r += sh[1][threadIdx.x + 64 * w]; }
+            if (a.dbeta) a.dbeta[c] = (float)p;
+            if (a.dgamma) a.dgamma[c] = (float)r;
+        }
+        return;
+    }
+    const GnPlace q = gn_place<VEC>(a);
+    if (!q.on) return;
+    const long long at = (long long)q.n * a.HW * a.C + q.c;
+    const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
+    T* dx = (T*)a.dx + at;
+    float mean[VEC], scale[VEC], beta[VEC], k1[VEC], k2[VEC];          // dx = scale du - k1 - (x - mean) k2
+    gn_channels<VEC>(a, q, mean, scale, beta);
+    const int cpg = a.C / a.G;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const long long g = (long long)q.n * a.G + (q.c + e) / cpg;
+        const float2 m = *(const float2*)(a.sums + 2 * (long long)a.N * a.C + 2 * g);
+        const float rstd = a.rstd[g];
+        k1[e] = rstd * m.x;
+        k2[e] = rstd * rstd * m.y;
+    }
+    for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
+        float f[U][VEC], d[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (p + u * a.lanes < q.last) {
+                vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+                vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (p + u * a.lanes < q.last) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
+                    d[u][e] = fmaf(scale[e], du, -fmaf(f[u][e] - mean[e], k2[e], k1[e]));
+                }
+                vec_store<T, VEC>(dx + (p + u * a.lanes) * a.C, d[u]);
+            }
+    }
 }
 
 static inline bool gn_shape_ok(int dtype, int N, long long HW, int C, int groups, int act) {
-    return (dtype == ERF_F32 || dtype == ERF_BF16) && N > 0 && HW > 0 && C > 0 && groups > 0 && C % groups == 0 && act >= 0 && act <= 2 &&
-           (long long)N * groups <= 0x7FFFFFFFll && HW <= (1ll << 40) / C;
+    return (dtype == ERF_F32 || dtype == ERF_BF16) && N > 0 && N <= (1 << 24) && HW > 0 && C > 0 && groups > 0 && C % groups == 0 && act >= 0 &&
+           act <= 2 && (long long)N * groups <= 0x7FFFFFFFll && C <= (1 << 20) && HW <= (1ll << 40) / C;
 }
 
-#define GN_PICK(KERNEL, GRID)                                                                                               \
-    do {                                                                                                                    \
-        hipStream_t s = (hipStream_t)stream;                                                                                \
-        const dim3 grid(GRID), block(256);                                                                                  \
-        if (dtype == ERF_F32) {                                                                                             \
-            if (act == ERF_ACT_RELU) hipLaunchKernelGGL((KERNEL<float, ERF_ACT_RELU>), grid, block, 0, s, a);               \
-            else if (act == ERF_ACT_SILU) hipLaunchKernelGGL((KERNEL<float, ERF_ACT_SILU>), grid, block, 0, s, a);          \
-            else hipLaunchKernelGGL((KERNEL<float, ERF_ACT_NONE>), grid, block, 0, s, a);                                   \
-        } else {                                                                                                            \
-            if (act == ERF_ACT_RELU) hipLaunchKernelGGL((KERNEL<bf16raw, ERF_ACT_RELU>), grid, block, 0, s, a);             \
-            else if (act == ERF_ACT_SILU) hipLaunchKernelGGL((KERNEL<bf16raw, ERF_ACT_SILU>), grid, block, 0, s, a);        \
-            else hipLaunchKernelGGL((KERNEL<bf16raw, ERF_ACT_NONE>), grid, block, 0, s, a);                                 \
-        }                                                                                                                   \
+// Channels per access: the most that divide C, fit 16 bytes and lie on their boundaries
+static inline int gn_vec(int dtype, int C, unsigned long long addresses) {
+    const int size = dtype == ERF_BF16 ? 2 : 4;
+    int v = 16 / size;
+    while (v > 1 && (C % v || addresses % (v * size))) v /= 2;
+    return v;
+}
+// Runs of pixels per image: about 1024 workgroups in all, each thread with a few sets of loads, at most 512 runs to be joined
+static inline int gn_runs(int N, long long HW, int lanes, int slabs) {
+    const long long want = (1024 + (long long)N * slabs - 1) / ((long long)N * slabs), most = (HW + (long long)lanes * GN_UNROLL - 1) / ((long long)lanes * GN_UNROLL);
+    const long long p = want < most ? want : most;
+    return (int)(p < 1 ? 1 : p > 512 ? 512 : p);
+}
+#define GN_MAX_RUNS 512
+
+template <int VEC> static inline void gn_plan(GnArgs& a, dim3& grid) {
+    const int chunks = a.C / VEC;
+    a.chunks = chunks < GN_THREADS ? chunks : GN_THREADS;
+    a.lanes = GN_THREADS / a.chunks;
+    const int slabs = (chunks + a.chunks - 1) / a.chunks;
+    a.P = gn_runs(a.N, a.HW, a.lanes, slabs);
+    grid = dim3((unsigned)a.P * (unsigned)a.N, (unsigned)slabs);
+}
+
+template <typename T, int VEC, int ACT>
+static void gn_fwd_launch(GnArgs a, hipStream_t s) {
+    dim3 grid;
+    gn_plan<VEC>(a, grid);
+    hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), grid, dim3(GN_THREADS), 0, s, a);
+    hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+}
+
+template <typename T, int VEC, int ACT>
+static void gn_bwd_launch(GnArgs a, hipStream_t s) {
+    dim3 grid;
+    gn_plan<VEC>(a, grid);
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+    hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
+    grid.x += (unsigned)((a.C + 63) / 64);
+    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+}
+
+#define GN_ACT(FN, T, VEC)                                            \
+    do {                                                              \
+        if (act == ERF_ACT_RELU) FN<T, VEC, ERF_ACT_RELU>(a, s);      \
+        else if (act == ERF_ACT_SILU) FN<T, VEC, ERF_ACT_SILU>(a, s); \
+        else FN<T, VEC, ERF_ACT_NONE>(a, s);                          \
+    } while (0)
+#define GN_PICK(FN, VECTOR)                                                           \
+    do {                                                                              \
+        hipStream_t s = (hipStream_t)stream;                                          \
+        const int v = VECTOR;                                                         \
+        if (dtype == ERF_F32) {                                                       \
+            if (v == 4) GN_ACT(FN, float, 4);                                         \
+            else if (v == 2) GN_ACT(FN, float, 2);                                    \
+            else GN_ACT(FN, float, 1);                                                \
+        } else {                                                                      \
+            if (v == 8) GN_ACT(FN, bf16raw, 8);                                       \
+            else if (v == 4) GN_ACT(FN, bf16raw, 4);                                  \
+            else if (v == 2) GN_ACT(FN, bf16raw, 2);                                  \
+            else GN_ACT(FN, bf16raw, 1);                                              \
+        }                                                                             \
     } while (0)
 
 extern "C" {
 
 size_t erf_group_norm_workspace_bytes(int dtype, int N, long long HW, int C, int groups) {
     if (!gn_shape_ok(dtype, N, HW, C, groups, 0)) return 0;
-    return (size_t)N * C * 2 * sizeof(float);
+    // the runs of one of the plans (which one depends on the addresses), and the per-channel and per-group sums
+    long long runs = (HW + GN_UNROLL - 1) / GN_UNROLL;
+    const long long want = (1024 + N - 1) / N;
+    runs = runs < want ? runs : want;
+    runs = runs < GN_MAX_RUNS ? runs : GN_MAX_RUNS;
+    return ((size_t)N * (size_t)runs * C + (size_t)N * C + (size_t)N * groups) * 2 * sizeof(float);
 }
 
 int erf_group_norm_fwd(const void* x, void* y, int dtype, int N, long long HW, int C, int groups, const float* gamma, const float* beta,
@@ -152,7 +505,9 @@ int erf_group_norm_fwd(const void* x, void* y, int dtype, int N, long long HW, i
     if (!x || !y || !mean || !rstd || !workspace || !(eps >= 0) || !gn_shape_ok(dtype, N, HW, C, groups, act)) return ERF_EINVAL;
     GnArgs a = {};
     a.x = x; a.y = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.rstd = rstd; a.HW = HW; a.N = N; a.C = C; a.G = groups; a.eps = eps;
-    GN_PICK(gn_fwd_group_kernel, (unsigned)(N * groups));
+    a.sums = (float*)workspace;
+    a.parts = a.sums + 2 * ((size_t)N * C + (size_t)N * groups);
+    GN_PICK(gn_fwd_launch, gn_vec(dtype, C, (unsigned long long)x | (unsigned long long)y));
     return erf_check_launch();
 }
 
@@ -162,9 +517,10 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
     if (!x || !dy || !dx || !mean || !rstd || !workspace || !gn_shape_ok(dtype, N, HW, C, groups, act)) return ERF_EINVAL;
     GnArgs a = {};
     a.x = x; a.dy = dy; a.dx = dx; a.gamma = gamma; a.beta = beta; a.mean = (float*)mean; a.rstd = (float*)rstd; a.dgamma = dgamma;
-    a.dbeta = dbeta; a.sums = (float*)workspace; a.HW = HW; a.N = N; a.C = C; a.G = groups;
-    GN_PICK(gn_bwd_group_kernel, (unsigned)(N * groups));
-    if (dgamma || dbeta) hipLaunchKernelGGL(gn_param_grads_kernel, dim3((C + 255) / 256), dim3(256), 0, (hipStream_t)stream, a);
+    a.dbeta = dbeta; a.HW = HW; a.N = N; a.C = C; a.G = groups;
+    a.sums = (float*)workspace;
+    a.parts = a.sums + 2 * ((size_t)N * C + (size_t)N * groups);
+    GN_PICK(gn_bwd_launch, gn_vec(dtype, C, (unsigned long long)x | (unsigned long long)dy | (unsigned long long)dx));
     return erf_check_launch();
 }
 
