@@ -79,29 +79,6 @@ class ClassLogProbs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
-class _ClassLogProbsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, target, top_k, ignore_index):
-        log_prob, entropy, stats, top, index = train_ops.class_log_probs_fwd(logits, target, top_k, ignore_index)
-        ctx.save_for_backward(logits, target, stats, entropy, index)
-        ctx.ignore_index = ignore_index
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(index)
-        return log_prob, entropy, top, index
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_log_prob, g_entropy, g_top, _):
-        logits, target, stats, entropy, index = ctx.saved_tensors
-        if target is None:
-            g_log_prob = None
-        if not index.shape[1]:
-            g_top = None
-        if g_log_prob is None and g_entropy is None and g_top is None:
-            return None, None, None, None
-        return train_ops.class_log_probs_bwd(logits, target, stats, entropy, index, g_log_prob, g_entropy, g_top, ctx.ignore_index), None, None, None
-
-
 def class_log_probs(logits, target=None, top_k=0, ignore_index=-100):
     """Log probability of the target class, entropy and the `top_k` most probable classes at every position, in one pass.
 
@@ -118,9 +95,5 @@ def class_log_probs(logits, target=None, top_k=0, ignore_index=-100):
     A logit of -inf has probability 0 and takes no part.  A position without any finite logit, or with +inf or NaN among its
     logits, has no distribution: its log_prob (if not ignored), entropy and top_log_probs are NaN, as log_softmax's.
     """
-    ops.require_gpu(logits, "class_log_probs")
-    if logits.requires_grad and torch.is_grad_enabled():
-        log_prob, entropy, top, index = _ClassLogProbsFn.apply(logits, target, int(top_k), int(ignore_index))
-    else:
-        log_prob, entropy, _, top, index = train_ops.class_log_probs_fwd(logits, target, int(top_k), int(ignore_index), False)
+    log_prob, entropy, top, index = train_ops._host.class_log_probs(logits, target, top_k, ignore_index)
     return ClassLogProbs(None if target is None else log_prob, entropy, top if top_k else None, index if top_k else None)

@@ -9,27 +9,9 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import ops, train_ops
+from .train_ops import _host
 
-ACTIVATIONS = train_ops.ACTIVATIONS
-
-
-class _GroupNormActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, activation):
-        last = train_ops.channels_last(x)
-        y, mean, rstd = train_ops.group_norm_act_fwd(last, weight, bias, groups, eps, activation)
-        ctx.save_for_backward(last, weight, bias, mean, rstd)
-        ctx.config = (groups, activation)
-        return y.movedim(-1, 1)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        last, weight, bias, mean, rstd = ctx.saved_tensors
-        dx, dweight, dbias = train_ops.group_norm_act_bwd(train_ops.channels_last(dy), last, weight, bias, mean, rstd, *ctx.config)
-        return (dx.movedim(-1, 1), None if weight is None else dweight.to(weight.dtype), None if bias is None else dbias.to(bias.dtype),
-                None, None, None)
+ACTIVATIONS = ("none", "relu", "silu")
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="relu"):
@@ -39,10 +21,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
     x [N, C, ...] fp32 or bf16, read where it lies if its memory is channels-last, else copied; the result has x's type and
     channels-last memory.  weight, bias [C] or None; statistics and parameter gradients are fp32.  activation: "none", "relu" or
     "silu".  Differentiable (once) in x, weight and bias."""
-    ops.require_gpu(x, "group_norm_act")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
-        return _GroupNormActFn.apply(x, weight, bias, int(num_groups), float(eps), activation)
-    return train_ops.group_norm_act_fwd(train_ops.channels_last(x), weight, bias, int(num_groups), float(eps), activation)[0].movedim(-1, 1)
+    return _host.group_norm_act(x, num_groups, weight, bias, eps, activation)
 
 
 class GroupNormAct2d(nn.Module):
@@ -53,7 +32,7 @@ class GroupNormAct2d(nn.Module):
         if num_groups < 1 or num_channels % num_groups:
             raise ValueError(f"num_channels ({num_channels}) is a multiple of num_groups ({num_groups})")
         if activation not in ACTIVATIONS:
-            raise ValueError(f"activation is one of {sorted(ACTIVATIONS)}, got {activation!r}")
+            raise ValueError(f"activation is one of {ACTIVATIONS}, got {activation!r}")
         self.num_groups, self.num_channels, self.eps, self.affine, self.activation = num_groups, num_channels, eps, affine, activation
         if affine:
             self.weight, self.bias = nn.Parameter(torch.ones(num_channels)), nn.Parameter(torch.zeros(num_channels))

@@ -23,15 +23,13 @@ bf16 step (2^-9 of the value) are lost: keep fp32 parameters where such changes 
 """
 from __future__ import annotations
 
-import ctypes
-import operator
-
+import numpy as np
 import torch
+from torch.optim import optimizer as _torch_optimizer
 
 from . import ops
 from ._lib import BF16, F32, call, size_query
-
-_data_ptr = torch.Tensor.data_ptr
+from .train_ops import _host
 
 
 class _Plan:
@@ -39,7 +37,7 @@ class _Plan:
 
     def __init__(self, device, code):
         self.device, self.code = device, code
-        self.params, self.bases = [], []
+        self.params, self.bases, self.which = [], [], []        # which: places among all parameters with a gradient
         self.captured = False                           # a captured launch may write the grad fields at any time
 
 
@@ -55,7 +53,8 @@ class AdamW(torch.optim.Optimizer):
         self._plans = None                              # [[_Plan, ...] per group], None: to be built
         self._lr = []                                   # per group: [value on the devices, {device: double tensor}]
         self._kept = []                                 # what captured launches still read
-        self._copies, self._copies_captured = [], False
+        self._copies, self._copies_captured = {}, False
+        self._watch = _host.ParamWatch()
 
     def __getstate__(self):
         self._write_back_steps()
@@ -126,7 +125,7 @@ class AdamW(torch.optim.Optimizer):
             for plan in plans:
                 counts = plan.steps.cpu()
                 for p, first in zip(plan.params, plan.first_chunk):
-                    self.state[p]["step"] = counts[first].float()
+                    self.state[p]["step"] = counts[int(first)].float()
 
     def _drop_plans(self):
         """Forget the device tables: the next step builds them anew from `state` and the parameters."""
@@ -165,8 +164,8 @@ class AdamW(torch.optim.Optimizer):
         self._plans = None                              # the loaded step counts stand
 
     # -- device tables --------------------------------------------------------------------------
-    def _build(self):
-        live = [p for g in self.param_groups for p in g["params"] if p.grad is not None and p.numel()]
+    def _build(self, groups):
+        live = [p for g in groups for p in g if p.grad is not None and p.numel()]
         for p in live:
             ops.require_gpu(p, "AdamW")
         if live and torch.cuda.is_current_stream_capturing():
@@ -174,63 +173,52 @@ class AdamW(torch.optim.Optimizer):
                                "run one step before the capture")
         self._drop_plans()
         chunk, block = size_query("erf_adamw_chunk_elements"), size_query("erf_adamw_scale_block")
-        plans, base = [], 0
-        for group in self.param_groups:
+        plans, base, place = [], 0, 0
+        for group in groups:
             mine = {}
-            for p in group["params"]:
+            for p in group:
                 if p.grad is not None and p.numel():
                     key = (p.device, F32 if p.dtype == torch.float32 else BF16)
                     plan = mine.setdefault(key, _Plan(*key))
                     plan.params.append(p)
                     plan.bases.append(base)
+                    plan.which.append(place)
+                    place += 1
                 base += -(-p.numel() // block) * block
             plans.append(list(mine.values()))
-        _no_overlap([p for ps in plans for plan in ps for p in plan.params])
+        _no_overlap(live)
         for ps in plans:
             for plan in ps:
-                rows, where, steps, plan.first_chunk, at = [], [], [], [], 0
-                for t, (p, b) in enumerate(zip(plan.params, plan.bases)):
+                rows, steps, plan.holds = [], [], []
+                for p, b in zip(plan.params, plan.bases):
                     st = self._state_of(p)
-                    second = st["exp_avg_sq"] if self.state_bits == 32 else st["exp_avg_sq_root"]
-                    scales = (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_root_scale"].data_ptr()) if self.state_bits == 8 else (0, 0)
-                    rows.append([p.data_ptr(), 0, st["exp_avg"].data_ptr(), second.data_ptr(), *scales, p.numel(), b])
-                    n = -(-p.numel() // chunk)
-                    plan.first_chunk.append(at)
-                    at += n
-                    where.append(torch.stack([torch.full((n,), t, dtype=torch.int32), torch.arange(n, dtype=torch.int32)], 1))
-                    steps.append(torch.full((n,), int(st["step"]), dtype=torch.int32))
-                plan.table = torch.tensor(rows, dtype=torch.int64).to(plan.device)
-                plan.chunks = torch.cat(where).to(plan.device)
-                plan.steps = torch.cat(steps).to(plan.device)
-                # the states that the table points at live as long as it does
-                plan.holds = [t for p in plan.params for t in self.state[p].values()] + [p.data for p in plan.params]
+                    names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
+                    own = [st[k] for k in names]
+                    rows.append([p.data_ptr(), 0, *(t.data_ptr() for t in own), *((0, 0) if self.state_bits == 32 else ()), p.numel(), b])
+                    steps.append(int(st["step"]))
+                    plan.holds += own                   # what the table points at lives as long as it does
+                    plan.holds.append(p.detach())
+                rows = np.array(rows, dtype=np.int64)
+                per = -(-rows[:, 6] // chunk)           # chunks of each tensor
+                plan.first_chunk = np.cumsum(per) - per
+                which = np.repeat(np.arange(len(per)), per)
+                where = np.stack([which, np.arange(len(which)) - plan.first_chunk[which]], 1).astype(np.int32)
+                plan.table = torch.from_numpy(rows).to(plan.device)
+                plan.chunks = torch.from_numpy(where).to(plan.device)
+                plan.steps = torch.from_numpy(np.array(steps, dtype=np.int32)[which]).to(plan.device)
+        self._watch.bind(groups)
         self._plans = plans
-        self._params = [p for ps in plans for plan in ps for p in plan.params]
-        self._ptrs = tuple(map(_data_ptr, self._params))
 
-    def _bind_grads(self, grads):
-        """Check new gradients and note the addresses for the tables."""
-        copies, used = [], []
-        for p, g in zip(self._params, grads):
-            if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
-                raise ValueError(f"AdamW: a gradient of a parameter {p.dtype} {tuple(p.shape)} has to be a dense tensor of the same type, "
-                                 f"shape and device, got {g.dtype} {tuple(g.shape)}")
-            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
-                own = torch.empty_like(p)               # other strides than the parameter's: a copy in its order, renewed every step
-                copies.append((own, g))
-                g = own
-            used.append(g)
+    def _copy_places(self):
+        """Gradients with other strides than their parameter's are copied into its order every step; where the copies lie."""
         if self._copies_captured:
             self._kept.append(self._copies)
-        self._copies, self._copies_captured = copies, False
-        at = 0
+        self._copies_captured = False
+        params = [p for _, p in sorted((i, p) for ps in self._plans for plan in ps for i, p in zip(plan.which, plan.params))] if self._watch.copied() else []
+        self._copies = {i: (torch.empty_like(params[i]).detach(), params[i]) for i in self._watch.copied()}
         for ps in self._plans:
             for plan in ps:
-                n = len(plan.params)
-                plan.grads = (ctypes.c_void_p * n)(*map(_data_ptr, used[at:at + n]))
-                plan.fresh = True
-                at += n
-        self._grads, self._grad_ptrs = grads, tuple(map(_data_ptr, grads))
+                plan.copies = [self._copies[i][0].data_ptr() if i in self._copies else 0 for i in plan.which]
 
     def refresh_lr(self):
         """Bring the learning rates to the device.  step() does so by itself; a program that replays a captured step calls this
@@ -263,62 +251,60 @@ class AdamW(torch.optim.Optimizer):
         ops.bump_param_epoch()
 
     # -- the step -------------------------------------------------------------------------------
-    @torch.no_grad()
-    def step(self, closure=None):
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        grads = [p.grad for g in self.param_groups for p in g["params"]]
-        if self._plans is None or not self._same(grads):
-            self._build()
-            self._bind_grads([p.grad for p in self._params])
-            self._all_grads, self._without = grads, [g is None for g in grads]
-        if not self._params:
+        groups = [g["params"] for g in self.param_groups]
+        seen = 2 if self._plans is None else self._watch.look(groups)
+        if seen:
+            with torch.no_grad():
+                if seen == 2:
+                    self._build(groups)
+                    self._watch.look(groups)
+                self._copy_places()
+        if not any(self._plans):
             return loss
         capturing = torch.cuda.is_current_stream_capturing()
         if self._copies:
             self._copies_captured = self._copies_captured or capturing
-            for own, g in self._copies:
-                own.copy_(g)
+            with torch.no_grad():
+                for own, p in self._copies.values():
+                    own.copy_(p.grad)
         self.refresh_lr()
         for group, where, plans in zip(self.param_groups, self._lr, self._plans):
             for plan in plans:
                 if plan.device.index == torch._C._cuda_getDevice():
-                    self._launch(group, where[1][plan.device], plan, capturing)
+                    self._launch(group, where[1][plan.device], plan, seen, capturing)
                 else:
                     with torch.cuda.device(plan.device):
-                        self._launch(group, where[1][plan.device], plan, capturing)
-        torch.autograd.graph.increment_version(self._params)
+                        self._launch(group, where[1][plan.device], plan, seen, capturing)
+        self._watch.bump()
         ops.bump_param_epoch()                          # the parameters changed through raw pointers
         return loss
 
-    def _same(self, grads):
-        """Whether the tables describe these gradients, and the parameters are where they were; new gradients of the same
-        parameters are bound on the way."""
-        if len(grads) != len(self._all_grads):
-            return False
-        if all(map(operator.is_, grads, self._all_grads)):
-            if tuple(map(_data_ptr, self._params)) != self._ptrs:
-                return False
-            if tuple(map(_data_ptr, self._grads)) != self._grad_ptrs:
-                self._bind_grads(self._grads)
-            return True
-        if [g is None for g in grads] != self._without or tuple(map(_data_ptr, self._params)) != self._ptrs:
-            return False
-        self._bind_grads([p.grad for p in self._params])
-        self._all_grads = grads
-        return True
+    def step(self, closure=None):
+        """One update of every parameter that has a gradient."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _torch_optimizer._global_optimizer_pre_hooks or \
+                _torch_optimizer._global_optimizer_post_hooks:
+            return _hooked_step(self, closure)
+        return self._step(closure)
 
-    def _launch(self, group, lr, plan, capturing):
+    step.hooked = True                                  # torch's wrapper (hooks and a profiler range, 8 us) is used where a hook asks for it
+
+    def _launch(self, group, lr, plan, seen, capturing):
         stream = ops._stream()
-        if plan.fresh or plan.captured or capturing:
-            call("erf_adamw_set_grads", plan.table.data_ptr(), plan.grads, len(plan.params), stream)
-            plan.fresh = False
+        table = plan.table.data_ptr()
+        if seen or plan.captured or capturing:
+            self._watch.set_grads(table, plan.which, plan.copies, stream)
             plan.captured = plan.captured or capturing
         b1, b2 = group["betas"]
-        call("erf_adamw_step", plan.table.data_ptr(), plan.chunks.data_ptr(), plan.steps.data_ptr(), plan.chunks.shape[0], lr.data_ptr(),
+        call("erf_adamw_step", table, plan.chunks.data_ptr(), plan.steps.data_ptr(), plan.chunks.shape[0], lr.data_ptr(),
              b1, b2, group["eps"], group["weight_decay"], plan.code, self.state_bits, self.seed, stream)
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
 
 
 def _dense(t):

@@ -51,6 +51,33 @@ def test_cpu_parameters_are_refused_at_the_step_and_no_gradient_is_no_step():
     assert torch.equal(p.detach(), torch.zeros(4))
 
 
+def test_the_watch_reports_what_changed():
+    from erfnet_pytorch_amd.optim import _host
+    ps = [torch.nn.Parameter(torch.zeros(2, 3)) for _ in range(3)]
+    ps[0].grad, ps[2].grad = torch.zeros(2, 3), torch.zeros(2, 3)
+    w = _host.ParamWatch()
+    w.bind([ps[:1], ps[1:]])
+    assert [w.look([ps[:1], ps[1:]]) for _ in range(2)] == [1, 0]
+    old = ps[2].grad
+    ps[2].grad = torch.zeros(2, 3)
+    assert [w.look([ps]) for _ in range(2)] == [1, 0]
+    ps[2].grad = old.t().contiguous().t()
+    assert w.look([ps]) == 1 and w.copied() == [1] and w.look([ps]) == 1
+    ps[2].grad = old
+    assert w.look([ps]) == 1 and w.copied() == [] and w.look([ps]) == 0
+    ps[0].data = torch.ones(2, 3)
+    assert w.look([ps]) == 2 and w.look([ps[:2]]) == 2
+    w.bind([ps])
+    ps[1].grad = torch.zeros(2, 3)
+    assert w.look([ps]) == 2
+    before = ps[0]._version
+    w.bump()
+    assert ps[0]._version == before + 1
+    with pytest.raises(ValueError, match="gradient"):
+        ps[0].grad = torch.sparse_coo_tensor(torch.tensor([[0], [0]]), torch.tensor([1.0]), (2, 3))
+        w.look([ps])
+
+
 def test_parameters_that_share_memory_are_found():
     from erfnet_pytorch_amd.optim import _no_overlap
     t = torch.zeros(10)
@@ -403,6 +430,37 @@ def test_captured_steps_count_and_follow_the_learning_rate(bits, lr_tensor):
         return [p.detach().clone() for p in ps], [float(s["step"]) for s in opt.state_dict()["state"].values()]
     (a, ca), (b, cb) = run(False), run(True)
     assert ca == cb == [6.0, 6.0] and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_hooks_schedulers_and_closures():
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = _adamw([p], lr=0.5, weight_decay=0.0, betas=(0.0, 0.0), eps=0.0)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    seen = []
+    handles = [opt.register_step_pre_hook(lambda o, a, k: seen.append("pre")), opt.register_step_post_hook(lambda o, a, k: seen.append("post"))]
+
+    def closure():
+        p.grad = torch.full_like(p, 3.0)
+        return 7.0
+    assert opt.step(closure) == 7.0 and seen == ["pre", "post"] and torch.equal(p.detach(), torch.full_like(p, 0.5))
+    sched.step()
+    for h in handles:
+        h.remove()
+    opt.step()
+    assert seen == ["pre", "post"] and torch.equal(p.detach(), torch.full_like(p, 0.25))
+
+
+@pytest.mark.gpu
+def test_the_optimizer_keeps_no_gradient_alive():
+    import weakref
+    p = torch.nn.Parameter(torch.ones(1000, device="cuda"))
+    opt = _adamw([p])
+    p.grad = torch.ones_like(p)
+    gone = weakref.ref(p.grad)
+    opt.step()
+    opt.zero_grad(set_to_none=True)
+    assert gone() is None
 
 
 @pytest.mark.gpu

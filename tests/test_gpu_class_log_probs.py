@@ -277,6 +277,14 @@ def test_without_target_and_partial_gradients():
 
 
 @pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits((3, 30), torch.float32, "plain", 17).requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(class_log_probs(z).entropy.sum(), z, create_graph=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(3, 11), (1, 11, 1, 3)])
 def test_gradient_against_differences(shape):
     """(f(z + h) - f(z - h)) / 2h with h = 2^-6: truncated at h^2 / 6 |f'''|, |f'''| <= 40 for log p and H of logits this flat
@@ -307,8 +315,8 @@ def test_rows_of_the_gradient_do_not_touch_what_lies_between_them():
     gen = torch.Generator().manual_seed(19)
     z, t = torch.randn(n, s, generator=gen).cuda(), torch.randint(0, c, (n,), generator=gen).cuda()
     d, one = torch.full((n, s), 7.0, device="cuda"), torch.ones(n, device="cuda")
-    _, ent, stats, _, index = train_ops.class_log_probs_fwd(z[:, :c], t)
-    want = train_ops.class_log_probs_bwd(z[:, :c], t, stats, ent, index, one, None, None)
+    _, ent, stats, _, index = train_ops.class_log_probs_fwd(z[:, :c], t, 0, -100)
+    want = train_ops.class_log_probs_bwd(z[:, :c], t, stats, ent, index, one, None, None, -100)
     _lib.call("erf_class_log_probs_bwd", z.data_ptr(), _lib.F32, n, c, 1, s, 1, t.data_ptr(), -100, stats.data_ptr(), ent.data_ptr(), one.data_ptr(),
               0, 0, 0, 0, d.data_ptr(), s, 1, ops._stream())
     assert torch.equal(d[:, :c], want) and (d[:, c:] == 7.0).all()
@@ -360,7 +368,8 @@ def test_wrong_arguments_are_refused():
     z = torch.zeros(3, 5)
     with pytest.raises(RuntimeError, match="MI355X"):
         class_log_probs(z, torch.zeros(3, dtype=torch.int64))
-    f = train_ops.class_log_probs_fwd
+    def f(z, target, top_k=0):
+        return train_ops.class_log_probs_fwd(z, target, top_k, -100)
     with pytest.raises(TypeError, match="float32 or bfloat16"):
         f(z.half(), None)
     with pytest.raises(TypeError, match="int64"):
@@ -368,8 +377,10 @@ def test_wrong_arguments_are_refused():
     for bad in (torch.zeros(4, dtype=torch.int64), torch.zeros(3, 5, dtype=torch.int64)):
         with pytest.raises(ValueError, match="targets of shape"):
             f(z, bad)
-    with pytest.raises(ValueError, match="device|on meta"):
+    with pytest.raises(ValueError, match="on meta"):
         f(z, torch.zeros(3, dtype=torch.int64, device="meta"))
+    with pytest.raises(RuntimeError, match="MI355X"):
+        f(z, None)
     for k in (-1, 6):
         with pytest.raises(ValueError, match="top_k"):
             f(z, None, k)
@@ -378,6 +389,14 @@ def test_wrong_arguments_are_refused():
     for bad in (torch.zeros(3), torch.zeros(3, 0)):
         with pytest.raises(ValueError, match="shape"):
             f(bad, None)
+    b = train_ops.class_log_probs_bwd
+    t, v, two, index = torch.zeros(3, dtype=torch.int64), torch.zeros(3), torch.zeros(2, 3), torch.zeros(3, 2, dtype=torch.int64)
+    for args in ((z, t, torch.zeros(2, 4), v, index, v, None, None), (z, t, two, torch.zeros(4), index, v, None, None),
+                 (z, None, two, v, index, v, None, None), (z, t, two, v, index, torch.zeros(4), None, None), (z, t, two, v, index, None, torch.zeros(2), None),
+                 (z, t, two, v, index, None, None, torch.zeros(3, 1)), (z, t, two, v, index.int(), None, None, torch.zeros(3, 2)),
+                 (z, t, two.double(), v, index, v, None, None), (z, t, two, v, index, v.to("meta"), None, None)):
+        with pytest.raises(ValueError):
+            b(*args, -100)
 
 
 def test_abi_refuses_bad_arguments_without_a_gpu():
@@ -397,7 +416,11 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
 
 
 def test_layouts_are_recognised():
-    from erfnet_pytorch_amd.train_ops import class_layout
+    from erfnet_pytorch_amd.train_ops import class_layout as whole
+
+    def class_layout(t):
+        z, n, c, length, sn, sc, rows = whole(t)
+        return z, n, c, length, sn, sc
     z = torch.zeros(2, 5, 3, 4)
     assert class_layout(z)[1:6] == (2, 5, 12, 60, 12)
     assert class_layout(z.contiguous(memory_format=torch.channels_last))[1:6] == (24, 5, 1, 5, 1)

@@ -241,6 +241,15 @@ def test_captured_calls_and_another_stream(shape, groups):
 
 
 @pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    from erfnet_pytorch_amd.norm import group_norm_act
+    x, w, b, dy = _inputs((1, 8, 4, 4), torch.float32, 12)
+    y = group_norm_act(x.requires_grad_(), 2, w, b)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, x, dy, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_module_and_empty_maps():
     from erfnet_pytorch_amd.norm import GroupNormAct2d, group_norm_act
     m = GroupNormAct2d(4, 16).cuda()
@@ -288,9 +297,10 @@ def test_wrong_arguments_are_refused():
     with pytest.raises(ValueError, match="on meta"):
         f(x, torch.zeros(4, device="meta"), None, 2, 1e-5, "relu")
     with pytest.raises(ValueError, match="dy"):
-        train_ops.group_norm_act_bwd(x.bfloat16(), x, None, None, torch.zeros(1, 2), torch.zeros(1, 2), 2, "relu")
-    with pytest.raises(ValueError, match="mean and rstd"):
-        train_ops.group_norm_act_bwd(x, x, None, None, torch.zeros(1, 3), torch.zeros(1, 2), 2, "relu")
+        train_ops.group_norm_act_bwd(x.bfloat16(), x, None, None, torch.zeros(2, 1, 2), 2, "relu")
+    for bad in (torch.zeros(2, 1, 3), torch.zeros(2, 1, 2, dtype=torch.float64), torch.zeros(2, 1, 4)[..., ::2]):
+        with pytest.raises(ValueError, match="stats"):
+            train_ops.group_norm_act_bwd(x, x, None, None, bad, 2, "relu")
 
 
 def test_abi_refuses_bad_arguments_without_a_gpu():
