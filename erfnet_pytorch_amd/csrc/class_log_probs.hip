@@ -75,11 +75,14 @@ template <int TEAM> __device__ __forceinline__ u64 team_best(u64 v) {
     if (TEAM == 16) up(dpp_u<ROTATE8>(v));
     return v;
 }
+template <int CTRL> __device__ __forceinline__ float dpp_largest(float v) {           // lanes without a partner keep their own
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xF, 0xF, false)));
+}
 template <int TEAM> __device__ __forceinline__ float team_largest(float v) {
     if (TEAM == 64) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-        return v;
+        v = dpp_largest<0x111>(v); v = dpp_largest<0x112>(v); v = dpp_largest<0x114>(v); v = dpp_largest<0x118>(v);
+        v = dpp_largest<0x142>(v); v = dpp_largest<0x143>(v);
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
     }
     v = fmaxf(v, dpp_f<SWAP1>(v)); v = fmaxf(v, dpp_f<SWAP2>(v)); v = fmaxf(v, dpp_f<MIRROR8>(v));
     if (TEAM == 16) v = fmaxf(v, dpp_f<ROTATE8>(v));
@@ -98,17 +101,22 @@ struct LpArgs {
     u64* parts;                        // [N][segments][2 + k]: (m, s), (t, -), the segment's best ranks
 };
 
-// log p of the target, entropy and the saved pair of position i from its statistics
+// The target's logit of row i, fetched while the row is on its way; NaN for a target outside [0, C), as in the weighted cross entropy
+struct LpTarget { float z; bool ignored; };
 template <typename T>
-__device__ __forceinline__ void lp_finish(const LpArgs& a, const T* row, long long i, const Stat& st, float logs) {
-    const float base = base_of(st.m);
+__device__ __forceinline__ LpTarget lp_target(const LpArgs& a, const T* row, long long i) {
+    LpTarget q{__builtin_nanf(""), false};
     if (a.log_prob) {
         const long long t = a.target[i];
-        float v = __builtin_nanf("");                                  // a target outside [0, C): as in the weighted cross entropy
-        if (t == a.ignore) v = 0.f;
-        else if (t >= 0 && t < a.C) v = (Elem<T>::ld(row + t * a.sc) - base) - logs;
-        a.log_prob[i] = v;
+        q.ignored = t == a.ignore;
+        if (t >= 0 && t < a.C) q.z = Elem<T>::ld(row + t);
     }
+    return q;
+}
+// log p of the target, entropy and the saved pair of row i from its statistics
+__device__ __forceinline__ void lp_finish(const LpArgs& a, const LpTarget& q, long long i, const Stat& st, float logs) {
+    const float base = base_of(st.m);
+    if (a.log_prob) a.log_prob[i] = q.ignored ? 0.f : (q.z - base) - logs;
     a.entropy[i] = logs - st.t * LN2 / st.s;
     if (a.stats) {
         a.stats[i] = base;
@@ -342,6 +350,20 @@ __device__ __forceinline__ void load_chunk(const T* row, int off, int C, int q, 
     }
 }
 
+// How many of n ranks in LDS are above r; 8 reads are in flight together
+__device__ __forceinline__ int count_above(const u64* ranks, int n, u64 r) {
+    int above = 0, o = 0;
+    for (; o + 8 <= n; o += 8) {
+        u64 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ranks[o + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) above += v[e] > r;
+    }
+    for (; o < n; ++o) above += ranks[o] > r;
+    return above;
+}
+
 // Best rank below `last` among the classes of chunks [q0, q1), by the whole team
 template <typename T, int TEAM>
 __device__ __forceinline__ u64 team_round(TeamShared<TEAM>& sh, const T* row, int off, int C, int q0, int q1, int tid, u64 last) {
@@ -400,6 +422,8 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     const int chunks = (a.C + off + E - 1) / E, per = (chunks + a.segments - 1) / a.segments;
     const int seg = blockIdx.y, q0 = min(seg * per, chunks), q1 = min(q0 + per, chunks);
 
+    LpTarget target{};
+    if (tid == 0 && a.segments == 1) target = lp_target(a, row, i);
     Stat st{-INFINITY, 0.f, 0.f};
     float f[UNROLL][E];
     for (int q = q0 + tid; q < (TEAM < 256 ? q0 + TEAM : q1); q += TEAM * UNROLL) {
@@ -446,7 +470,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     u64* part = whole ? nullptr : a.parts + (i * a.segments + seg) * (2 + a.k);
     const float base = base_of(st.m), logs = logf(st.s);
     if (tid == 0) {
-        if (whole) lp_finish(a, row, i, st, logs);
+        if (whole) lp_finish(a, target, i, st, logs);
         else {
             part[0] = ((u64)__float_as_uint(st.s) << 32) | __float_as_uint(st.m);
             part[1] = __float_as_uint(st.t);
@@ -510,8 +534,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
             if (!slow) {
                 for (int c = tid; c < n; c += TEAM) {
                     const u64 r = sh.cand[c];
-                    int before = 0;
-                    for (int o = 0; o < n && before < a.k; ++o) before += sh.cand[o] > r;
+                    const int before = count_above(sh.cand, n, r);
                     if (before < a.k) put(before, r);
                 }
                 for (int k = n + tid; k < a.k; k += TEAM) put(k, 0);   // a segment of fewer classes
@@ -527,14 +550,21 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     }
 }
 
-// The segments of a row joined by one wave
+// The segments of a row joined by one workgroup: their alternatives meet in LDS and find their places by counting, or, where they
+// are many, by rounds
+#define JOIN 1024
 template <typename T>
-__global__ __launch_bounds__(64) void lp_join_kernel(const LpArgs a) {
+__global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs a) {
+    __shared__ float m4[4], s4[4], t4[4];
+    __shared__ u64 cand[JOIN];
     const long long i = blockIdx.x;
-    const int step = 2 + a.k;
+    const int step = 2 + a.k, tid = threadIdx.x, n = a.segments * a.k;
     const u64* part = a.parts + i * a.segments * step;
+    LpTarget target{};
+    if (tid == 0) target = lp_target(a, (const T*)a.z + i * a.sn, i);
+    for (int c = tid; c < n && c < JOIN; c += 256) cand[c] = part[(long long)(c / a.k) * step + 2 + c % a.k];
     Stat st{-INFINITY, 0.f, 0.f};
-    for (int g = threadIdx.x; g < a.segments; g += 64) {
+    for (int g = tid; g < a.segments; g += 256) {
         const u64 ms = part[(long long)g * step];
         Stat p{__uint_as_float((unsigned)ms), __uint_as_float((unsigned)(ms >> 32)), __uint_as_float((unsigned)part[(long long)g * step + 1])};
         const float m = fmaxf(p.m, st.m);
@@ -546,21 +576,38 @@ __global__ __launch_bounds__(64) void lp_join_kernel(const LpArgs a) {
     stat_move(st, team_largest<64>(st.m));
     st.s = team_sum<64>(st.s);
     st.t = team_sum<64>(st.t);
-    const float logs = logf(st.s);
-    if (threadIdx.x == 0) lp_finish(a, (const T*)a.z + i * a.sn, i, st, logs);
+    if ((tid & 63) == 0) { m4[tid >> 6] = st.m; s4[tid >> 6] = st.s; t4[tid >> 6] = st.t; }
+    __syncthreads();
+    st = Stat{fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), 0.f, 0.f};
+    for (int w = 0; w < 4; ++w) {
+        Stat p{m4[w], s4[w], t4[w]};
+        stat_move(p, st.m);
+        st.s += p.s;
+        st.t += p.t;
+    }
+    const float logs = logf(st.s), base = base_of(st.m);
+    if (tid == 0) lp_finish(a, target, i, st, logs);
+    auto put = [&](int k, u64 r) {
+        a.top[i * a.k + k] = (rank_value(r) - base) - logs;
+        a.top_index[i * a.k + k] = rank_index(r);
+    };
+    if (n <= JOIN) {
+        for (int c = tid; c < n; c += 256) {
+            const u64 r = cand[c];
+            const int before = count_above(cand, n, r);
+            if (r && before < a.k) put(before, r);                     // 0: a segment of fewer classes
+        }
+        return;
+    }
     u64 last = ~0ull;
-    const int n = a.segments * a.k;
-    for (int k = 0; k < a.k; ++k) {
+    for (int k = 0; k < a.k && tid < 64; ++k) {
         u64 r = 0;
-        for (int c = threadIdx.x; c < n; c += 64) {
+        for (int c = tid; c < n; c += 64) {
             const u64 o = part[(long long)(c / a.k) * step + 2 + c % a.k];
             r = o < last && o > r ? o : r;
         }
         last = team_best<64>(r);
-        if (threadIdx.x == 0) {
-            a.top[i * a.k + k] = (rank_value(last) - base_of(st.m)) - logs;
-            a.top_index[i * a.k + k] = rank_index(last);
-        }
+        if (tid == 0) put(k, last);
     }
 }
 
@@ -790,7 +837,7 @@ static void lp_rows_launch(const LpArgs& a, int dtype, hipStream_t s) {
     else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, TOP>), grid, block, 0, s, a);
     else if (team == 64) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), grid, block, 0, s, a);
-    if (a.segments > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)a.N), dim3(64), 0, s, a);
+    if (a.segments > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)a.N), dim3(256), 0, s, a);
 }
 
 template <typename T>

@@ -36,7 +36,9 @@ struct GnArgs {
     float* sums;                       // [N][C][2]: A, B;  then [N][G][2]: s1 / M, s2 / M
     long long HW;
     int N, C, G, P;
-    int chunks, lanes;                 // a pixel's chunks of VEC channels in one workgroup, and the pixels side by side in it
+    int chunks, lanes;                 // a pixel's chunks of VEC channels in one workgroup (team), and the pixels side by side in it
+    int team;                          // a group per team: its threads
+    int rows;                          // parameter gradients: rows of `sums` (N, or runs of images already summed up)
     float eps;
 };
 
@@ -356,29 +358,64 @@ __global__ __launch_bounds__(1024) void gn_bwd_finalize_kernel(const GnArgs a) {
     }
 }
 
-// dx; and, by the workgroups behind those of the last run, dbeta = sum_n A and dgamma = sum_n B: 64 channels each, four image lanes
+// dbeta = sum_n A and dgamma = sum_n B: 64 channels a workgroup, four image lanes with 4 loads in flight each
+__device__ __forceinline__ void gn_row_sums(const float* sums, long long first, long long last, int C, int c, double (*sh)[GN_THREADS], double& p, double& r) {
+    p = r = 0;
+    if (c < C) {
+        long long n = first + (threadIdx.x >> 6);
+        for (; n + 12 < last; n += 16) {
+            float2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = *(const float2*)(sums + 2 * ((n + 4 * u) * C + c));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { p += v[u].x; r += v[u].y; }
+        }
+        for (; n < last; n += 4) {
+            const float2 v = *(const float2*)(sums + 2 * (n * C + c));
+            p += v.x;
+            r += v.y;
+        }
+    }
+    sh[0][threadIdx.x] = p;
+    sh[1][threadIdx.x] = r;
+    __syncthreads();
+    if (threadIdx.x < 64)
+        for (int w = 1; w < 4; ++w) { p += sh[0][threadIdx.x + 64 * w]; r += sh[1][threadIdx.x + 64 * w]; }
+}
+__device__ __forceinline__ void gn_param_grads(const GnArgs& a, const float* sums, int block, double (*sh)[GN_THREADS]) {
+    const int c = block * 64 + (threadIdx.x & 63);
+    double p, r;
+    gn_row_sums(sums, 0, a.rows, a.C, c, sh, p, r);
+    if (threadIdx.x < 64 && c < a.C) {
+        if (a.dbeta) a.dbeta[c] = (float)p;
+        if (a.dgamma) a.dgamma[c] = (float)r;
+    }
+}
+__global__ __launch_bounds__(GN_THREADS) void gn_param_grads_kernel(const GnArgs a, const float* sums) {
+    __shared__ double sh[2][GN_THREADS];
+    gn_param_grads(a, sums, blockIdx.x, sh);
+}
+// ... of many images: runs of them first, to rows of `out`
+__global__ __launch_bounds__(GN_THREADS) void gn_image_runs_kernel(const GnArgs a, float* out) {
+    __shared__ double sh[2][GN_THREADS];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
+    const long long per = (a.N + (long long)gridDim.y - 1) / gridDim.y, first = blockIdx.y * per, last = first + per < a.N ? first + per : a.N;
+    double p, r;
+    gn_row_sums(a.sums, first, last, a.C, c, sh, p, r);
+    if (threadIdx.x < 64 && c < a.C) {
+        out[2 * ((long long)blockIdx.y * a.C + c)] = (float)p;
+        out[2 * ((long long)blockIdx.y * a.C + c) + 1] = (float)r;
+    }
+}
+
+// dx; and, by the workgroups behind those of the last run, the parameter gradients
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnArgs a) {
     constexpr int U = 4;
     if (blockIdx.x >= (unsigned)(a.N * a.P)) {
         __shared__ double sh[2][GN_THREADS];
         if (blockIdx.y) return;
-        const int c = (int)(blockIdx.x - (unsigned)(a.N * a.P)) * 64 + (threadIdx.x & 63);
-        double p = 0, r = 0;
-        if (c < a.C)
-            for (int n = threadIdx.x >> 6; n < a.N; n += 4) {
-                const float2 v = *(const float2*)(a.sums + 2 * ((long long)n * a.C + c));
-                p += v.x;
-                r += v.y;
-            }
-        sh[0][threadIdx.x] = p;
-        sh[1][threadIdx.x] = r;
-        __syncthreads();
-        if (threadIdx.x < 64 && c < a.C) {
-            for (int w = 1; w < 4; ++w) { p += sh[0][threadIdx.x + 64 * w]; r += sh[1][threadIdx.x + 64 * w]; }
-            if (a.dbeta) a.dbeta[c] = (float)p;
-            if (a.dgamma) a.dgamma[c] = (float)r;
-        }
+        gn_param_grads(a, a.sums, (int)(blockIdx.x - (unsigned)(a.N * a.P)), sh);
         return;
     }
     const GnPlace q = gn_place<VEC>(a);
@@ -418,6 +455,170 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnArgs a
     }
 }
 
+// ------------------------------------------------------------------------------------------------ a whole group in registers
+// Where the values of one (image, group) fit the registers of a team of 8 or 64 lanes or of a workgroup, KEEP of them per thread, x
+// (and dy) are read once and one launch does it all.  Threads are (pixel lane, chunk of VEC channels of the group).  Neighbouring
+// groups, which share cache lines, go to one XCD: workgroups are dealt to the 8 XCDs in turn.
+#define GN_KEEP 32
+struct GnGroup { int n, g, c, tid, lane; long long at; bool on; };          // c: first channel; at: its place in the image's first pixel of the lane
+template <int VEC> __device__ __forceinline__ GnGroup gn_group(const GnArgs& a) {
+    GnGroup q;
+    const unsigned teams = blockDim.x / a.team, id = ((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) * teams + threadIdx.x / a.team;
+    q.tid = threadIdx.x % a.team;
+    q.n = id / (unsigned)a.G;
+    q.g = id - q.n * a.G;
+    q.lane = q.tid / a.chunks;
+    q.c = q.g * (a.C / a.G) + (q.tid - q.lane * a.chunks) * VEC;
+    q.on = q.n < a.N && q.lane < a.lanes;
+    q.at = ((long long)q.n * a.HW + q.lane) * a.C + q.c;
+    return q;
+}
+
+// Sum over the team; every thread gets it
+__device__ __forceinline__ float gn_total(float v, float* sh, int team) {
+    v += __shfl_xor(v, 1, 64);
+    v += __shfl_xor(v, 2, 64);
+    v += __shfl_xor(v, 4, 64);
+    if (team == 8) return v;
+    v += __shfl_xor(v, 8, 64);
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    if (team == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) s += sh[w];
+    return s;
+}
+__device__ __forceinline__ void gn_sync(int team) {
+    if (team > 64) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(1024) void gn_group_fwd_kernel(const GnArgs a) {
+    constexpr int R = GN_KEEP / VEC;
+    __shared__ float sh[16];
+    const GnGroup q = gn_group<VEC>(a);
+    const T* x = (const T*)a.x + q.at;
+    float f[R][VEC];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (q.on && q.lane + r * a.lanes < a.HW) vec_load<T, VEC>(x + (long long)r * a.lanes * a.C, f[r]);
+        else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[r][e] = 0.f;
+        }
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s += f[r][e];
+    const float m = (float)(a.HW * (a.C / a.G)), mean = gn_total(s, sh, a.team) / m;
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (q.on && q.lane + r * a.lanes < a.HW) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s = fmaf(f[r][e] - mean, f[r][e] - mean, s);
+        }
+    const float rstd = 1.f / sqrtf(gn_total(s, sh, a.team) / m + a.eps);
+    if (q.on && q.tid == 0) { a.mean[(long long)q.n * a.G + q.g] = mean; a.rstd[(long long)q.n * a.G + q.g] = rstd; }
+    if (!q.on) return;
+    float scale[VEC], beta[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        scale[e] = rstd * (a.gamma ? a.gamma[q.c + e] : 1.f);
+        beta[e] = a.beta ? a.beta[q.c + e] : 0.f;
+    }
+    T* y = (T*)a.y + q.at;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (q.lane + r * a.lanes < a.HW) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[r][e] = gn_act<ACT>(gn_u(f[r][e], mean, scale[e], beta[e]));
+            vec_store<T, VEC>(y + (long long)r * a.lanes * a.C, f[r]);
+        }
+}
+
+// dx, and A and B of the group's channels; gn_param_grads_kernel sums those over the images
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(1024) void gn_group_bwd_kernel(const GnArgs a) {
+    constexpr int R = GN_KEEP / VEC;
+    __shared__ float sh[16];
+    extern __shared__ float part[];                                    // [2][VEC][threads]
+    const GnGroup q = gn_group<VEC>(a);
+    const T *x = (const T*)a.x + q.at, *dy = (const T*)a.dy + q.at;
+    const float mean = q.on ? a.mean[(long long)q.n * a.G + q.g] : 0.f, rstd = q.on ? a.rstd[(long long)q.n * a.G + q.g] : 0.f;
+    float f[R][VEC], d[R][VEC], gamma[VEC], beta[VEC], p[VEC], s[VEC];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (q.on && q.lane + r * a.lanes < a.HW) {
+            vec_load<T, VEC>(x + (long long)r * a.lanes * a.C, f[r]);
+            vec_load<T, VEC>(dy + (long long)r * a.lanes * a.C, d[r]);
+        }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        gamma[e] = q.on && a.gamma ? a.gamma[q.c + e] : 1.f;
+        beta[e] = q.on && a.beta ? a.beta[q.c + e] : 0.f;
+        p[e] = s[e] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (q.on && q.lane + r * a.lanes < a.HW) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                d[r][e] *= gn_slope<ACT>(gn_u(f[r][e], mean, rstd * gamma[e], beta[e]));
+                f[r][e] = (f[r][e] - mean) * rstd;
+                p[e] += d[r][e];
+                s[e] = fmaf(d[r][e], f[r][e], s[e]);
+            }
+        }
+    for (int have = a.lanes; have > 1;) {
+        const int keep = (have + 1) / 2;
+        gn_sync(a.team);
+        if (q.on && q.lane >= keep && q.lane < have) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { part[e * blockDim.x + threadIdx.x] = p[e]; part[(VEC + e) * blockDim.x + threadIdx.x] = s[e]; }
+        }
+        gn_sync(a.team);
+        if (q.on && q.lane + keep < have) {
+            const int o = threadIdx.x + keep * a.chunks;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { p[e] += part[e * blockDim.x + o]; s[e] += part[(VEC + e) * blockDim.x + o]; }
+        }
+        have = keep;
+    }
+    float g1 = 0.f, g2 = 0.f;
+    if (q.on && q.lane == 0) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float* out = a.sums + 2 * ((long long)q.n * a.C + q.c + e);
+            out[0] = p[e];
+            out[1] = s[e];
+            g1 = fmaf(gamma[e], p[e], g1);
+            g2 = fmaf(gamma[e], s[e], g2);
+        }
+    }
+    const float m = (float)(a.HW * (a.C / a.G));
+    g1 = gn_total(g1, sh, a.team) / m;
+    g2 = gn_total(g2, sh, a.team) / m;
+    if (!q.on) return;
+    T* dx = (T*)a.dx + q.at;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (q.lane + r * a.lanes < a.HW) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) d[r][e] = rstd * (gamma[e] * d[r][e] - fmaf(f[r][e], g2, g1));
+            vec_store<T, VEC>(dx + (long long)r * a.lanes * a.C, d[r]);
+        }
+}
+
 static inline bool gn_shape_ok(int dtype, int N, long long HW, int C, int groups, int act) {
     return (dtype == ERF_F32 || dtype == ERF_BF16) && N > 0 && N <= (1 << 24) && HW > 0 && C > 0 && groups > 0 && C % groups == 0 && act >= 0 &&
            act <= 2 && (long long)N * groups <= 0x7FFFFFFFll && C <= (1 << 20) && HW <= (1ll << 40) / C;
@@ -430,74 +631,119 @@ static inline int gn_vec(int dtype, int C, unsigned long long addresses) {
     while (v > 1 && (C % v || addresses % (v * size))) v /= 2;
     return v;
 }
-// Runs of pixels per image: about 1024 workgroups in all, each thread with a few sets of loads, at most 512 runs to be joined
-static inline int gn_runs(int N, long long HW, int lanes, int slabs) {
-    const long long want = (1024 + (long long)N * slabs - 1) / ((long long)N * slabs), most = (HW + (long long)lanes * GN_UNROLL - 1) / ((long long)lanes * GN_UNROLL);
-    const long long p = want < most ? want : most;
-    return (int)(p < 1 ? 1 : p > 512 ? 512 : p);
-}
+// Runs of pixels per image: about 1024 workgroups in all (512 to 4096 are within 5 % of each other on large maps), each thread with `each`
+// pixels at least, at most `most` runs
 #define GN_MAX_RUNS 512
-
-template <int VEC> static inline void gn_plan(GnArgs& a, dim3& grid) {
+template <int VEC> static inline dim3 gn_plan(GnArgs& a, int each, int most) {
     const int chunks = a.C / VEC;
     a.chunks = chunks < GN_THREADS ? chunks : GN_THREADS;
     a.lanes = GN_THREADS / a.chunks;
     const int slabs = (chunks + a.chunks - 1) / a.chunks;
-    a.P = gn_runs(a.N, a.HW, a.lanes, slabs);
-    grid = dim3((unsigned)a.P * (unsigned)a.N, (unsigned)slabs);
+    const long long images = (long long)a.N * slabs, want = (1024 + images - 1) / images, full = (a.HW + (long long)a.lanes * each - 1) / ((long long)a.lanes * each);
+    const long long p = want < full ? want : full;
+    a.P = (int)(p < 1 ? 1 : p > most ? most : p);
+    return dim3((unsigned)a.P * (unsigned)a.N, (unsigned)slabs);
+}
+
+// The plan of a group per team: channels per access (the most that divide a group) and the smallest team that has the values in
+// registers and either fills the chip with threads or leaves each thread one access.  Groups of more values than 4096 (backward 2048)
+// for each channel of an access are faster by runs of pixels, in three launches.  Group against runs, forward / backward, in us:
+// 64 x 64 x 1024 in 8 groups bf16 9 / 18 against 17 / 24; 64 x 128 x 4096 in 32 groups 73 / 155 against 57 / 97;
+// 3 x 30 x 5673 in 6 groups 15 / 23 against 11 / 13; 512 x 128 x 64 in 16 groups 9 / 24 against 65 / 96.
+static bool gn_group_plan(GnArgs& a, int dtype, unsigned long long addresses, int& vec, bool backward) {
+    const int cpg = a.C / a.G;
+    vec = gn_vec(dtype, cpg, addresses);
+    a.chunks = cpg / vec;
+    const long long groups = (long long)a.N * a.G;
+    if (a.HW * cpg > (backward ? 2048 : 4096) * vec) return false;
+    for (a.team = 8; a.team <= 1024; a.team = a.team == 8 ? 64 : 4 * a.team) {
+        a.lanes = a.team / a.chunks;
+        if (a.lanes && a.HW <= (long long)a.lanes * GN_KEEP / vec && (a.team == 1024 || groups * a.team >= (1 << 17) || a.HW <= a.lanes)) return true;
+    }
+    return false;
+}
+static inline dim3 gn_group_block(const GnArgs& a) { return dim3(a.team < 256 ? 256 : (unsigned)a.team); }
+static inline dim3 gn_group_grid(const GnArgs& a) {
+    const long long teams = gn_group_block(a).x / a.team, blocks = ((long long)a.N * a.G + teams - 1) / teams;
+    return dim3((unsigned)((blocks + 7) / 8 * 8));
+}
+// Images summed up before the parameter gradients are: runs of at least 64
+static inline int gn_image_runs(int N) { return N <= 256 ? 1 : N / 64 < 64 ? N / 64 : 64; }
+
+template <typename T, int VEC, int ACT>
+static void gn_group_fwd_launch(GnArgs a, hipStream_t s) {
+    hipLaunchKernelGGL((gn_group_fwd_kernel<T, VEC, ACT>), gn_group_grid(a), gn_group_block(a), 0, s, a);
+}
+static void gn_param_grads_launch(GnArgs a, hipStream_t s) {
+    if (!a.dgamma && !a.dbeta) return;
+    const unsigned blocks = (unsigned)((a.C + 63) / 64);
+    const float* sums = a.sums;
+    a.rows = gn_image_runs(a.N);
+    if (a.rows > 1) {
+        hipLaunchKernelGGL(gn_image_runs_kernel, dim3(blocks, (unsigned)a.rows), dim3(GN_THREADS), 0, s, a, a.parts);
+        sums = a.parts;
+    } else {
+        a.rows = a.N;
+    }
+    hipLaunchKernelGGL(gn_param_grads_kernel, dim3(blocks), dim3(GN_THREADS), 0, s, a, sums);
+}
+template <typename T, int VEC, int ACT>
+static void gn_group_bwd_launch(GnArgs a, hipStream_t s) {
+    hipLaunchKernelGGL((gn_group_bwd_kernel<T, VEC, ACT>), gn_group_grid(a), gn_group_block(a), 2 * VEC * gn_group_block(a).x * sizeof(float), s, a);
+    gn_param_grads_launch(a, s);
 }
 
 template <typename T, int VEC, int ACT>
 static void gn_fwd_launch(GnArgs a, hipStream_t s) {
-    dim3 grid;
-    gn_plan<VEC>(a, grid);
-    hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), grid, dim3(GN_THREADS), 0, s, a);
+    hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS), dim3(GN_THREADS), 0, s, a);
     hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
-    hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+    hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT>), gn_plan<VEC>(a, 4, 1 << 20), dim3(GN_THREADS), 0, s, a);
 }
 
 template <typename T, int VEC, int ACT>
 static void gn_bwd_launch(GnArgs a, hipStream_t s) {
-    dim3 grid;
-    gn_plan<VEC>(a, grid);
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, VEC, ACT>), gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS), dim3(GN_THREADS), 0, s, a);
     hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
-    grid.x += (unsigned)((a.C + 63) / 64);
+    dim3 grid = gn_plan<VEC>(a, 4, 1 << 20);
+    const bool few = gn_image_runs(a.N) == 1 && (a.dgamma || a.dbeta);
+    a.rows = a.N;
+    if (few) grid.x += (unsigned)((a.C + 63) / 64);
     hipLaunchKernelGGL((gn_bwd_apply_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+    if (!few) gn_param_grads_launch(a, s);
 }
 
-#define GN_ACT(FN, T, VEC)                                            \
-    do {                                                              \
+#define GN_ACT(FN, T, VEC)                                                    \
+    do {                                                                      \
         if (act == ERF_ACT_RELU) FN<T, VEC, ERF_ACT_RELU>(a, s);      \
         else if (act == ERF_ACT_SILU) FN<T, VEC, ERF_ACT_SILU>(a, s); \
         else FN<T, VEC, ERF_ACT_NONE>(a, s);                          \
     } while (0)
-#define GN_PICK(FN, VECTOR)                                                           \
-    do {                                                                              \
-        hipStream_t s = (hipStream_t)stream;                                          \
-        const int v = VECTOR;                                                         \
-        if (dtype == ERF_F32) {                                                       \
-            if (v == 4) GN_ACT(FN, float, 4);                                         \
-            else if (v == 2) GN_ACT(FN, float, 2);                                    \
-            else GN_ACT(FN, float, 1);                                                \
-        } else {                                                                      \
-            if (v == 8) GN_ACT(FN, bf16raw, 8);                                       \
-            else if (v == 4) GN_ACT(FN, bf16raw, 4);                                  \
-            else if (v == 2) GN_ACT(FN, bf16raw, 2);                                  \
-            else GN_ACT(FN, bf16raw, 1);                                              \
-        }                                                                             \
+#define GN_PICK(FN)                                    \
+    do {                                               \
+        hipStream_t s = (hipStream_t)stream;           \
+        if (dtype == ERF_F32) {                        \
+            if (vec == 4) GN_ACT(FN, float, 4);        \
+            else if (vec == 2) GN_ACT(FN, float, 2);   \
+            else GN_ACT(FN, float, 1);                 \
+        } else {                                       \
+            if (vec == 8) GN_ACT(FN, bf16raw, 8);      \
+            else if (vec == 4) GN_ACT(FN, bf16raw, 4); \
+            else if (vec == 2) GN_ACT(FN, bf16raw, 2); \
+            else GN_ACT(FN, bf16raw, 1);               \
+        }                                              \
     } while (0)
 
 extern "C" {
 
 size_t erf_group_norm_workspace_bytes(int dtype, int N, long long HW, int C, int groups) {
     if (!gn_shape_ok(dtype, N, HW, C, groups, 0)) return 0;
-    // the runs of one of the plans (which one depends on the addresses), and the per-channel and per-group sums
+    // the runs of pixels of any plan (which one depends on the addresses) or the runs of images, and the per-channel and per-group sums
     long long runs = (HW + GN_UNROLL - 1) / GN_UNROLL;
     const long long want = (1024 + N - 1) / N;
     runs = runs < want ? runs : want;
-    runs = runs < GN_MAX_RUNS ? runs : GN_MAX_RUNS;
-    return ((size_t)N * (size_t)runs * C + (size_t)N * C + (size_t)N * groups) * 2 * sizeof(float);
+    runs = (runs < GN_MAX_RUNS ? runs : GN_MAX_RUNS) * N;
+    runs = runs < gn_image_runs(N) ? gn_image_runs(N) : runs;
+    return ((size_t)runs * C + (size_t)N * C + (size_t)N * groups) * 2 * sizeof(float);
 }
 
 int erf_group_norm_fwd(const void* x, void* y, int dtype, int N, long long HW, int C, int groups, const float* gamma, const float* beta,
@@ -507,7 +753,14 @@ int erf_group_norm_fwd(const void* x, void* y, int dtype, int N, long long HW, i
     a.x = x; a.y = y; a.gamma = gamma; a.beta = beta; a.mean = mean; a.rstd = rstd; a.HW = HW; a.N = N; a.C = C; a.G = groups; a.eps = eps;
     a.sums = (float*)workspace;
     a.parts = a.sums + 2 * ((size_t)N * C + (size_t)N * groups);
-    GN_PICK(gn_fwd_launch, gn_vec(dtype, C, (unsigned long long)x | (unsigned long long)y));
+    const unsigned long long addresses = (unsigned long long)x | (unsigned long long)y;
+    int vec;
+    if (gn_group_plan(a, dtype, addresses, vec, false)) {
+        GN_PICK(gn_group_fwd_launch);
+    } else {
+        vec = gn_vec(dtype, C, addresses);
+        GN_PICK(gn_fwd_launch);
+    }
     return erf_check_launch();
 }
 
@@ -520,7 +773,14 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
     a.dbeta = dbeta; a.HW = HW; a.N = N; a.C = C; a.G = groups;
     a.sums = (float*)workspace;
     a.parts = a.sums + 2 * ((size_t)N * C + (size_t)N * groups);
-    GN_PICK(gn_bwd_launch, gn_vec(dtype, C, (unsigned long long)x | (unsigned long long)dy | (unsigned long long)dx));
+    const unsigned long long addresses = (unsigned long long)x | (unsigned long long)dy | (unsigned long long)dx;
+    int vec;
+    if (gn_group_plan(a, dtype, addresses, vec, true)) {
+        GN_PICK(gn_group_bwd_launch);
+    } else {
+        vec = gn_vec(dtype, C, addresses);
+        GN_PICK(gn_bwd_launch);
+    }
     return erf_check_launch();
 }
 
