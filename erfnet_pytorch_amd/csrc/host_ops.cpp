@@ -417,6 +417,56 @@ struct ParamWatch {
     }
 };
 
+// What a device table points at stays allocated as long as the table
+struct TableHold { std::vector<c10::Storage> storages; };
+
+// The table's records (CPU int64 [n, 8], grad fields 0) of these parameters with these states: (exp_avg, exp_avg_sq), or (exp_avg,
+// exp_avg_sq_root, exp_avg_scale, exp_avg_sq_root_scale)
+static std::tuple<Tensor, std::shared_ptr<TableHold>> adamw_table(const std::vector<Tensor>& params, const std::vector<std::vector<Tensor>>& states,
+                                                                  const std::vector<int64_t>& bases) {
+    const int64_t block = erf_adamw_scale_block();
+    static const char* const names32[] = {"exp_avg", "exp_avg_sq"};
+    static const char* const names8[] = {"exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale"};
+    auto hold = std::make_shared<TableHold>();
+    Tensor rows = at::zeros({(int64_t)params.size(), 8}, at::kLong);
+    int64_t* r = rows.data_ptr<int64_t>();
+    for (size_t i = 0; i < params.size(); ++i, r += 8) {
+        const Tensor& p = params[i];
+        const std::vector<Tensor>& st = states.at(i);
+        const bool eight = st.size() == 4;
+        const at::ScalarType type = eight ? at::kFloat8_e4m3fn : at::kFloat;
+        for (size_t k = 0; k < st.size(); ++k) {
+            const Tensor& t = st[k];
+            const char* name = eight ? names8[k] : names32[k];
+            if (k < 2) {
+                TORCH_CHECK_VALUE(t.defined() && t.scalar_type() == type && t.device() == p.device() && t.sizes() == p.sizes() &&
+                                      (t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous())),
+                                  "AdamW: state '", name, "' of a parameter of shape ", p.sizes(), ": expected a ", type, " tensor laid out as the parameter");
+            } else {
+                TORCH_CHECK_VALUE(t.defined() && t.scalar_type() == at::kFloat && t.device() == p.device() && t.is_contiguous() &&
+                                      t.numel() == (p.numel() + block - 1) / block,
+                                  "AdamW: state '", name, "' of a parameter of shape ", p.sizes(), ": expected one fp32 value per ", block, " elements");
+            }
+            hold->storages.push_back(t.storage());
+        }
+        hold->storages.push_back(p.storage());
+        const int64_t row[8] = {(int64_t)p.data_ptr(), 0, (int64_t)st[0].data_ptr(), (int64_t)st[1].data_ptr(), eight ? (int64_t)st[2].data_ptr() : 0,
+                                eight ? (int64_t)st[3].data_ptr() : 0, p.numel(), bases.at(i)};
+        std::copy(row, row + 8, r);
+    }
+    return {rows, hold};
+}
+
+// Two parameters that share memory would be updated by two workgroups at once
+static void adamw_no_overlap(const std::vector<Tensor>& params) {
+    std::vector<std::tuple<int, const char*, const char*>> spans;
+    for (const Tensor& p : params) spans.emplace_back(p.device().index(), (const char*)p.data_ptr(), (const char*)p.data_ptr() + p.numel() * p.element_size());
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        TORCH_CHECK_VALUE(std::get<0>(spans[i]) != std::get<0>(spans[i - 1]) || std::get<1>(spans[i]) >= std::get<2>(spans[i - 1]),
+                          "AdamW: two parameters share memory; give the optimizer one of them");
+}
+
 static std::tuple<Tensor, Tensor> group_norm_act_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps,
                                                      const std::string& activation) {
     return group_norm_fwd(x, weight, bias, groups, eps, activation_code(activation));
@@ -444,6 +494,9 @@ PYBIND11_MODULE(_host, m) {
     m.def("class_log_probs_fwd", wrap_pybind_function(class_log_probs_with_stats));
     m.def("class_log_probs_bwd", wrap_pybind_function(class_log_probs_bwd));
     m.def("class_layout", wrap_pybind_function(layout_of));
+    m.def("adamw_table", wrap_pybind_function(adamw_table));
+    m.def("adamw_no_overlap", wrap_pybind_function(adamw_no_overlap));
+    py::class_<TableHold, std::shared_ptr<TableHold>>(m, "TableHold");
     py::class_<ParamWatch>(m, "ParamWatch")
         .def(py::init<>())
         .def("look", wrap_pybind_function(&ParamWatch::look))

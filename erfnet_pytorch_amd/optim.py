@@ -106,18 +106,6 @@ class AdamW(torch.optim.Optimizer):
                 for k in ("exp_avg", "exp_avg_sq_root"):
                     st[k] = torch.zeros_like(p, dtype=torch.uint8).view(torch.float8_e4m3fn)
                     st[k + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root")
-        want = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
-        for k in names:
-            t = st.get(k)
-            if t is None or t.dtype != want or t.device != p.device or t.numel() != p.numel() or not (
-                    t.stride() == p.stride() or (t.is_contiguous() and p.is_contiguous())):
-                raise ValueError(f"state '{k}' of a parameter of shape {tuple(p.shape)}: expected a {want} tensor laid out as the parameter")
-            if self.state_bits == 8:
-                s = st.get(k + "_scale")
-                if s is None or s.dtype != torch.float32 or s.device != p.device or not s.is_contiguous() or \
-                        s.numel() != -(-p.numel() // size_query("erf_adamw_scale_block")):
-                    raise ValueError(f"state '{k}_scale' of a parameter of shape {tuple(p.shape)}: expected one fp32 value per 256 elements")
         return st
 
     def _write_back_steps(self):
@@ -179,33 +167,32 @@ class AdamW(torch.optim.Optimizer):
             for p in group:
                 if p.grad is not None and p.numel():
                     key = (p.device, F32 if p.dtype == torch.float32 else BF16)
-                    plan = mine.setdefault(key, _Plan(*key))
+                    plan = mine.get(key)
+                    if plan is None:
+                        plan = mine[key] = _Plan(*key)
                     plan.params.append(p)
                     plan.bases.append(base)
                     plan.which.append(place)
                     place += 1
                 base += -(-p.numel() // block) * block
             plans.append(list(mine.values()))
-        _no_overlap(live)
+        _host.adamw_no_overlap(live)
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
         for ps in plans:
             for plan in ps:
-                rows, steps, plan.holds = [], [], []
-                for p, b in zip(plan.params, plan.bases):
-                    st = self._state_of(p)
-                    names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
-                    own = [st[k] for k in names]
-                    rows.append([p.data_ptr(), 0, *(t.data_ptr() for t in own), *((0, 0) if self.state_bits == 32 else ()), p.numel(), b])
-                    steps.append(int(st["step"]))
-                    plan.holds += own                   # what the table points at lives as long as it does
-                    plan.holds.append(p.detach())
-                rows = np.array(rows, dtype=np.int64)
-                per = -(-rows[:, 6] // chunk)           # chunks of each tensor
+                states = [self._state_of(p) for p in plan.params]
+                try:
+                    states, steps = [[st[k] for k in names] for st in states], np.array([int(st["step"]) for st in states], dtype=np.int32)
+                except KeyError as e:
+                    raise ValueError(f"AdamW: a parameter's state lacks {e} (state_bits={self.state_bits})") from None
+                rows, plan.holds = _host.adamw_table(plan.params, states, plan.bases)
+                per = -(-rows[:, 6].numpy() // chunk)   # chunks of each tensor
                 plan.first_chunk = np.cumsum(per) - per
                 which = np.repeat(np.arange(len(per)), per)
                 where = np.stack([which, np.arange(len(which)) - plan.first_chunk[which]], 1).astype(np.int32)
-                plan.table = torch.from_numpy(rows).to(plan.device)
+                plan.table = rows.to(plan.device)
                 plan.chunks = torch.from_numpy(where).to(plan.device)
-                plan.steps = torch.from_numpy(np.array(steps, dtype=np.int32)[which]).to(plan.device)
+                plan.steps = torch.from_numpy(steps[which]).to(plan.device)
         self._watch.bind(groups)
         self._plans = plans
 
@@ -319,10 +306,3 @@ def _dense(t):
 
 def _raw(t):
     return t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
-
-
-def _no_overlap(params):
-    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), p.device.index) for p in params)
-    for a, b in zip(spans, spans[1:]):
-        if a[2] == b[2] and b[0] < a[1]:
-            raise ValueError("AdamW: two parameters share memory; give the optimizer one of them")

@@ -79,11 +79,11 @@ def test_the_watch_reports_what_changed():
 
 
 def test_parameters_that_share_memory_are_found():
-    from erfnet_pytorch_amd.optim import _no_overlap
+    from erfnet_pytorch_amd.optim import _host
     t = torch.zeros(10)
-    _no_overlap([t[:5], t[5:]])
+    _host.adamw_no_overlap([t[:5], t[5:]])
     with pytest.raises(ValueError, match="share memory"):
-        _no_overlap([t[5:], t[:6]])
+        _host.adamw_no_overlap([t[5:], t[:6]])
 
 
 def test_abi_refuses_bad_arguments_without_a_gpu():

@@ -1,0 +1,186 @@
+"""Group norm, label log probabilities and AdamW together: as registered ops (schema, fake kernels, no CPU kernel) and as the pieces
+of one training step."""
+import pytest
+import torch
+
+from erfnet_pytorch_amd import train_ops as TO
+
+T = torch.ops.erfnet_mi355
+U = 2.0 ** -24
+
+
+def _samples(dev, dtype=torch.bfloat16):
+    """op name -> [(args, expected outputs (shape, dtype, strides or None))]"""
+    def t(*shape, dt=dtype):
+        return torch.empty(shape, dtype=dt, device=dev)
+    f, i = torch.float32, torch.int64
+    maps, rows, last = t(2, 20, 8, 16), t(6, 1000), t(2, 20, 8, 16).contiguous(memory_format=torch.channels_last)
+    x = t(2, 8, 16, 24)
+
+    def fwd(z, k, target=True):
+        pos = (z.shape[0], *z.shape[2:])
+        tgt = t(*pos, dt=i) if target else None
+        top = (pos[0], k, *pos[1:])
+        return (z, tgt, k, -100), [(pos if target else (0,), f), (pos, f), ((2, *pos), f), (top, f), (top, i)]
+
+    def bwd(z, k):
+        pos = (z.shape[0], *z.shape[2:])
+        top = (pos[0], k, *pos[1:])
+        return (z, t(*pos, dt=i), t(2, *pos, dt=f), t(*pos, dt=f), t(*top, dt=i), t(*pos, dt=f), t(*pos, dt=f), t(*top, dt=f) if k else None, -100), [(tuple(z.shape), dtype)]
+    return {
+        "class_log_probs_fwd": [fwd(maps, 3), fwd(rows, 5), fwd(last, 2), fwd(maps, 0, False)],
+        "class_log_probs_bwd": [bwd(maps, 3), bwd(rows, 0), bwd(last, 2)],
+        "group_norm_act_fwd": [((x, t(24, dt=f), t(24, dt=f), 4, 1e-5, "relu"), [((2, 8, 16, 24), dtype), ((2, 2, 4), f)]),
+                               ((x, None, None, 24, 1e-5, "silu"), [((2, 8, 16, 24), dtype), ((2, 2, 24), f)])],
+        "group_norm_act_bwd": [((x, x, t(24, dt=f), None, t(2, 2, 4, dt=f), 4, "none"), [((2, 8, 16, 24), dtype), ((24,), f), ((24,), f)])],
+    }
+
+
+def _outs(res):
+    return list(res) if isinstance(res, (tuple, list)) else [res]
+
+
+def test_every_op_is_registered_with_a_schema_a_device_kernel_and_a_fake_kernel():
+    assert set(TO.OPS) == set(_samples("meta"))
+    for name in TO.OPS:
+        op = getattr(T, name).default
+        assert op._schema.name == f"erfnet_mi355::{name}"
+        assert torch._C._dispatch_has_kernel_for_dispatch_key(op.name(), "CUDA") and torch._C._dispatch_has_kernel_for_dispatch_key(op.name(), "Meta")
+        assert not torch._C._dispatch_has_kernel_for_dispatch_key(op.name(), "CPU"), name
+
+
+@pytest.mark.parametrize("name", sorted(_samples("meta")))
+def test_fake_kernels_give_shapes_on_meta_tensors(name):
+    for args, want in _samples("meta")[name]:
+        got = _outs(getattr(T, name)(*args))
+        assert [(tuple(o.shape), o.dtype) for o in got] == want and all(o.device.type == "meta" for o in got)
+
+
+def test_ops_trace_under_fake_tensor_mode():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(4, 64, 128, 64, dtype=torch.bfloat16, device="cuda")
+        y, stats = T.group_norm_act_fwd(x, torch.empty(64, device="cuda"), None, 8, 1e-5, "silu")
+        z = torch.empty(4, 20, 64, 128, device="cuda").contiguous(memory_format=torch.channels_last)
+        lp, ent, st, top, idx = T.class_log_probs_fwd(z, torch.empty(4, 64, 128, dtype=torch.int64, device="cuda"), 3, -100)
+        dz = T.class_log_probs_bwd(z, torch.empty(4, 64, 128, dtype=torch.int64, device="cuda"), st, ent, idx, lp, ent, top, -100)
+    assert tuple(y.shape) == (4, 64, 128, 64) and y.device.type == "cuda" and tuple(stats.shape) == (2, 4, 8)
+    assert tuple(top.shape) == (4, 3, 64, 128) and top.stride() == idx.stride() == (64 * 128 * 3, 1, 128 * 3, 3)
+    assert dz.is_contiguous(memory_format=torch.channels_last)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(NotImplementedError):
+        T.group_norm_act_fwd(torch.zeros(1, 2, 2, 4), None, None, 2, 1e-5, "relu")
+    with pytest.raises(NotImplementedError):
+        T.class_log_probs_fwd(torch.zeros(3, 4), None, 0, -100)
+
+
+@pytest.mark.gpu
+def test_opcheck_against_the_device_kernels():
+    checks = ("test_schema", "test_faketensor")
+    x, dy, w, b = (torch.randn(*s, device="cuda") for s in ((2, 8, 16, 24), (2, 8, 16, 24), (24,), (24,)))
+    torch.library.opcheck(T.group_norm_act_fwd.default, (x, w, b, 4, 1e-5, "silu"), test_utils=checks)
+    y, stats = T.group_norm_act_fwd(x, w, b, 4, 1e-5, "silu")
+    torch.library.opcheck(T.group_norm_act_bwd.default, (dy, x, w, b, stats, 4, "silu"), test_utils=checks)
+    for z in (torch.randn(2, 20, 8, 16, device="cuda"), torch.randn(5, 1000, device="cuda"),
+              torch.randn(2, 20, 8, 16, device="cuda").contiguous(memory_format=torch.channels_last)):
+        t = torch.randint(0, 20, (z.shape[0], *z.shape[2:]), device="cuda")
+        torch.library.opcheck(T.class_log_probs_fwd.default, (z, t, 3, -100), test_utils=checks)
+        lp, ent, st, top, idx = T.class_log_probs_fwd(z, t, 3, -100)
+        torch.library.opcheck(T.class_log_probs_bwd.default, (z, t, st, ent, idx, lp, ent, top, -100), test_utils=checks)
+
+
+def _step_reference(x, params, t, groups):
+    """Loss and gradients of the step below in float64 on the CPU, through torch's own group_norm and log_softmax."""
+    w1, gamma, beta, w2 = (p.detach().cpu().double().requires_grad_() for p in params)
+    h = x.cpu().double().permute(0, 2, 3, 1) @ w1
+    h = torch.nn.functional.silu(torch.nn.functional.group_norm(h.permute(0, 3, 1, 2), groups, gamma, beta, 1e-5))
+    logp = torch.log_softmax(h.permute(0, 2, 3, 1) @ w2, -1)
+    live = (t != -100).double()
+    lp = logp.gather(-1, t.clamp_min(0).unsqueeze(-1))[..., 0] * live
+    ent = -(logp.exp() * logp).sum(-1)
+    loss = (-(lp.sum()) - 0.01 * (ent * live).sum()) / live.sum()
+    return loss, torch.autograd.grad(loss, (w1, gamma, beta, w2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_training_step_of_all_three(bits):
+    """features = x W1, group norm + silu, logits = h W2, mean log loss with an entropy bonus, AdamW; channels-last throughout.
+    Every gradient is a sum of at most 2 x 24 x 40 positions' terms, each a product of a chain of sums of at most 32 terms and of the
+    norm's sums over 24 x 40 x 8 values: 2048 + 8 x 256 additions one after another at the most (far fewer: they are split), so the
+    2-norm of the error is at most 4096 U of the gradient's majorant, which |terms| of one sign bound; twice that is allowed."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    from erfnet_pytorch_amd.norm import GroupNormAct2d
+    from erfnet_pytorch_amd.optim import AdamW
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(2, 16, 24, 40, generator=gen).cuda().contiguous(memory_format=torch.channels_last)
+    t = torch.randint(0, 20, (2, 24, 40), generator=gen)
+    t[:, :3] = -100
+    norm = GroupNormAct2d(4, 32, activation="silu").cuda()
+    w1, w2 = (torch.nn.Parameter((torch.randn(*s, generator=gen) / 4).cuda()) for s in ((16, 32), (32, 20)))
+    params = [w1, norm.weight, norm.bias, w2]
+    opt = AdamW(params, lr=1e-2, weight_decay=1e-2, state_bits=bits)
+    for step in (1, 2, 3):
+        want_loss, want = _step_reference(x, params, t, 4)
+        opt.zero_grad()
+        h = norm((x.permute(0, 2, 3, 1) @ w1).permute(0, 3, 1, 2))
+        out = class_log_probs((h.permute(0, 2, 3, 1) @ w2).permute(0, 3, 1, 2), t.cuda(), top_k=2)
+        live = (t != -100).cuda()
+        loss = (-out.log_prob.sum() - 0.01 * (out.entropy * live).sum()) / live.sum()
+        loss.backward()
+        assert abs(float(loss.detach()) - float(want_loss.detach())) <= 8192 * U * 10
+        for p, g in zip(params, want):
+            assert float((p.grad.cpu().double() - g).norm()) <= 8192 * U * float(g.norm())
+        before = [p.detach().clone() for p in params]
+        state = [{k: v.clone() for k, v in opt.state[p].items()} for p in params] if step > 1 else None
+        opt.step()
+        for i, p in enumerate(params):                     # the update itself, from the gradient that the step had
+            g, q = p.grad.double(), before[i].double()
+            if state is None:
+                m = v = torch.zeros_like(g)
+            elif bits == 32:
+                m, v = state[i]["exp_avg"].double(), state[i]["exp_avg_sq"].double()
+            else:
+                each = lambda k: state[i][k].double().repeat_interleave(256)[:p.numel()].view(p.shape)               # noqa: E731
+                m = state[i]["exp_avg"].float().double() * each("exp_avg_scale")
+                v = (state[i]["exp_avg_sq_root"].float().double() * each("exp_avg_sq_root_scale")) ** 2
+            m, v = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g * g
+            u = 1e-2 / (1 - 0.9 ** step) * m / ((v / (1 - 0.999 ** step)).sqrt() + 1e-8)
+            # 16 roundings of u and of its cancelling moment (|0.9 m| + |0.1 g| <= 20 |u|'s scale), 3 of p: see the optimizer's own tests
+            assert ((p.double() - (q * (1 - 1e-4) - u)).abs() <= 64 * U * (q.abs() + 1e-2 * 10)).all()
+        assert out.top_log_probs.shape == (2, 2, 24, 40)
+
+
+@pytest.mark.gpu
+def test_the_network_trains_on_label_log_probabilities_with_adamw():
+    """ERFNet's logits through class_log_probs: the gradient is the cross entropy's, and AdamW's update reaches the packed weights of
+    the next forward pass."""
+    from erfnet_pytorch_amd import erfnet as E, synthetic as S
+    from erfnet_pytorch_amd.loss import CrossEntropyLoss2d, class_log_probs
+    from erfnet_pytorch_amd.optim import AdamW
+    model = E.ERFNet(20)
+    S.load_synthetic(model)
+    model = model.cuda().eval()                             # running statistics, no dropout: the same logits every time
+    x = S.synthetic_images(2, 64, 128, seed=1).cuda()
+    t = S.synthetic_labels(2, 64, 128, 20, seed=1).cuda().view(2, 64, 128)
+    opt = AdamW(model.parameters(), lr=1e-3, state_bits=8)
+    logits = model(x)
+    loss = -class_log_probs(logits, t).log_prob.mean()
+    d1, = torch.autograd.grad(loss, logits, retain_graph=True)
+    d2, = torch.autograd.grad(CrossEntropyLoss2d()(logits, t), logits, retain_graph=True)
+    # each entry (p - [j = t]) / count: log p to 100 U at logits below 100 either way, the exponentials of the cross entropy another 100 U
+    assert (d1 - d2).abs().max() <= 400 * U * 2 / t.numel()
+    loss.backward()
+    with torch.no_grad():
+        before = model(x)
+    opt.step()
+    assert all(p.isfinite().all() for p in model.parameters())
+    with torch.no_grad():
+        after = model(x)
+    fresh = E.ERFNet(20)
+    fresh.load_state_dict(model.state_dict())
+    with torch.no_grad():
+        again = fresh.cuda().eval()(x)
+    assert not torch.equal(before, after) and torch.equal(after, again)
