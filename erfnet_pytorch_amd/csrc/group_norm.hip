@@ -37,6 +37,7 @@ struct GnArgs {
     long long HW;
     int N, C, G, P;
     int chunks, lanes;                 // a pixel's chunks of VEC channels in one workgroup (team), and the pixels side by side in it
+    int runs;                          // runs that `parts` holds (P of the launch that wrote it)
     int team;                          // a group per team: its threads
     int rows;                          // parameter gradients: rows of `sums` (N, or runs of images already summed up)
     float eps;
@@ -87,6 +88,7 @@ template <typename T, int VEC> __device__ __forceinline__ void vec_store(T* p, c
 // chunk), so that a thread keeps its channels and the workgroup reads whole pixels side by side.
 #define GN_THREADS 256
 #define GN_UNROLL 8
+#define GN_JOIN_CHANNELS 512       // at most, where the apply kernels join the runs themselves
 struct GnPlace { int n, run, chunk, lane, c; long long first, last; bool on; };        // c: first channel; pixels [first, last) of image n
 template <int VEC> __device__ __forceinline__ GnPlace gn_place(const GnArgs& a) {
     GnPlace q;
@@ -110,6 +112,52 @@ __device__ __forceinline__ void gn_join(float& mean, float& m2, float& n, float 
         mean = fmaf(d, w, mean);
         m2 += om2 + d * d * (n * w);
         n = all;
+    }
+}
+
+// The pixel lanes of a workgroup joined in halves: lane 0 has its channels' mean and sum of squares over all lanes
+template <int VEC>
+__device__ __forceinline__ void gn_join_lanes(const GnArgs& a, const GnPlace& q, float* mean, float* m2, float& n, float (*sh)[VEC][GN_THREADS], float* shn) {
+    for (int have = a.lanes; have > 1;) {
+        const int keep = (have + 1) / 2;
+        __syncthreads();
+        if (q.on && q.lane >= keep && q.lane < have) {
+            shn[threadIdx.x] = n;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { sh[0][e][threadIdx.x] = mean[e]; sh[1][e][threadIdx.x] = m2[e]; }
+        }
+        __syncthreads();
+        if (q.on && q.lane + keep < have) {
+            const int o = threadIdx.x + keep * a.chunks;
+            const float on = shn[o], all = n + on, w = all > 0.f ? on / all : 0.f, nw = n * w;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = sh[0][e][o] - mean[e];
+                mean[e] = fmaf(d, w, mean[e]);
+                m2[e] += sh[1][e][o] + d * d * nw;
+            }
+            n = all;
+        }
+        have = keep;
+    }
+}
+// ... added in halves
+template <int VEC>
+__device__ __forceinline__ void gn_add_lanes(const GnArgs& a, const GnPlace& q, float* s, float* r, float (*sh)[VEC][GN_THREADS]) {
+    for (int have = a.lanes; have > 1;) {
+        const int keep = (have + 1) / 2;
+        __syncthreads();
+        if (q.on && q.lane >= keep && q.lane < have) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { sh[0][e][threadIdx.x] = s[e]; sh[1][e][threadIdx.x] = r[e]; }
+        }
+        __syncthreads();
+        if (q.on && q.lane + keep < have) {
+            const int o = threadIdx.x + keep * a.chunks;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { s[e] += sh[0][e][o]; r[e] += sh[1][e][o]; }
+        }
+        have = keep;
     }
 }
 
@@ -157,29 +205,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnArgs a) {
             n += 1.f;
         }
     }
-    // the pixel lanes in halves
-    for (int have = a.lanes; have > 1;) {
-        const int keep = (have + 1) / 2;
-        __syncthreads();
-        if (q.on && q.lane >= keep && q.lane < have) {
-            shn[threadIdx.x] = n;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) { sh[0][e][threadIdx.x] = mean[e]; sh[1][e][threadIdx.x] = m2[e]; }
-        }
-        __syncthreads();
-        if (q.on && q.lane + keep < have) {
-            const int o = threadIdx.x + keep * a.chunks;
-            const float on = shn[o], all = n + on, w = all > 0.f ? on / all : 0.f, nw = n * w;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float d = sh[0][e][o] - mean[e];
-                mean[e] = fmaf(d, w, mean[e]);
-                m2[e] += sh[1][e][o] + d * d * nw;
-            }
-            n = all;
-        }
-        have = keep;
-    }
+    gn_join_lanes<VEC>(a, q, mean, m2, n, sh, shn);
     if (q.on && q.lane == 0) {
         float* out = a.parts + 2 * (((long long)q.n * a.P + q.run) * a.C + q.c);
 #pragma unroll
@@ -191,11 +217,11 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnArgs a) {
 __global__ __launch_bounds__(1024) void gn_finalize_kernel(const GnArgs a) {
     __shared__ float sh[3][16];
     const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
-    const long long per = (a.HW + a.P - 1) / a.P;
+    const long long per = (a.HW + a.runs - 1) / a.runs;
     float mean = 0.f, m2 = 0.f, count = 0.f;
-    for (long long i = threadIdx.x; i < (long long)a.P * cpg; i += 1024) {
+    for (long long i = threadIdx.x; i < (long long)a.runs * cpg; i += 1024) {
         const long long p = i / cpg, c = g * cpg + (i - p * cpg), left = a.HW - p * per;
-        const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.P + p) * a.C + c));
+        const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.runs + p) * a.C + c));
         gn_join(mean, m2, count, v.x, v.y, left <= 0 ? 0.f : (float)(left < per ? left : per));
     }
 #pragma unroll
@@ -222,15 +248,75 @@ __device__ __forceinline__ void gn_channels(const GnArgs& a, const GnPlace& q, f
     }
 }
 
-template <typename T, int VEC, int ACT>
+// The same from the runs, where a workgroup has all of an image's channels: its threads join their channels' runs, and each then goes
+// over the channels of its groups.  All channels count the same pixels: a group's mean is the mean of theirs, its sum of squares that
+// of theirs and of HW times the squares of their distances.
+template <int VEC>
+__device__ __forceinline__ void gn_channels_from_runs(const GnArgs& a, const GnPlace& q, float* mean, float* scale, float* beta, float (*sh)[VEC][GN_THREADS],
+                                                      float* shn, float (*channel)[GN_JOIN_CHANNELS]) {
+    float m2[VEC], n = 0.f;
+    const long long per = (a.HW + a.runs - 1) / a.runs;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) mean[e] = m2[e] = 0.f;
+    if (q.on)
+        for (int p = q.lane; p < a.runs; p += a.lanes) {
+            const float* v = a.parts + 2 * (((long long)q.n * a.runs + p) * a.C + q.c);
+            const long long left = a.HW - p * per;
+            const float on = left <= 0 ? 0.f : (float)(left < per ? left : per), all = n + on, w = all > 0.f ? on / all : 0.f, nw = n * w;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = v[2 * e] - mean[e];
+                mean[e] = fmaf(d, w, mean[e]);
+                m2[e] += v[2 * e + 1] + d * d * nw;
+            }
+            n = all;
+        }
+    gn_join_lanes<VEC>(a, q, mean, m2, n, sh, shn);
+    if (q.on && q.lane == 0) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { channel[0][q.c + e] = mean[e]; channel[1][q.c + e] = m2[e]; }
+    }
+    __syncthreads();
+    if (!q.on) return;
+    const int cpg = a.C / a.G;
+    int have = -1;
+    float gmean = 0.f, rstd = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const int c = q.c + e, g = c / cpg;
+        if (g != have) {
+            float s = 0.f, d = 0.f;
+            for (int j = g * cpg; j < (g + 1) * cpg; ++j) s += channel[0][j];
+            gmean = s / (float)cpg;
+            for (int j = g * cpg; j < (g + 1) * cpg; ++j) d += channel[1][j] + (float)a.HW * (channel[0][j] - gmean) * (channel[0][j] - gmean);
+            rstd = 1.f / sqrtf(d / ((float)a.HW * cpg) + a.eps);
+            have = g;
+            if (q.run == 0 && q.lane == 0 && c == g * cpg) {
+                a.mean[(long long)q.n * a.G + g] = gmean;
+                a.rstd[(long long)q.n * a.G + g] = rstd;
+            }
+        }
+        mean[e] = gmean;
+        scale[e] = rstd * (a.gamma ? a.gamma[c] : 1.f);
+        beta[e] = a.beta ? a.beta[c] : 0.f;
+    }
+}
+
+template <typename T, int VEC, int ACT, bool JOINED>
 __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnArgs a) {
     constexpr int U = 4;
     const GnPlace q = gn_place<VEC>(a);
-    if (!q.on) return;
     const T* x = (const T*)a.x + (long long)q.n * a.HW * a.C + q.c;
     T* y = (T*)a.y + (long long)q.n * a.HW * a.C + q.c;
     float mean[VEC], scale[VEC], beta[VEC];
-    gn_channels<VEC>(a, q, mean, scale, beta);
+    if constexpr (JOINED) {
+        if (!q.on) return;
+        gn_channels<VEC>(a, q, mean, scale, beta);
+    } else {
+        __shared__ float sh[2][VEC][GN_THREADS], shn[GN_THREADS], channel[2][GN_JOIN_CHANNELS];
+        gn_channels_from_runs<VEC>(a, q, mean, scale, beta, sh, shn, channel);
+        if (!q.on) return;
+    }
     for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
         float f[U][VEC];
 #pragma unroll
@@ -288,21 +374,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const GnArgs a)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) r[e] *= a.rstd[(long long)q.n * a.G + (q.c + e) / cpg];
     }
-    for (int have = a.lanes; have > 1;) {
-        const int keep = (have + 1) / 2;
-        __syncthreads();
-        if (q.on && q.lane >= keep && q.lane < have) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) { sh[0][e][threadIdx.x] = s[e]; sh[1][e][threadIdx.x] = r[e]; }
-        }
-        __syncthreads();
-        if (q.on && q.lane + keep < have) {
-            const int o = threadIdx.x + keep * a.chunks;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) { s[e] += sh[0][e][o]; r[e] += sh[1][e][o]; }
-        }
-        have = keep;
-    }
+    gn_add_lanes<VEC>(a, q, s, r, sh);
     if (q.on && q.lane == 0) {
         float* out = a.parts + 2 * (((long long)q.n * a.P + q.run) * a.C + q.c);
 #pragma unroll
@@ -322,8 +394,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_finalize_kernel(const GnArgs a) {
         const bool on = lane < lanes && c0 + j < cpg;
         double p = 0, r = 0;
         if (on)
-            for (int i = lane; i < a.P; i += lanes) {
-                const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.P + i) * a.C + c));
+            for (int i = lane; i < a.runs; i += lanes) {
+                const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.runs + i) * a.C + c));
                 p += v.x;
                 r += v.y;
             }
@@ -358,19 +430,21 @@ __global__ __launch_bounds__(1024) void gn_bwd_finalize_kernel(const GnArgs a) {
     }
 }
 
-// dbeta = sum_n A and dgamma = sum_n B: 64 channels a workgroup, four image lanes with 4 loads in flight each
+// dbeta = sum A and dgamma = sum B over rows [C][2] of images or runs: 16 channels a workgroup, 16 row lanes with 4 loads in flight each
+#define GN_SIDE 16
 __device__ __forceinline__ void gn_row_sums(const float* sums, long long first, long long last, int C, int c, double (*sh)[GN_THREADS], double& p, double& r) {
+    constexpr int LANES = GN_THREADS / GN_SIDE;
     p = r = 0;
     if (c < C) {
-        long long n = first + (threadIdx.x >> 6);
-        for (; n + 12 < last; n += 16) {
+        long long n = first + threadIdx.x / GN_SIDE;
+        for (; n + 3 * LANES < last; n += 4 * LANES) {
             float2 v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = *(const float2*)(sums + 2 * ((n + 4 * u) * C + c));
+            for (int u = 0; u < 4; ++u) v[u] = *(const float2*)(sums + 2 * ((n + u * LANES) * C + c));
 #pragma unroll
             for (int u = 0; u < 4; ++u) { p += v[u].x; r += v[u].y; }
         }
-        for (; n < last; n += 4) {
+        for (; n < last; n += LANES) {
             const float2 v = *(const float2*)(sums + 2 * (n * C + c));
             p += v.x;
             r += v.y;
@@ -378,15 +452,18 @@ __device__ __forceinline__ void gn_row_sums(const float* sums, long long first, 
     }
     sh[0][threadIdx.x] = p;
     sh[1][threadIdx.x] = r;
-    __syncthreads();
-    if (threadIdx.x < 64)
-        for (int w = 1; w < 4; ++w) { p += sh[0][threadIdx.x + 64 * w]; r += sh[1][threadIdx.x + 64 * w]; }
+    for (int o = GN_THREADS / 2; o >= GN_SIDE; o /= 2) {
+        __syncthreads();
+        if ((int)threadIdx.x < o) { sh[0][threadIdx.x] += sh[0][threadIdx.x + o]; sh[1][threadIdx.x] += sh[1][threadIdx.x + o]; }
+    }
+    p = sh[0][threadIdx.x];
+    r = sh[1][threadIdx.x];
 }
 __device__ __forceinline__ void gn_param_grads(const GnArgs& a, const float* sums, int block, double (*sh)[GN_THREADS]) {
-    const int c = block * 64 + (threadIdx.x & 63);
+    const int c = block * GN_SIDE + (threadIdx.x % GN_SIDE);
     double p, r;
     gn_row_sums(sums, 0, a.rows, a.C, c, sh, p, r);
-    if (threadIdx.x < 64 && c < a.C) {
+    if (threadIdx.x < GN_SIDE && c < a.C) {
         if (a.dbeta) a.dbeta[c] = (float)p;
         if (a.dgamma) a.dgamma[c] = (float)r;
     }
@@ -398,41 +475,94 @@ __global__ __launch_bounds__(GN_THREADS) void gn_param_grads_kernel(const GnArgs
 // ... of many images: runs of them first, to rows of `out`
 __global__ __launch_bounds__(GN_THREADS) void gn_image_runs_kernel(const GnArgs a, float* out) {
     __shared__ double sh[2][GN_THREADS];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
+    const int c = blockIdx.x * GN_SIDE + (threadIdx.x % GN_SIDE);
     const long long per = (a.N + (long long)gridDim.y - 1) / gridDim.y, first = blockIdx.y * per, last = first + per < a.N ? first + per : a.N;
     double p, r;
     gn_row_sums(a.sums, first, last, a.C, c, sh, p, r);
-    if (threadIdx.x < 64 && c < a.C) {
+    if (threadIdx.x < GN_SIDE && c < a.C) {
         out[2 * ((long long)blockIdx.y * a.C + c)] = (float)p;
         out[2 * ((long long)blockIdx.y * a.C + c) + 1] = (float)r;
     }
 }
 
+// s1 / M and s2 / M of a thread's channels from the runs, as gn_channels_from_runs
+template <int VEC>
+__device__ __forceinline__ void gn_sums_from_runs(const GnArgs& a, const GnPlace& q, float* k1, float* k2, float (*sh)[VEC][GN_THREADS],
+                                                  float (*channel)[GN_JOIN_CHANNELS]) {
+    float s[VEC], r[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s[e] = r[e] = 0.f;
+    if (q.on)
+        for (int p = q.lane; p < a.runs; p += a.lanes) {
+            const float* v = a.parts + 2 * (((long long)q.n * a.runs + p) * a.C + q.c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { s[e] += v[2 * e]; r[e] += v[2 * e + 1]; }
+        }
+    gn_add_lanes<VEC>(a, q, s, r, sh);
+    if (q.on && q.lane == 0) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float gamma = a.gamma ? a.gamma[q.c + e] : 1.f;
+            channel[0][q.c + e] = gamma * s[e];
+            channel[1][q.c + e] = gamma * r[e];
+        }
+    }
+    __syncthreads();
+    if (!q.on) return;
+    const int cpg = a.C / a.G;
+    const float m = (float)a.HW * cpg;
+    int have = -1;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const int g = (q.c + e) / cpg;
+        if (g != have) {
+            s1 = s2 = 0.f;
+            for (int j = g * cpg; j < (g + 1) * cpg; ++j) { s1 += channel[0][j]; s2 += channel[1][j]; }
+            s1 /= m;
+            s2 /= m;
+            have = g;
+        }
+        k1[e] = s1;
+        k2[e] = s2;
+    }
+}
+
 // dx; and, by the workgroups behind those of the last run, the parameter gradients
-template <typename T, int VEC, int ACT>
+template <typename T, int VEC, int ACT, bool JOINED>
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnArgs a) {
     constexpr int U = 4;
     if (blockIdx.x >= (unsigned)(a.N * a.P)) {
         __shared__ double sh[2][GN_THREADS];
         if (blockIdx.y) return;
-        gn_param_grads(a, a.sums, (int)(blockIdx.x - (unsigned)(a.N * a.P)), sh);
+        gn_param_grads(a, JOINED ? a.sums : a.parts, (int)(blockIdx.x - (unsigned)(a.N * a.P)), sh);
         return;
     }
     const GnPlace q = gn_place<VEC>(a);
-    if (!q.on) return;
     const long long at = (long long)q.n * a.HW * a.C + q.c;
     const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
     T* dx = (T*)a.dx + at;
     float mean[VEC], scale[VEC], beta[VEC], k1[VEC], k2[VEC];          // dx = scale du - k1 - (x - mean) k2
-    gn_channels<VEC>(a, q, mean, scale, beta);
     const int cpg = a.C / a.G;
+    if constexpr (JOINED) {
+        if (!q.on) return;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float2 m = *(const float2*)(a.sums + 2 * (long long)a.N * a.C + 2 * ((long long)q.n * a.G + (q.c + e) / cpg));
+            k1[e] = m.x;
+            k2[e] = m.y;
+        }
+    } else {
+        __shared__ float sh[2][VEC][GN_THREADS], channel[2][GN_JOIN_CHANNELS];
+        gn_sums_from_runs<VEC>(a, q, k1, k2, sh, channel);
+        if (!q.on) return;
+    }
+    gn_channels<VEC>(a, q, mean, scale, beta);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        const long long g = (long long)q.n * a.G + (q.c + e) / cpg;
-        const float2 m = *(const float2*)(a.sums + 2 * (long long)a.N * a.C + 2 * g);
-        const float rstd = a.rstd[g];
-        k1[e] = rstd * m.x;
-        k2[e] = rstd * rstd * m.y;
+        const float rstd = a.rstd[(long long)q.n * a.G + (q.c + e) / cpg];
+        k1[e] *= rstd;
+        k2[e] *= rstd * rstd;
     }
     for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
         float f[U][VEC], d[U][VEC];
@@ -646,16 +776,17 @@ template <int VEC> static inline dim3 gn_plan(GnArgs& a, int each, int most) {
 }
 
 // The plan of a group per team: channels per access (the most that divide a group) and the smallest team that has the values in
-// registers and either fills the chip with threads or leaves each thread one access.  Groups of more values than 4096 (backward 2048)
-// for each channel of an access are faster by runs of pixels, in three launches.  Group against runs, forward / backward, in us:
-// 64 x 64 x 1024 in 8 groups bf16 9 / 18 against 17 / 24; 64 x 128 x 4096 in 32 groups 73 / 155 against 57 / 97;
-// 3 x 30 x 5673 in 6 groups 15 / 23 against 11 / 13; 512 x 128 x 64 in 16 groups 9 / 24 against 65 / 96.
+// registers and either fills the chip with threads or leaves each thread one access.  Large groups, and those whose narrow accesses
+// leave most of each cache line to other workgroups, are faster by runs of pixels.  Group against runs, forward / backward, in us:
+// 64 x 64 x 1024 in 8 groups (8 channels an access) bf16 9 / 18 against 17 / 24; 64 x 128 x 4096 in 32 groups (4) 73 / 155 against
+// 57 / 95; 64 x 64 x 4096 in 8 groups (8) 25 / 54 against 28 / 47; 3 x 30 x 5673 in 6 groups (1) 15 / 23 against 10 / 10;
+// 64 x 48 x 512 in 16 groups (1) 11 / 16 against 19 / 26; 512 x 128 x 64 in 16 groups (8) 9 / 24 against 65 / 96.
 static bool gn_group_plan(GnArgs& a, int dtype, unsigned long long addresses, int& vec, bool backward) {
     const int cpg = a.C / a.G;
     vec = gn_vec(dtype, cpg, addresses);
     a.chunks = cpg / vec;
     const long long groups = (long long)a.N * a.G;
-    if (a.HW * cpg > (backward ? 2048 : 4096) * vec) return false;
+    if (a.HW * cpg > (backward ? 2048 * vec : vec == 8 ? 32768 : vec == 4 ? 8192 : 4096)) return false;
     for (a.team = 8; a.team <= 1024; a.team = a.team == 8 ? 64 : 4 * a.team) {
         a.lanes = a.team / a.chunks;
         if (a.lanes && a.HW <= (long long)a.lanes * GN_KEEP / vec && (a.team == 1024 || groups * a.team >= (1 << 17) || a.HW <= a.lanes)) return true;
@@ -676,7 +807,7 @@ static void gn_group_fwd_launch(GnArgs a, hipStream_t s) {
 }
 static void gn_param_grads_launch(GnArgs a, hipStream_t s) {
     if (!a.dgamma && !a.dbeta) return;
-    const unsigned blocks = (unsigned)((a.C + 63) / 64);
+    const unsigned blocks = (unsigned)((a.C + GN_SIDE - 1) / GN_SIDE);
     const float* sums = a.sums;
     a.rows = gn_image_runs(a.N);
     if (a.rows > 1) {
@@ -693,22 +824,38 @@ static void gn_group_bwd_launch(GnArgs a, hipStream_t s) {
     gn_param_grads_launch(a, s);
 }
 
+// Whether the apply kernels join the runs: that costs each of their workgroups a look at all runs of its image, and saves a launch
+// (3 x 30 x 5673 forward / backward 10.2 / 10.4 us against 11.4 / 13.3; 6 x 128 x 8192 and larger maps alike)
+static inline bool gn_join_in_apply(const GnArgs& a, dim3 grid) {
+    return grid.y == 1 && a.C <= GN_JOIN_CHANNELS && a.C / a.G <= 128 && (long long)a.P * a.C <= 8192;
+}
+
 template <typename T, int VEC, int ACT>
 static void gn_fwd_launch(GnArgs a, hipStream_t s) {
-    hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS), dim3(GN_THREADS), 0, s, a);
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
-    hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT>), gn_plan<VEC>(a, 4, 1 << 20), dim3(GN_THREADS), 0, s, a);
+    dim3 grid = gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS);
+    hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), grid, dim3(GN_THREADS), 0, s, a);
+    const bool join = gn_join_in_apply(a, grid);
+    a.runs = a.P;
+    if (!join) hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
+    grid = gn_plan<VEC>(a, 4, 1 << 20);
+    if (join) hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT, false>), grid, dim3(GN_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT, true>), grid, dim3(GN_THREADS), 0, s, a);
 }
 
 template <typename T, int VEC, int ACT>
 static void gn_bwd_launch(GnArgs a, hipStream_t s) {
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, VEC, ACT>), gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS), dim3(GN_THREADS), 0, s, a);
-    hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
-    dim3 grid = gn_plan<VEC>(a, 4, 1 << 20);
-    const bool few = gn_image_runs(a.N) == 1 && (a.dgamma || a.dbeta);
-    a.rows = a.N;
-    if (few) grid.x += (unsigned)((a.C + 63) / 64);
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+    dim3 grid = gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS);
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, VEC, ACT>), grid, dim3(GN_THREADS), 0, s, a);
+    a.runs = a.P;
+    // the parameter gradients come from the runs as they are where these are few, else from the images' sums
+    const bool params = a.dgamma || a.dbeta, join = gn_join_in_apply(a, grid) && (!params || (long long)a.N * a.runs <= 1024);
+    if (!join) hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
+    grid = gn_plan<VEC>(a, 4, 1 << 20);
+    const bool few = params && (join || gn_image_runs(a.N) == 1);
+    a.rows = join ? a.N * a.runs : a.N;
+    if (few) grid.x += (unsigned)((a.C + GN_SIDE - 1) / GN_SIDE);
+    if (join) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, VEC, ACT, false>), grid, dim3(GN_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, VEC, ACT, true>), grid, dim3(GN_THREADS), 0, s, a);
     if (!few) gn_param_grads_launch(a, s);
 }
 
