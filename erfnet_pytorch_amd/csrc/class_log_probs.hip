@@ -130,33 +130,35 @@ __device__ __forceinline__ void lp_finish(const LpArgs& a, const LpTarget& q, lo
 // registers, sorted; more (KT < 0) are found by rounds over the classes, as they are where NaN or too few finite values upset the order.
 #define BATCH 8
 
+// P neighbouring values as they lie in memory, taken apart after all loads of a set
+template <typename T, int P> struct Positions;
+template <> struct Positions<float, 1> { float raw; };
+template <> struct Positions<float, 4> { f32x4 raw; };
+template <> struct Positions<bf16raw, 1> { bf16raw raw; };
+template <> struct Positions<bf16raw, 4> { i32x2 raw; };
 template <typename T, int P>
-__device__ __forceinline__ void load_positions(const T* p, float* f) {
-    if constexpr (P == 1) f[0] = Elem<T>::ld(p);
-    else if constexpr (sizeof(T) * P == 16) {
-        const f32x4 v = *(const f32x4*)p;
+__device__ __forceinline__ Positions<T, P> read_positions(const T* p) {
+    return Positions<T, P>{*(const decltype(Positions<T, P>::raw)*)p};
+}
+template <typename T, int P>
+__device__ __forceinline__ void position_values(const Positions<T, P>& v, float* f) {
+    if constexpr (P == 1) f[0] = Elem<T>::to_f32(v.raw);
+    else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = v[i];
-    } else if constexpr (sizeof(T) == 4) {
-        const f32x2 v = *(const f32x2*)p;
-        f[0] = v[0]; f[1] = v[1];
-    } else if constexpr (P == 4) {
-        const i32x2 r = *(const i32x2*)p;
-        f[0] = __uint_as_float((unsigned)r[0] << 16); f[1] = __uint_as_float((unsigned)r[0] & 0xFFFF0000u);
-        f[2] = __uint_as_float((unsigned)r[1] << 16); f[3] = __uint_as_float((unsigned)r[1] & 0xFFFF0000u);
+        for (int i = 0; i < 4; ++i) f[i] = v.raw[i];
     } else {
-        const unsigned r = *(const unsigned*)p;
-        f[0] = __uint_as_float(r << 16); f[1] = __uint_as_float(r & 0xFFFF0000u);
+        f[0] = __uint_as_float((unsigned)v.raw[0] << 16); f[1] = __uint_as_float((unsigned)v.raw[0] & 0xFFFF0000u);
+        f[2] = __uint_as_float((unsigned)v.raw[1] << 16); f[3] = __uint_as_float((unsigned)v.raw[1] & 0xFFFF0000u);
     }
 }
+template <typename T, int P>
+__device__ __forceinline__ void load_positions(const T* p, float* f) { position_values<T, P>(read_positions<T, P>(p), f); }
 
 template <typename T, int P>
 __device__ __forceinline__ void store_positions(T* p, const float* f) {
     if constexpr (P == 1) Elem<T>::st(p, f[0]);
-    else if constexpr (sizeof(T) * P == 16) *(f32x4*)p = f32x4{f[0], f[1], f[2], f[3]};
-    else if constexpr (sizeof(T) == 4) *(f32x2*)p = f32x2{f[0], f[1]};
-    else if constexpr (P == 4) *(i32x2*)p = pack_bf16x4(f32x4{f[0], f[1], f[2], f[3]});
-    else *(int*)p = pack_bf16x2(f[0], f[1]);
+    else if constexpr (sizeof(T) == 4) *(f32x4*)p = f32x4{f[0], f[1], f[2], f[3]};
+    else *(i32x2*)p = pack_bf16x4(f32x4{f[0], f[1], f[2], f[3]});
 }
 
 template <int P>
@@ -212,14 +214,16 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
             for (int k = 0; k < K; ++k) { tv[p][k] = -INFINITY; tc[p][k] = -1; }
         }
         for (int c0 = 0; c0 < a.C; c0 += BATCH) {
+            Positions<T, P> raw[BATCH];
             float f[BATCH][P];
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                if (c0 + b < a.C) load_positions<T, P>(row + (c0 + b) * a.sc, f[b]);
-                else {
+            for (int b = 0; b < BATCH; ++b)
+                if (c0 + b < a.C) raw[b] = read_positions<T, P>(row + (c0 + b) * a.sc);
 #pragma unroll
-                    for (int p = 0; p < P; ++p) f[b][p] = -INFINITY;
-                }
+            for (int b = 0; b < BATCH; ++b) {
+                position_values<T, P>(raw[b], f[b]);
+#pragma unroll
+                for (int p = 0; p < P; ++p) f[b][p] = c0 + b < a.C ? f[b][p] : -INFINITY;
             }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -332,23 +336,36 @@ template <int TEAM> __device__ __forceinline__ void team_sync() {
     }
 }
 
-// Classes of chunk q of a row whose first class lies `off` classes behind a boundary; what is not part of the row reads -inf
+// Chunk q of a row whose first class lies `off` classes behind a boundary, as it lies in memory; what is not part of the row is -inf.
+// It is taken apart by chunk_values, after all loads of a set: taken apart behind the branch, each load would be waited for alone.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int off, int C, int q, float* f) {
+__device__ __forceinline__ i32x4 load_chunk(const T* row, int off, int C, int q) {
     constexpr int E = Elem<T>::EPC;
     const int c0 = q * E - off;
-    if (c0 >= 0 && c0 + E <= C) {
-        const i32x4 r = *(const i32x4*)(row + c0);
+    if (c0 >= 0 && c0 + E <= C) return *(const i32x4*)(row + c0);
+    i32x4 r;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (E == 4) f[e] = __int_as_float(r[e & 3]);
-            else f[e] = (e & 1) ? __uint_as_float((unsigned)r[(e >> 1) & 3] & 0xFFFF0000u) : __uint_as_float((unsigned)r[(e >> 1) & 3] << 16);
+    for (int w = 0; w < 4; ++w) {
+        if constexpr (E == 4) {
+            r[w] = c0 + w >= 0 && c0 + w < C ? __float_as_int(row[c0 + w]) : (int)0xFF800000u;
+        } else {
+            const int c = c0 + 2 * w;
+            const unsigned lo = c >= 0 && c < C ? row[c] : 0xFF80u, hi = c + 1 >= 0 && c + 1 < C ? row[c + 1] : 0xFF80u;
+            r[w] = (int)(lo | hi << 16);
         }
-    } else {
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void chunk_values(const i32x4& r, float* f) {
+    constexpr int E = Elem<T>::EPC;
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = c0 + e >= 0 && c0 + e < C ? Elem<T>::ld(row + c0 + e) : -INFINITY;
+    for (int e = 0; e < E; ++e) {
+        if (E == 4) f[e] = __int_as_float(r[e & 3]);
+        else f[e] = (e & 1) ? __uint_as_float((unsigned)r[(e >> 1) & 3] & 0xFFFF0000u) : __uint_as_float((unsigned)r[(e >> 1) & 3] << 16);
     }
 }
+#define NO_CLASSES(T) (Elem<T>::EPC == 4 ? (int)0xFF800000u : (int)0xFF80FF80u)          // -inf in every place of a word
 
 // How many of n ranks in LDS are above r; 8 reads are in flight together
 __device__ __forceinline__ int count_above(const u64* ranks, int n, u64 r) {
@@ -427,14 +444,14 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     Stat st{-INFINITY, 0.f, 0.f};
     float f[UNROLL][E];
     for (int q = q0 + tid; q < (TEAM < 256 ? q0 + TEAM : q1); q += TEAM * UNROLL) {
+        i32x4 raw[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            if (q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
-            else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) f[u][e] = -INFINITY;
-            }
+            raw[u] = i32x4{NO_CLASSES(T), NO_CLASSES(T), NO_CLASSES(T), NO_CLASSES(T)};
+            if (q + u * TEAM < q1) raw[u] = load_chunk(row, off, a.C, q + u * TEAM);
         }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) chunk_values<T>(raw[u], f[u]);
         float most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
@@ -524,7 +541,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
                     const int q = q0 + sh.winner[p / each] + p % each * TEAM;
                     if (q >= q1) continue;
                     float v[E];
-                    load_chunk(row, off, a.C, q, v);
+                    chunk_values<T>(load_chunk(row, off, a.C, q), v);
                     collect(v, q, least);
                 }
             }
@@ -692,14 +709,15 @@ __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a)
 #pragma unroll
         for (int p = 0; p < P; ++p) some = some || any[p];
         for (int c0 = 0; c0 < a.C; c0 += BATCH) {
-            float f[BATCH][P];
+            Positions<T, P> raw[BATCH];
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
-                if (some && c0 + b < a.C) load_positions<T, P>(row + (c0 + b) * a.sc, f[b]);
+                if (some && c0 + b < a.C) raw[b] = read_positions<T, P>(row + (c0 + b) * a.sc);
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
                 if (c0 + b < a.C) {
-                    float d[P];
+                    float f[P], d[P];
+                    position_values<T, P>(raw[b], f);
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
                         float own = t[p] == c0 + b ? gl[p] : 0.f;
@@ -707,7 +725,7 @@ __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a)
 #pragma unroll
                             for (int k = 0; k < K; ++k) own += jk[k][p] == c0 + b ? gk[k][p] : 0.f;
                         }
-                        d[p] = any[p] ? lp_grad(f[b][p], base[p], logs[p], gh[p], pull[p]) + own : 0.f;
+                        d[p] = any[p] ? lp_grad(f[p], base[p], logs[p], gh[p], pull[p]) + own : 0.f;
                     }
                     store_positions<T, P>(out + (c0 + b) * a.dc, d);
                 }
@@ -755,17 +773,18 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     if (gh != 0.f) pull = fmaf(gh, a.entropy[i], pull);
     {
         const int q = q0 + tid;
-        float f[BWD_UNROLL][E];
+        i32x4 raw[BWD_UNROLL];
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u)
-            if (any && q + u * TEAM < q1) load_chunk(row, off, a.C, q + u * TEAM, f[u]);
+            if (any && q + u * TEAM < q1) raw[u] = load_chunk(row, off, a.C, q + u * TEAM);
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u) {
             if (q + u * TEAM >= q1) break;
             const int c0 = (q + u * TEAM) * E - off;
-            float d[E];
+            float f[E], d[E];
+            chunk_values<T>(raw[u], f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) d[e] = any ? lp_grad(f[u][e], base, logs, gh, pull) : 0.f;
+            for (int e = 0; e < E; ++e) d[e] = any ? lp_grad(f[e], base, logs, gh, pull) : 0.f;
             if (c0 >= 0 && c0 + E <= a.C && off == dist) {
                 if constexpr (E == 4) *(f32x4*)(out + c0) = f32x4{d[0], d[1], d[2], d[3]};
                 else *(i32x4*)(out + c0) = i32x4{pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3]), pack_bf16x2(d[4], d[5]), pack_bf16x2(d[6], d[7])};

@@ -8,6 +8,9 @@
 // forward pass's signs; folding the mean into a shift instead would cost u its digits where |mean| is far above the spread.
 #include "../../include/erfnet_mi355.h"
 #include "common.cuh"
+#include <type_traits>
+
+template <int N> using Int = std::integral_constant<int, N>;
 
 __device__ __forceinline__ float gn_u(float x, float mean, float a, float beta) { return fmaf(x - mean, a, beta); }
 
@@ -317,19 +320,22 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnArgs a) {
         gn_channels_from_runs<VEC>(a, q, mean, scale, beta, sh, shn, channel);
         if (!q.on) return;
     }
-    for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
-        float f[U][VEC];
+    // whole sets of loads first, without a branch between a load and what takes its value apart; then one by one
+    auto set = [&](long long p, auto count) {
+        constexpr int N = decltype(count)::value;
+        float f[N][VEC];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (p + u * a.lanes < q.last) vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+        for (int u = 0; u < N; ++u) vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (p + u * a.lanes < q.last) {
+        for (int u = 0; u < N; ++u) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) f[u][e] = gn_act<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
-                vec_store<T, VEC>(y + (p + u * a.lanes) * a.C, f[u]);
-            }
-    }
+            for (int e = 0; e < VEC; ++e) f[u][e] = gn_act<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
+            vec_store<T, VEC>(y + (p + u * a.lanes) * a.C, f[u]);
+        }
+    };
+    long long p = q.first + q.lane;
+    for (; p + (U - 1) * a.lanes < q.last; p += U * a.lanes) set(p, Int<U>());
+    for (; p < q.last; p += a.lanes) set(p, Int<1>());
 }
 
 // Backward sums A, B of a run of pixels
@@ -346,30 +352,31 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const GnArgs a)
     if (q.on) {
         float mean[VEC], scale[VEC], beta[VEC];
         gn_channels<VEC>(a, q, mean, scale, beta);
-        for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
-            float f[U][VEC], d[U][VEC];
+        auto set = [&](long long p, auto count) {
+            constexpr int N = decltype(count)::value;
+            float f[N][VEC], d[N][VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (p + u * a.lanes < q.last) {
-                    vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
-                    vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
-                }
+            for (int u = 0; u < N; ++u) {
+                vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+                vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
+            }
             float ls[VEC], lr[VEC];                                    // these few first: shorter chains of roundings
 #pragma unroll
             for (int e = 0; e < VEC; ++e) ls[e] = lr[e] = 0.f;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (p + u * a.lanes < q.last) {
+            for (int u = 0; u < N; ++u)
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
-                        ls[e] += du;
-                        lr[e] = fmaf(du, f[u][e] - mean[e], lr[e]);
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
+                    ls[e] += du;
+                    lr[e] = fmaf(du, f[u][e] - mean[e], lr[e]);
                 }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) { s[e] += ls[e]; r[e] += lr[e]; }
-        }
+        };
+        long long p = q.first + q.lane;
+        for (; p + (U - 1) * a.lanes < q.last; p += U * a.lanes) set(p, Int<U>());
+        for (; p < q.last; p += a.lanes) set(p, Int<1>());
         const int cpg = a.C / a.G;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) r[e] *= a.rstd[(long long)q.n * a.G + (q.c + e) / cpg];
@@ -564,25 +571,27 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnArgs a
         k1[e] *= rstd;
         k2[e] *= rstd * rstd;
     }
-    for (long long p = q.first + q.lane; p < q.last; p += U * a.lanes) {
-        float f[U][VEC], d[U][VEC];
+    auto set = [&](long long p, auto count) {
+        constexpr int N = decltype(count)::value;
+        float f[N][VEC], d[N][VEC];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (p + u * a.lanes < q.last) {
-                vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
-                vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
+        for (int u = 0; u < N; ++u) {
+            vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
+            vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
+                d[u][e] = fmaf(scale[e], du, -fmaf(f[u][e] - mean[e], k2[e], k1[e]));
             }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (p + u * a.lanes < q.last) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
-                    d[u][e] = fmaf(scale[e], du, -fmaf(f[u][e] - mean[e], k2[e], k1[e]));
-                }
-                vec_store<T, VEC>(dx + (p + u * a.lanes) * a.C, d[u]);
-            }
-    }
+            vec_store<T, VEC>(dx + (p + u * a.lanes) * a.C, d[u]);
+        }
+    };
+    long long p = q.first + q.lane;
+    for (; p + (U - 1) * a.lanes < q.last; p += U * a.lanes) set(p, Int<U>());
+    for (; p < q.last; p += a.lanes) set(p, Int<1>());
 }
 
 // ------------------------------------------------------------------------------------------------ a whole group in registers
