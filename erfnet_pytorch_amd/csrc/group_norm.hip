@@ -46,21 +46,21 @@ struct GnArgs {
     float eps;
 };
 
-// VEC neighbouring channels of one pixel
-template <typename T, int VEC> __device__ __forceinline__ void vec_load(const T* p, float* f) {
-    if constexpr (VEC == 1) f[0] = Elem<T>::ld(p);
+// VEC neighbouring channels of one pixel as they lie in memory, and their values
+template <typename T, int VEC> struct Raw { typedef __attribute__((ext_vector_type(VEC * sizeof(T) / 4))) int type; };
+template <> struct Raw<bf16raw, 1> { typedef bf16raw type; };
+template <> struct Raw<bf16raw, 2> { typedef unsigned type; };
+template <> struct Raw<float, 1> { typedef float type; };
+template <typename T, int VEC> __device__ __forceinline__ typename Raw<T, VEC>::type vec_read(const T* p) { return *(const typename Raw<T, VEC>::type*)p; }
+template <typename T, int VEC> __device__ __forceinline__ void vec_values(const typename Raw<T, VEC>::type& v, float* f) {
+    if constexpr (VEC == 1) f[0] = Elem<T>::to_f32(v);
     else if constexpr (sizeof(T) == 4) {
-        typedef __attribute__((ext_vector_type(VEC))) float V;
-        const V v = *(const V*)p;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = v[e];
+        for (int e = 0; e < VEC; ++e) f[e] = __int_as_float(v[e]);
     } else if constexpr (VEC == 2) {
-        const unsigned r = *(const unsigned*)p;
-        f[0] = __uint_as_float(r << 16);
-        f[1] = __uint_as_float(r & 0xFFFF0000u);
+        f[0] = __uint_as_float(v << 16);
+        f[1] = __uint_as_float(v & 0xFFFF0000u);
     } else {
-        typedef __attribute__((ext_vector_type(VEC / 2))) int V;
-        const V v = *(const V*)p;
 #pragma unroll
         for (int e = 0; e < VEC / 2; ++e) {
             f[2 * e] = __uint_as_float((unsigned)v[e] << 16);
@@ -68,6 +68,7 @@ template <typename T, int VEC> __device__ __forceinline__ void vec_load(const T*
         }
     }
 }
+template <typename T, int VEC> __device__ __forceinline__ void vec_load(const T* p, float* f) { vec_values<T, VEC>(vec_read<T, VEC>(p), f); }
 template <typename T, int VEC> __device__ __forceinline__ void vec_store(T* p, const float* f) {
     if constexpr (VEC == 1) Elem<T>::st(p, f[0]);
     else if constexpr (sizeof(T) == 4) {
@@ -164,7 +165,7 @@ __device__ __forceinline__ void gn_add_lanes(const GnArgs& a, const GnPlace& q, 
     }
 }
 
-// Forward statistics of a run of pixels.  A thread sums UNROLL pixels of a channel, then their squares about their own mean, and joins
+// Forward statistics of a run of pixels.  A thread sums 4 pixels of a channel, then their squares about their own mean, and joins
 // that to what it has: no shift has to be guessed and no large squares cancel.
 template <typename T, int VEC>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnArgs a) {
@@ -175,20 +176,29 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnArgs a) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) mean[e] = m2[e] = 0.f;
     if (q.on) {
+        constexpr int U = 4;
         long long p = q.first + q.lane;
-        for (; p + (GN_UNROLL - 1) * a.lanes < q.last; p += GN_UNROLL * a.lanes) {
-            float f[GN_UNROLL][VEC];
+        typename Raw<T, VEC>::type raw[U];
+        auto whole = [&](long long at) { return at + (U - 1) * a.lanes < q.last; };
+        auto fetch = [&](long long at) {
 #pragma unroll
-            for (int u = 0; u < GN_UNROLL; ++u) vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
-            const float all = n + GN_UNROLL, w = GN_UNROLL / all, nw = n * w;
+            for (int u = 0; u < U; ++u) raw[u] = vec_read<T, VEC>(x + (at + u * a.lanes) * a.C);
+        };
+        if (whole(p)) fetch(p);
+        for (; whole(p); p += U * a.lanes) {
+            float f[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) vec_values<T, VEC>(raw[u], f[u]);
+            if (whole(p + U * a.lanes)) fetch(p + U * a.lanes);        // on its way while this set is worked on
+            const float all = n + U, w = U / all, nw = n * w;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 float s = 0.f, r = 0.f;
 #pragma unroll
-                for (int u = 0; u < GN_UNROLL; ++u) s += f[u][e];
-                s *= 1.f / GN_UNROLL;
+                for (int u = 0; u < U; ++u) s += f[u][e];
+                s *= 1.f / U;
 #pragma unroll
-                for (int u = 0; u < GN_UNROLL; ++u) r = fmaf(f[u][e] - s, f[u][e] - s, r);
+                for (int u = 0; u < U; ++u) r = fmaf(f[u][e] - s, f[u][e] - s, r);
                 const float d = s - mean[e];
                 mean[e] = fmaf(d, w, mean[e]);
                 m2[e] += r + d * d * nw;
@@ -352,31 +362,43 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const GnArgs a)
     if (q.on) {
         float mean[VEC], scale[VEC], beta[VEC];
         gn_channels<VEC>(a, q, mean, scale, beta);
-        auto set = [&](long long p, auto count) {
-            constexpr int N = decltype(count)::value;
-            float f[N][VEC], d[N][VEC];
+        typename Raw<T, VEC>::type rx[U], ry[U];
+        auto whole = [&](long long at) { return at + (U - 1) * a.lanes < q.last; };
+        auto fetch = [&](long long at) {
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
-                vec_load<T, VEC>(x + (p + u * a.lanes) * a.C, f[u]);
-                vec_load<T, VEC>(dy + (p + u * a.lanes) * a.C, d[u]);
+            for (int u = 0; u < U; ++u) {
+                rx[u] = vec_read<T, VEC>(x + (at + u * a.lanes) * a.C);
+                ry[u] = vec_read<T, VEC>(dy + (at + u * a.lanes) * a.C);
             }
-            float ls[VEC], lr[VEC];                                    // these few first: shorter chains of roundings
+        };
+        auto add = [&](const float* f, const float* d, float* ls, float* lr) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float du = d[e] * gn_slope<ACT>(gn_u(f[e], mean[e], scale[e], beta[e]));
+                ls[e] += du;
+                lr[e] = fmaf(du, f[e] - mean[e], lr[e]);
+            }
+        };
+        long long p = q.first + q.lane;
+        if (whole(p)) fetch(p);
+        for (; whole(p); p += U * a.lanes) {
+            float f[U][VEC], d[U][VEC], ls[VEC], lr[VEC];              // these few first: shorter chains of roundings
 #pragma unroll
             for (int e = 0; e < VEC; ++e) ls[e] = lr[e] = 0.f;
 #pragma unroll
-            for (int u = 0; u < N; ++u)
+            for (int u = 0; u < U; ++u) { vec_values<T, VEC>(rx[u], f[u]); vec_values<T, VEC>(ry[u], d[u]); }
+            if (whole(p + U * a.lanes)) fetch(p + U * a.lanes);        // on its way while this set is worked on
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float du = d[u][e] * gn_slope<ACT>(gn_u(f[u][e], mean[e], scale[e], beta[e]));
-                    ls[e] += du;
-                    lr[e] = fmaf(du, f[u][e] - mean[e], lr[e]);
-                }
+            for (int u = 0; u < U; ++u) add(f[u], d[u], ls, lr);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) { s[e] += ls[e]; r[e] += lr[e]; }
-        };
-        long long p = q.first + q.lane;
-        for (; p + (U - 1) * a.lanes < q.last; p += U * a.lanes) set(p, Int<U>());
-        for (; p < q.last; p += a.lanes) set(p, Int<1>());
+        }
+        for (; p < q.last; p += a.lanes) {
+            float f[VEC], d[VEC];
+            vec_load<T, VEC>(x + p * a.C, f);
+            vec_load<T, VEC>(dy + p * a.C, d);
+            add(f, d, s, r);
+        }
         const int cpg = a.C / a.G;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) r[e] *= a.rstd[(long long)q.n * a.G + (q.c + e) / cpg];
