@@ -29,6 +29,14 @@ __device__ __forceinline__ void stat_add(Stat& a, float base, float z) {        
     a.s += e;
     a.t += e * fmaxf(y, -200.f);                                       // 0 * -inf; NaN comes through e
 }
+// The largest of N values, two to an instruction; NaN if one is, which leaves the running maximum as it is: the sums are NaN then
+template <int N, typename VALUE>
+__device__ __forceinline__ float largest(VALUE value) {
+    float m = value(0);
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = __builtin_elementwise_maximum(m, value(i));
+    return m;
+}
 
 // Order of the alternatives as one integer: larger value first, then lower index; NaN before everything, -0 as 0.  No rank
 // is 0 or ~0: these stand for nothing and for a bound above all.
@@ -227,9 +235,7 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
             }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                float most = f[0][p];
-#pragma unroll
-                for (int b = 1; b < BATCH; ++b) most = fmaxf(most, f[b][p]);
+                const float most = largest<BATCH>([&](int b) { return f[b][p]; });
                 if (most > st[p].m) stat_move(st[p], most);
                 const float base = base_of(st[p].m);
 #pragma unroll
@@ -452,11 +458,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) chunk_values<T>(raw[u], f[u]);
-        float most = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e) most = fmaxf(most, f[u][e]);
+        const float most = largest<UNROLL * E>([&](int n) { return f[n / E][n % E]; });
         if (most > st.m) stat_move(st, most);
         const float base = base_of(st.m);
 #pragma unroll
