@@ -40,7 +40,7 @@ __device__ __forceinline__ double ipow(double b, int t) {
     return r;
 }
 
-// The 32-bit mixing function "lowbias32" of C. Wellons' hash prospector (public domain)
+// Mixing of 32 bits by xor-shifts and odd multipliers, these from a published search for the least bias between input and output bits
 __device__ __forceinline__ unsigned mix32(unsigned h) {
     h ^= h >> 16; h *= 0x7FEB352Du;
     h ^= h >> 15; h *= 0x846CA68Bu;

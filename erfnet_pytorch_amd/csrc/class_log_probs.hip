@@ -823,20 +823,23 @@ static inline unsigned lp_grid(long long total) {
     return (unsigned)(g > 65536 ? 65536 : g);
 }
 
-// Positions per thread: 4 where whole vectors lie on their boundaries, enough threads are left to fill the chip and the alternatives
-// leave registers (most_k).  6 x 20 x 512 x 1024, 4 positions against 1: bf16 52 / 75 us forward, 83 / 128 us backward; fp32 alike.
+// Positions per thread: 4 where whole vectors lie on their boundaries, enough threads are left to fill the chip and no alternatives
+// take up registers.  1 / 4 positions, us, forward and backward: 6 x 20 x 512 x 1024 bf16 46 / 41 and 69 / 69, fp32 64 / 65 and 103 / 111,
+// 6 x 5 x 512 x 1024 bf16 22 / 21 and 29 / 25, fp32 26 / 24 and 38 / 37; with 2 alternatives 6 x 20 x 512 x 1024 bf16 66 / 63 and 87 / 96,
+// fp32 80 / 83 and 119 / 126.
 static inline int lp_positions(int dtype, long long N, long long L, long long sc, unsigned long long addresses, unsigned long long strides,
-                               unsigned long long per_position, int k, int most_k) {
+                               unsigned long long per_position, int k) {
     const int size = dtype == ERF_BF16 ? 2 : 4;
-    return sc != 1 && L % 4 == 0 && strides % 4 == 0 && addresses % (4 * size) == 0 && per_position % 16 == 0 && N * L >= (1ll << 19) && k <= most_k ? 4 : 1;
+    return sc != 1 && L % 4 == 0 && strides % 4 == 0 && addresses % (4 * size) == 0 && per_position % 16 == 0 && N * L >= (1ll << 19) && !k ? 4 : 1;
 }
 
 // Rows of more classes than a thread walks through by itself are taken by the smallest team that has the whole row in registers
 // wherever it starts (and lanes for the alternatives), or by a workgroup; few rows of very many classes are split so that about 1024 workgroups have work.
 static inline int lp_epc(int dtype) { return dtype == ERF_BF16 ? 8 : 4; }
-// A thread takes a whole row of up to `alone` classes.  Forward, 1000000 rows of 24 / 40 classes: 51 / 126 us by threads and 47 / 55 us by
-// teams in fp32, 40 / 133 and 69 / 70 us in bf16; backward, 12 / 24 classes: 49 / 146 and 46 / 71 us, 32 / 105 and 74 / 48 us.
-#define ALONE_FWD 24
+// A thread takes a whole row of up to `alone` classes: up to there a wave's rows fill the cache lines that its loads touch.  1000000
+// rows by threads / by teams, us: forward fp32 24 classes 59 / 53, 32 88 / 54, bf16 40 51 / 75, 48 101 / 80; with 2 alternatives fp32 32
+// 90 / 90, 40 129 / 107, bf16 56 99 / 129, 64 162 / 127; backward fp32 12 49 / 51, 16 88 / 57; bf16 12 27 / 68, 16 55 / 48, 24 91 / 48.
+#define ALONE_FWD(dtype, k) ((dtype) == ERF_BF16 ? ((k) ? 56 : 44) : ((k) ? 32 : 24))
 #define ALONE_BWD 12
 static inline int lp_team(int dtype, int C, int k, int alone) {
     if (C <= alone) return 1;
@@ -845,14 +848,14 @@ static inline int lp_team(int dtype, int C, int k, int alone) {
     return 256;
 }
 static inline int lp_segments(int dtype, long long N, int C, int k) {
-    if (lp_team(dtype, C, k, ALONE_FWD) < 256) return 1;
+    if (lp_team(dtype, C, k, ALONE_FWD(dtype, k)) < 256) return 1;
     const long long most = ((long long)C + 256 * UNROLL * lp_epc(dtype) - 1) / (256 * UNROLL * lp_epc(dtype)), want = (1024 + N - 1) / N;
     return (int)(want < most ? want : most);
 }
 
 template <typename T, bool TOP>
 static void lp_rows_launch(const LpArgs& a, int dtype, hipStream_t s) {
-    const int team = lp_team(dtype, a.C, a.k, ALONE_FWD);
+    const int team = lp_team(dtype, a.C, a.k, ALONE_FWD(dtype, a.k));
     const dim3 grid((unsigned)((a.N * team + 255) / 256), (unsigned)a.segments), block(256);
     if (team == 8) hipLaunchKernelGGL((lp_rows_kernel<T, 8, TOP>), grid, block, 0, s, a);
     else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, TOP>), grid, block, 0, s, a);
@@ -889,26 +892,25 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         return ERF_EINVAL;
     LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, (u64*)workspace};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && lp_team(dtype, C, top_k, ALONE_FWD) > 1) {
+    if (stride_c == 1 && lp_team(dtype, C, top_k, ALONE_FWD(dtype, top_k)) > 1) {
         a.segments = lp_segments(dtype, N, C, top_k);
         if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
         else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
     } else {
         const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits, (unsigned long long)(stride_n | stride_c),
-                                   (unsigned long long)log_prob | (unsigned long long)entropy | (unsigned long long)stats |
-                                       (unsigned long long)top_log_probs | (unsigned long long)top_indices, top_k, 4);
+                                   (unsigned long long)log_prob | (unsigned long long)entropy | (unsigned long long)stats, top_k);
         const dim3 grid(lp_grid(N * L / p)), block(256);
-#define LP_KT(T, P)                                                                                          \
-    do {                                                                                                     \
-        if (top_k == 0) hipLaunchKernelGGL((lp_position_kernel<T, P, 0>), grid, block, 0, s, a);             \
-        else if (top_k == 1) hipLaunchKernelGGL((lp_position_kernel<T, P, 1>), grid, block, 0, s, a);        \
-        else if (top_k == 2) hipLaunchKernelGGL((lp_position_kernel<T, P, 2>), grid, block, 0, s, a);        \
-        else if (top_k <= 4) hipLaunchKernelGGL((lp_position_kernel<T, P, 4>), grid, block, 0, s, a);        \
-        else if (top_k <= 8) hipLaunchKernelGGL((lp_position_kernel<T, 1, 8>), grid, block, 0, s, a);        \
-        else hipLaunchKernelGGL((lp_position_kernel<T, 1, -1>), grid, block, 0, s, a);                       \
+#define LP_KT(T)                                                                                            \
+    do {                                                                                                    \
+        if (p == 4) hipLaunchKernelGGL((lp_position_kernel<T, 4, 0>), grid, block, 0, s, a);                \
+        else if (top_k == 0) hipLaunchKernelGGL((lp_position_kernel<T, 1, 0>), grid, block, 0, s, a);       \
+        else if (top_k == 1) hipLaunchKernelGGL((lp_position_kernel<T, 1, 1>), grid, block, 0, s, a);       \
+        else if (top_k == 2) hipLaunchKernelGGL((lp_position_kernel<T, 1, 2>), grid, block, 0, s, a);       \
+        else if (top_k <= 4) hipLaunchKernelGGL((lp_position_kernel<T, 1, 4>), grid, block, 0, s, a);       \
+        else if (top_k <= 8) hipLaunchKernelGGL((lp_position_kernel<T, 1, 8>), grid, block, 0, s, a);       \
+        else hipLaunchKernelGGL((lp_position_kernel<T, 1, -1>), grid, block, 0, s, a);                      \
     } while (0)
-        if (dtype == ERF_BF16) { if (p == 4) LP_KT(bf16raw, 4); else LP_KT(bf16raw, 1); }
-        else { if (p == 4) LP_KT(float, 4); else LP_KT(float, 1); }
+        if (dtype == ERF_BF16) LP_KT(bf16raw); else LP_KT(float);
 #undef LP_KT
     }
     return erf_check_launch();
@@ -931,18 +933,18 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
         const int p = lp_positions(dtype, N, L, stride_c, (unsigned long long)logits | (unsigned long long)dlogits,
                                    (unsigned long long)(stride_n | stride_c | dstride_n | dstride_c),
                                    (unsigned long long)stats | (unsigned long long)entropy | (unsigned long long)g_log_prob |
-                                       (unsigned long long)g_entropy | (unsigned long long)g_top, a.k, 2);
+                                       (unsigned long long)g_entropy, a.k);
         const dim3 grid(lp_grid(N * L / p)), block(256);
-#define LP_KT(T, P)                                                                                          \
-    do {                                                                                                     \
-        if (a.k == 0) hipLaunchKernelGGL((lp_position_bwd_kernel<T, P, 0>), grid, block, 0, s, a);           \
-        else if (a.k <= 2) hipLaunchKernelGGL((lp_position_bwd_kernel<T, P, 2>), grid, block, 0, s, a);      \
-        else if (a.k <= 4) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 4>), grid, block, 0, s, a);      \
-        else if (a.k <= 8) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 8>), grid, block, 0, s, a);      \
-        else hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, -1>), grid, block, 0, s, a);                   \
+#define LP_KT(T)                                                                                            \
+    do {                                                                                                    \
+        if (p == 4) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 4, 0>), grid, block, 0, s, a);            \
+        else if (a.k == 0) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 0>), grid, block, 0, s, a);     \
+        else if (a.k <= 2) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 2>), grid, block, 0, s, a);     \
+        else if (a.k <= 4) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 4>), grid, block, 0, s, a);     \
+        else if (a.k <= 8) hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, 8>), grid, block, 0, s, a);     \
+        else hipLaunchKernelGGL((lp_position_bwd_kernel<T, 1, -1>), grid, block, 0, s, a);                  \
     } while (0)
-        if (dtype == ERF_BF16) { if (p == 4) LP_KT(bf16raw, 4); else LP_KT(bf16raw, 1); }
-        else { if (p == 4) LP_KT(float, 4); else LP_KT(float, 1); }
+        if (dtype == ERF_BF16) LP_KT(bf16raw); else LP_KT(float);
 #undef LP_KT
     }
     return erf_check_launch();

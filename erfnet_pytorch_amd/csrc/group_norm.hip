@@ -807,17 +807,23 @@ template <int VEC> static inline dim3 gn_plan(GnArgs& a, int each, int most) {
 }
 
 // The plan of a group per team: channels per access (the most that divide a group) and the smallest team that has the values in
-// registers and either fills the chip with threads or leaves each thread one access.  Large groups, and those whose narrow accesses
-// leave most of each cache line to other workgroups, are faster by runs of pixels.  Group against runs, forward / backward, in us:
-// 64 x 64 x 1024 in 8 groups (8 channels an access) bf16 9 / 18 against 17 / 24; 64 x 128 x 4096 in 32 groups (4) 73 / 155 against
-// 57 / 95; 64 x 64 x 4096 in 8 groups (8) 25 / 54 against 28 / 47; 3 x 30 x 5673 in 6 groups (1) 15 / 23 against 10 / 10;
-// 64 x 48 x 512 in 16 groups (1) 11 / 16 against 19 / 26; 512 x 128 x 64 in 16 groups (8) 9 / 24 against 65 / 96.
+// registers and either fills the chip with threads or leaves each thread one access.  A group per team saves launches; by runs of
+// pixels the memory is read better, the more so the less of each cache line is one group's.  So a group per team up to so many
+// values of a group, which one workgroup works off alone, and up to so many pieces (a pixel's channels of one group), or for more
+// images than runs are good for.  Group against runs, us, forward at 16 bytes an access: 64 x 4096 x 64 in 8 groups bf16 24 / 28, twice
+// the pixels 43 / 43; 64 x 1024 x 128 in 32 fp32 24 / 23, twice 43 / 38; 3 channels a group: 64 x 1024 x 48 bf16 16 / 20, fp32 19 / 18,
+// twice 26 / 24 and 30 / 22; few large groups: 1 x 2048 x 48 in 16 10 / 16, 3 x 5673 x 30 in 6 15 / 10.  Backward, bf16: 64 x 1024 x 64
+// in 8 19 / 20, twice 36 / 29; 1 x 1024 x 64 in 8 13 / 15, twice 15 / 15; 16 x 2048 x 64 in 16 17 / 18; fp32: 1 x 512 x 64 in 8 11 / 10, 1 x
+// 2048 x 64 in 16 13 / 10, 512 x 64 x 128 in 16 22 / 24; 1024 x 512 x 48 in 16 bf16 123 / 62, 4096 x 128 x 64 in 8 90 / 376.
 static bool gn_group_plan(GnArgs& a, int dtype, unsigned long long addresses, int& vec, bool backward) {
     const int cpg = a.C / a.G;
     vec = gn_vec(dtype, cpg, addresses);
     a.chunks = cpg / vec;
     const long long groups = (long long)a.N * a.G;
-    if (a.HW * cpg > (backward ? 2048 * vec : vec == 8 ? 32768 : vec == 4 ? 8192 : 4096)) return false;
+    const bool bf16 = dtype == ERF_BF16, wide = vec * (bf16 ? 2 : 4) == 16;
+    const long long values = a.HW * cpg, pieces = groups * a.HW;
+    if (backward ? values > (bf16 ? 8192 : 4096) : wide ? a.HW > 4096 : values > 8192) return false;
+    if (pieces > (backward ? 1 << 19 : wide ? 1 << 21 : 1 << 20) && a.N <= 1024) return false;
     for (a.team = 8; a.team <= 1024; a.team = a.team == 8 ? 64 : 4 * a.team) {
         a.lanes = a.team / a.chunks;
         if (a.lanes && a.HW <= (long long)a.lanes * GN_KEEP / vec && (a.team == 1024 || groups * a.team >= (1 << 17) || a.HW <= a.lanes)) return true;
@@ -856,7 +862,7 @@ static void gn_group_bwd_launch(GnArgs a, hipStream_t s) {
 }
 
 // Whether the apply kernels join the runs: that costs each of their workgroups a look at all runs of its image, and saves a launch
-// (3 x 30 x 5673 forward / backward 10.2 / 10.4 us against 11.4 / 13.3; 6 x 128 x 8192 and larger maps alike)
+// (3 x 5673 x 30 forward / backward 10 / 10 us against 11 / 13, 2 x 100000 x 16 18 / 22 against 19 / 24; 6 x 8192 x 128 and larger alike)
 static inline bool gn_join_in_apply(const GnArgs& a, dim3 grid) {
     return grid.y == 1 && a.C <= GN_JOIN_CHANNELS && a.C / a.G <= 128 && (long long)a.P * a.C <= 8192;
 }
