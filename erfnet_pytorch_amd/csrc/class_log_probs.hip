@@ -106,6 +106,7 @@ struct LpArgs {
     float *log_prob, *entropy, *stats, *top;
     long long* top_index;
     int segments;                      // rows: workgroups per row
+    long long first;                   // rows: the launch's first one
     u64* parts;                        // [N][segments][2 + k]: (m, s), (t, -), the segment's best ranks
 };
 
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     constexpr int E = Elem<T>::EPC;
     __shared__ TeamShared<TOP || TEAM == 256 ? TEAM : 8> shared[TOP || TEAM == 256 ? 256 / TEAM : 1];
     const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
-    const long long i = (long long)blockIdx.x * (256 / TEAM) + team;
+    const long long i = a.first + (long long)blockIdx.x * (256 / TEAM) + team;
     if (TEAM < 256 && i >= a.N) return;                                // no barrier of the workgroup below for teams within a wave
     auto& sh = shared[TOP ? team : 0];
     const T* row = (const T*)a.z + i * a.sn;
@@ -639,6 +640,7 @@ struct LpBwdArgs {
     const float *stats, *entropy, *g_log_prob, *g_entropy, *g_top;
     const long long* top_index;
     void* dz;
+    long long first;                   // rows: the launch's first one
 };
 
 // dz_j = -p_j (pull + gh log p_j) for every class, pull = gl + sum gk + gh H; the target and the alternatives get their own terms
@@ -756,7 +758,7 @@ template <typename T, int TEAM>
 __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     constexpr int E = Elem<T>::EPC;
     const int tid = threadIdx.x % TEAM;
-    const long long i = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    const long long i = a.first + (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
     if (TEAM < 256 && i >= a.N) return;                                // no barrier of the workgroup below for teams within a wave
     const T* row = (const T*)a.z + i * a.sn;
     T* out = (T*)a.dz + i * a.dn;
@@ -853,26 +855,35 @@ static inline int lp_segments(int dtype, long long N, int C, int k) {
     return (int)(want < most ? want : most);
 }
 
+// A launch has less than 2^32 threads: very many rows are several launches' work
+#define ROWS_PER_LAUNCH(team) ((1ll << 30) / (team))
+
 template <typename T, bool TOP>
-static void lp_rows_launch(const LpArgs& a, int dtype, hipStream_t s) {
+static void lp_rows_launch(LpArgs a, int dtype, hipStream_t s) {
     const int team = lp_team(dtype, a.C, a.k, ALONE_FWD(dtype, a.k));
-    const dim3 grid((unsigned)((a.N * team + 255) / 256), (unsigned)a.segments), block(256);
-    if (team == 8) hipLaunchKernelGGL((lp_rows_kernel<T, 8, TOP>), grid, block, 0, s, a);
-    else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, TOP>), grid, block, 0, s, a);
-    else if (team == 64) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), grid, block, 0, s, a);
+    for (a.first = 0; a.first < a.N; a.first += ROWS_PER_LAUNCH(team)) {
+        const long long rows = a.N - a.first < ROWS_PER_LAUNCH(team) ? a.N - a.first : ROWS_PER_LAUNCH(team);
+        const dim3 grid((unsigned)((rows * team + 255) / 256), (unsigned)a.segments), block(256);
+        if (team == 8) hipLaunchKernelGGL((lp_rows_kernel<T, 8, TOP>), grid, block, 0, s, a);
+        else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, TOP>), grid, block, 0, s, a);
+        else if (team == 64) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), grid, block, 0, s, a);
+    }
     if (a.segments > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)a.N), dim3(256), 0, s, a);
 }
 
 template <typename T>
-static void lp_rows_bwd_launch(const LpBwdArgs& a, int dtype, hipStream_t s) {
+static void lp_rows_bwd_launch(LpBwdArgs a, int dtype, hipStream_t s) {
     const int team = lp_team(dtype, a.C, 0, ALONE_BWD), per = 256 * BWD_UNROLL;
     const int chunks = (a.C + 2 * (lp_epc(dtype) - 1)) / lp_epc(dtype);              // of a row that starts just before a boundary
-    const dim3 grid((unsigned)((a.N * team + 255) / 256), team < 256 ? 1u : (unsigned)((chunks + per - 1) / per)), block(256);
-    if (team == 8) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 8>), grid, block, 0, s, a);
-    else if (team == 16) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 16>), grid, block, 0, s, a);
-    else if (team == 64) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 64>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 256>), grid, block, 0, s, a);
+    for (a.first = 0; a.first < a.N; a.first += ROWS_PER_LAUNCH(team)) {
+        const long long rows = a.N - a.first < ROWS_PER_LAUNCH(team) ? a.N - a.first : ROWS_PER_LAUNCH(team);
+        const dim3 grid((unsigned)((rows * team + 255) / 256), team < 256 ? 1u : (unsigned)((chunks + per - 1) / per)), block(256);
+        if (team == 8) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 8>), grid, block, 0, s, a);
+        else if (team == 16) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 16>), grid, block, 0, s, a);
+        else if (team == 64) hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 64>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((lp_rows_bwd_kernel<T, 256>), grid, block, 0, s, a);
+    }
 }
 
 extern "C" {
@@ -890,7 +901,7 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         (top_k && (!top_log_probs || !top_indices)) ||
         (!workspace && erf_class_log_probs_workspace_bytes(dtype, N, C, L, stride_c, top_k)))
         return ERF_EINVAL;
-    LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, (u64*)workspace};
+    LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, 0, (u64*)workspace};
     hipStream_t s = (hipStream_t)stream;
     if (stride_c == 1 && lp_team(dtype, C, top_k, ALONE_FWD(dtype, top_k)) > 1) {
         a.segments = lp_segments(dtype, N, C, top_k);
@@ -924,7 +935,7 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
         (g_top && (!top_indices || !top_k)) || dstride_n < 0 || (dstride_c == 1) != (stride_c == 1) || (dstride_c != 1 && dstride_c < L))
         return ERF_EINVAL;
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
-                      g_log_prob, g_entropy, g_top, top_indices, dlogits};
+                      g_log_prob, g_entropy, g_top, top_indices, dlogits, 0};
     hipStream_t s = (hipStream_t)stream;
     if (stride_c == 1 && lp_team(dtype, C, 0, ALONE_BWD) > 1) {
         if (dtype == ERF_BF16) lp_rows_bwd_launch<bf16raw>(a, dtype, s);

@@ -229,22 +229,25 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnArgs a) {
 // One workgroup per (image, group): the group's channels and runs of pixels joined to its mean and 1 / sqrt(var + eps)
 __global__ __launch_bounds__(1024) void gn_finalize_kernel(const GnArgs a) {
     __shared__ float sh[3][16];
-    const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
-    const long long per = (a.HW + a.runs - 1) / a.runs;
-    float mean = 0.f, m2 = 0.f, count = 0.f;
-    for (long long i = threadIdx.x; i < (long long)a.runs * cpg; i += 1024) {
-        const long long p = i / cpg, c = g * cpg + (i - p * cpg), left = a.HW - p * per;
-        const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.runs + p) * a.C + c));
-        gn_join(mean, m2, count, v.x, v.y, left <= 0 ? 0.f : (float)(left < per ? left : per));
-    }
+    for (long long at = blockIdx.x; at < (long long)a.N * a.G; at += gridDim.x) {
+        const int n = (unsigned)at / (unsigned)a.G, g = (unsigned)at % (unsigned)a.G, cpg = a.C / a.G;
+        const long long per = (a.HW + a.runs - 1) / a.runs;
+        float mean = 0.f, m2 = 0.f, count = 0.f;
+        for (long long i = threadIdx.x; i < (long long)a.runs * cpg; i += 1024) {
+            const long long p = i / cpg, c = g * cpg + (i - p * cpg), left = a.HW - p * per;
+            const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.runs + p) * a.C + c));
+            gn_join(mean, m2, count, v.x, v.y, left <= 0 ? 0.f : (float)(left < per ? left : per));
+        }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) gn_join(mean, m2, count, __shfl_xor(mean, o, 64), __shfl_xor(m2, o, 64), __shfl_xor(count, o, 64));
-    if ((threadIdx.x & 63) == 0) { sh[0][threadIdx.x >> 6] = mean; sh[1][threadIdx.x >> 6] = m2; sh[2][threadIdx.x >> 6] = count; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) gn_join(mean, m2, count, sh[0][w], sh[1][w], sh[2][w]);
-        a.mean[blockIdx.x] = mean;
-        a.rstd[blockIdx.x] = 1.f / sqrtf(m2 / ((float)a.HW * cpg) + a.eps);
+        for (int o = 32; o > 0; o >>= 1) gn_join(mean, m2, count, __shfl_xor(mean, o, 64), __shfl_xor(m2, o, 64), __shfl_xor(count, o, 64));
+        if ((threadIdx.x & 63) == 0) { sh[0][threadIdx.x >> 6] = mean; sh[1][threadIdx.x >> 6] = m2; sh[2][threadIdx.x >> 6] = count; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 16; ++w) gn_join(mean, m2, count, sh[0][w], sh[1][w], sh[2][w]);
+            a.mean[at] = mean;
+            a.rstd[at] = 1.f / sqrtf(m2 / ((float)a.HW * cpg) + a.eps);
+        }
+        __syncthreads();                                               // the next group's values come to the same place
     }
 }
 
@@ -415,47 +418,50 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_sums_kernel(const GnArgs a)
 // (run lane, channel) with the channels side by side in memory; 1024 channels at a time.
 __global__ __launch_bounds__(1024) void gn_bwd_finalize_kernel(const GnArgs a) {
     __shared__ double sh[2][1024];
-    const int n = blockIdx.x / a.G, g = blockIdx.x % a.G, cpg = a.C / a.G;
-    const int side = cpg < 1024 ? cpg : 1024, lanes = 1024 / side, lane = threadIdx.x / side, j = threadIdx.x - lane * side;
-    double s1 = 0, s2 = 0;
-    for (int c0 = 0; c0 < cpg; c0 += side) {
-        const int c = g * cpg + c0 + j;
-        const bool on = lane < lanes && c0 + j < cpg;
-        double p = 0, r = 0;
-        if (on)
-            for (int i = lane; i < a.runs; i += lanes) {
-                const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.runs + i) * a.C + c));
-                p += v.x;
-                r += v.y;
+    for (long long at = blockIdx.x; at < (long long)a.N * a.G; at += gridDim.x) {
+        const int n = (unsigned)at / (unsigned)a.G, g = (unsigned)at % (unsigned)a.G, cpg = a.C / a.G;
+        const int side = cpg < 1024 ? cpg : 1024, lanes = 1024 / side, lane = threadIdx.x / side, j = threadIdx.x - lane * side;
+        double s1 = 0, s2 = 0;
+        for (int c0 = 0; c0 < cpg; c0 += side) {
+            const int c = g * cpg + c0 + j;
+            const bool on = lane < lanes && c0 + j < cpg;
+            double p = 0, r = 0;
+            if (on)
+                for (int i = lane; i < a.runs; i += lanes) {
+                    const float2 v = *(const float2*)(a.parts + 2 * (((long long)n * a.runs + i) * a.C + c));
+                    p += v.x;
+                    r += v.y;
+                }
+            for (int have = lanes; have > 1;) {
+                const int keep = (have + 1) / 2;
+                __syncthreads();
+                if (lane >= keep && lane < have) { sh[0][threadIdx.x] = p; sh[1][threadIdx.x] = r; }
+                __syncthreads();
+                if (lane + keep < have) { p += sh[0][threadIdx.x + keep * side]; r += sh[1][threadIdx.x + keep * side]; }
+                have = keep;
             }
-        for (int have = lanes; have > 1;) {
-            const int keep = (have + 1) / 2;
-            __syncthreads();
-            if (lane >= keep && lane < have) { sh[0][threadIdx.x] = p; sh[1][threadIdx.x] = r; }
-            __syncthreads();
-            if (lane + keep < have) { p += sh[0][threadIdx.x + keep * side]; r += sh[1][threadIdx.x + keep * side]; }
-            have = keep;
+            if (on && lane == 0) {
+                a.sums[2 * ((long long)n * a.C + c)] = (float)p;
+                a.sums[2 * ((long long)n * a.C + c) + 1] = (float)r;
+                const double gamma = a.gamma ? a.gamma[c] : 1.f;
+                s1 += gamma * p;
+                s2 += gamma * r;
+            }
         }
-        if (on && lane == 0) {
-            a.sums[2 * ((long long)n * a.C + c)] = (float)p;
-            a.sums[2 * ((long long)n * a.C + c) + 1] = (float)r;
-            const double gamma = a.gamma ? a.gamma[c] : 1.f;
-            s1 += gamma * p;
-            s2 += gamma * r;
-        }
-    }
-    __syncthreads();
-    sh[0][threadIdx.x] = s1;
-    sh[1][threadIdx.x] = s2;
-    for (int o = 512; o > 0; o >>= 1) {
         __syncthreads();
-        if ((int)threadIdx.x < o) { sh[0][threadIdx.x] += sh[0][threadIdx.x + o]; sh[1][threadIdx.x] += sh[1][threadIdx.x + o]; }
-    }
-    if (threadIdx.x == 0) {
-        const double m = (double)a.HW * cpg;
-        float* out = a.sums + 2 * (long long)a.N * a.C + 2 * (long long)blockIdx.x;
-        out[0] = (float)(sh[0][0] / m);
-        out[1] = (float)(sh[1][0] / m);
+        sh[0][threadIdx.x] = s1;
+        sh[1][threadIdx.x] = s2;
+        for (int o = 512; o > 0; o >>= 1) {
+            __syncthreads();
+            if ((int)threadIdx.x < o) { sh[0][threadIdx.x] += sh[0][threadIdx.x + o]; sh[1][threadIdx.x] += sh[1][threadIdx.x + o]; }
+        }
+        if (threadIdx.x == 0) {
+            const double m = (double)a.HW * cpg;
+            float* out = a.sums + 2 * (long long)a.N * a.C + 2 * at;
+            out[0] = (float)(sh[0][0] / m);
+            out[1] = (float)(sh[1][0] / m);
+        }
+        __syncthreads();                                               // the next group's values come to the same place
     }
 }
 
@@ -667,14 +673,15 @@ __global__ __launch_bounds__(1024) void gn_group_fwd_kernel(const GnArgs a) {
     __shared__ float sh[16];
     const GnGroup q = gn_group<VEC>(a);
     const T* x = (const T*)a.x + q.at;
+    typename Raw<T, VEC>::type raw[R];                                 // taken apart after all loads are on their way
     float f[R][VEC];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-        if (q.on && q.lane + r * a.lanes < a.HW) vec_load<T, VEC>(x + (long long)r * a.lanes * a.C, f[r]);
-        else {
+    for (int r = 0; r < R; ++r) {
+        raw[r] = typename Raw<T, VEC>::type{};
+        if (q.on && q.lane + r * a.lanes < a.HW) raw[r] = vec_read<T, VEC>(x + (long long)r * a.lanes * a.C);
+    }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[r][e] = 0.f;
-        }
+    for (int r = 0; r < R; ++r) vec_values<T, VEC>(raw[r], f[r]);
     float s = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -716,13 +723,16 @@ __global__ __launch_bounds__(1024) void gn_group_bwd_kernel(const GnArgs a) {
     const GnGroup q = gn_group<VEC>(a);
     const T *x = (const T*)a.x + q.at, *dy = (const T*)a.dy + q.at;
     const float mean = q.on ? a.mean[(long long)q.n * a.G + q.g] : 0.f, rstd = q.on ? a.rstd[(long long)q.n * a.G + q.g] : 0.f;
+    typename Raw<T, VEC>::type fraw[R], draw[R];
     float f[R][VEC], d[R][VEC], gamma[VEC], beta[VEC], p[VEC], s[VEC];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+        fraw[r] = draw[r] = typename Raw<T, VEC>::type{};
         if (q.on && q.lane + r * a.lanes < a.HW) {
-            vec_load<T, VEC>(x + (long long)r * a.lanes * a.C, f[r]);
-            vec_load<T, VEC>(dy + (long long)r * a.lanes * a.C, d[r]);
+            fraw[r] = vec_read<T, VEC>(x + (long long)r * a.lanes * a.C);
+            draw[r] = vec_read<T, VEC>(dy + (long long)r * a.lanes * a.C);
         }
+    }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         gamma[e] = q.on && a.gamma ? a.gamma[q.c + e] : 1.f;
@@ -730,7 +740,9 @@ __global__ __launch_bounds__(1024) void gn_group_bwd_kernel(const GnArgs a) {
         p[e] = s[e] = 0.f;
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+        vec_values<T, VEC>(fraw[r], f[r]);
+        vec_values<T, VEC>(draw[r], d[r]);
         if (q.on && q.lane + r * a.lanes < a.HW) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
@@ -740,6 +752,7 @@ __global__ __launch_bounds__(1024) void gn_group_bwd_kernel(const GnArgs a) {
                 s[e] = fmaf(d[r][e], f[r][e], s[e]);
             }
         }
+    }
     for (int have = a.lanes; have > 1;) {
         const int keep = (have + 1) / 2;
         gn_sync(a.team);
@@ -781,7 +794,7 @@ __global__ __launch_bounds__(1024) void gn_group_bwd_kernel(const GnArgs a) {
 }
 
 static inline bool gn_shape_ok(int dtype, int N, long long HW, int C, int groups, int act) {
-    return (dtype == ERF_F32 || dtype == ERF_BF16) && N > 0 && N <= (1 << 24) && HW > 0 && C > 0 && groups > 0 && C % groups == 0 && act >= 0 &&
+    return (dtype == ERF_F32 || dtype == ERF_BF16) && N > 0 && N <= (1 << 23) && HW > 0 && C > 0 && groups > 0 && C % groups == 0 && act >= 0 &&
            act <= 2 && (long long)N * groups <= 0x7FFFFFFFll && C <= (1 << 20) && HW <= (1ll << 40) / C;
 }
 
@@ -809,8 +822,8 @@ template <int VEC> static inline dim3 gn_plan(GnArgs& a, int each, int most) {
 // The plan of a group per team: channels per access (the most that divide a group) and the smallest team that has the values in
 // registers and either fills the chip with threads or leaves each thread one access.  A group per team saves launches; by runs of
 // pixels the memory is read better, the more so the less of each cache line is one group's.  So a group per team up to so many
-// values of a group, which one workgroup works off alone, and up to so many pieces (a pixel's channels of one group), or for more
-// images than runs are good for.  Group against runs, us, forward at 16 bytes an access: 64 x 4096 x 64 in 8 groups bf16 24 / 28, twice
+// values of a group, which one workgroup works off alone, and up to so many pieces (a pixel's channels of one group); in all
+// sizes of small groups, and for more images than runs are good for.  Group against runs, us, forward at 16 bytes an access: 64 x 4096 x 64 in 8 groups bf16 24 / 28, twice
 // the pixels 43 / 43; 64 x 1024 x 128 in 32 fp32 24 / 23, twice 43 / 38; 3 channels a group: 64 x 1024 x 48 bf16 16 / 20, fp32 19 / 18,
 // twice 26 / 24 and 30 / 22; few large groups: 1 x 2048 x 48 in 16 10 / 16, 3 x 5673 x 30 in 6 15 / 10.  Backward, bf16: 64 x 1024 x 64
 // in 8 19 / 20, twice 36 / 29; 1 x 1024 x 64 in 8 13 / 15, twice 15 / 15; 16 x 2048 x 64 in 16 17 / 18; fp32: 1 x 512 x 64 in 8 11 / 10, 1 x
@@ -823,10 +836,10 @@ static bool gn_group_plan(GnArgs& a, int dtype, unsigned long long addresses, in
     const bool bf16 = dtype == ERF_BF16, wide = vec * (bf16 ? 2 : 4) == 16;
     const long long values = a.HW * cpg, pieces = groups * a.HW;
     if (backward ? values > (bf16 ? 8192 : 4096) : wide ? a.HW > 4096 : values > 8192) return false;
-    if (pieces > (backward ? 1 << 19 : wide ? 1 << 21 : 1 << 20) && a.N <= 1024) return false;
+    if (pieces > (backward ? 1 << 19 : wide ? 1 << 21 : 1 << 20) && a.N <= 1024 && values > 512) return false;
     for (a.team = 8; a.team <= 1024; a.team = a.team == 8 ? 64 : 4 * a.team) {
         a.lanes = a.team / a.chunks;
-        if (a.lanes && a.HW <= (long long)a.lanes * GN_KEEP / vec && (a.team == 1024 || groups * a.team >= (1 << 17) || a.HW <= a.lanes)) return true;
+        if (a.lanes && a.HW <= (long long)a.lanes * GN_KEEP / vec && groups * a.team < 1ll << 31 && (a.team == 1024 || groups * a.team >= (1 << 17) || a.HW <= a.lanes)) return true;
     }
     return false;
 }
@@ -867,13 +880,19 @@ static inline bool gn_join_in_apply(const GnArgs& a, dim3 grid) {
     return grid.y == 1 && a.C <= GN_JOIN_CHANNELS && a.C / a.G <= 128 && (long long)a.P * a.C <= 8192;
 }
 
+// A launch has less than 2^32 threads: the workgroups take several groups each where there are very many
+static inline dim3 gn_finalize_grid(const GnArgs& a) {
+    const long long groups = (long long)a.N * a.G;
+    return dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20));
+}
+
 template <typename T, int VEC, int ACT>
 static void gn_fwd_launch(GnArgs a, hipStream_t s) {
     dim3 grid = gn_plan<VEC>(a, GN_UNROLL, GN_MAX_RUNS);
     hipLaunchKernelGGL((gn_stats_kernel<T, VEC>), grid, dim3(GN_THREADS), 0, s, a);
     const bool join = gn_join_in_apply(a, grid);
     a.runs = a.P;
-    if (!join) hipLaunchKernelGGL(gn_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
+    if (!join) hipLaunchKernelGGL(gn_finalize_kernel, gn_finalize_grid(a), dim3(1024), 0, s, a);
     grid = gn_plan<VEC>(a, 4, 1 << 20);
     if (join) hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT, false>), grid, dim3(GN_THREADS), 0, s, a);
     else hipLaunchKernelGGL((gn_apply_kernel<T, VEC, ACT, true>), grid, dim3(GN_THREADS), 0, s, a);
@@ -886,7 +905,7 @@ static void gn_bwd_launch(GnArgs a, hipStream_t s) {
     a.runs = a.P;
     // the parameter gradients come from the runs as they are where these are few, else from the images' sums
     const bool params = a.dgamma || a.dbeta, join = gn_join_in_apply(a, grid) && (!params || (long long)a.N * a.runs <= 1024);
-    if (!join) hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, a);
+    if (!join) hipLaunchKernelGGL(gn_bwd_finalize_kernel, gn_finalize_grid(a), dim3(1024), 0, s, a);
     grid = gn_plan<VEC>(a, 4, 1 << 20);
     const bool few = params && (join || gn_image_runs(a.N) == 1);
     a.rows = join ? a.N * a.runs : a.N;

@@ -131,6 +131,14 @@ class AdamW(torch.optim.Optimizer):
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
+        for group in state_dict["param_groups"]:        # before anything is taken over
+            lacking = [k for k in self.defaults if k not in group]
+            if lacking:
+                raise ValueError(f"AdamW: a saved group lacks {', '.join(lacking)}")
+            for k, plain in (("amsgrad", False), ("maximize", False), ("decoupled_weight_decay", True)):
+                if group.get(k, plain) != plain and (k != "decoupled_weight_decay" or group["weight_decay"]):
+                    raise ValueError(f"AdamW: a saved group has {k}={group[k]}, which this optimizer does not compute")
+            self._check_group({**group, "params": []})
         # torch's loader casts every state tensor to the parameter's type: the values are put in place again as they were saved
         self._write_back_steps()
         super().load_state_dict(state_dict)
@@ -145,8 +153,6 @@ class AdamW(torch.optim.Optimizer):
                         torch.empty(v.shape, dtype=v.dtype, device=p.device)
                     _raw(here).copy_(_raw(v))
                     self.state[p][k] = here
-        for group in self.param_groups:
-            self._check_group(group)
         if self._plans is not None:
             self._kept += [plan for plans in self._plans for plan in plans if plan.captured]
         self._plans = None                              # the loaded step counts stand

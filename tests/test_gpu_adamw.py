@@ -41,6 +41,24 @@ def test_constructor_refuses_what_it_cannot_do():
     assert len(opt.param_groups) == 1
 
 
+def test_saved_settings_that_it_does_not_compute_are_refused_before_anything_is_loaded():
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = _adamw([p], lr=1e-2)
+    for other in (torch.optim.AdamW([p], amsgrad=True), torch.optim.AdamW([p], maximize=True), torch.optim.Adam([p], weight_decay=0.1),
+                  torch.optim.SGD([p], lr=0.1)):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 1e-2
+    bad = opt.state_dict()
+    bad["param_groups"][0] = {**bad["param_groups"][0], "betas": (0.9, 1.0), "lr": 5.0}
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
+    assert opt.param_groups[0]["lr"] == 1e-2
+    for other in (torch.optim.AdamW([p], lr=0.5), torch.optim.Adam([p], lr=0.25)):              # Adam without weight decay is the same
+        opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == other.param_groups[0]["lr"]
+
+
 def test_cpu_parameters_are_refused_at_the_step_and_no_gradient_is_no_step():
     p = torch.nn.Parameter(torch.zeros(4))
     opt = _adamw([p])

@@ -277,6 +277,28 @@ def test_without_target_and_partial_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("classes,k,rows", [(60, 0, 2 ** 27 + 500), (600, 2, 2 ** 24 + 500), (2500, 1, 2 ** 22 + 500)])
+def test_more_rows_than_one_launch_takes(classes, k, rows):
+    """Rows that overlap in memory (the next one starts a class later), by teams of 8 and 64 and by workgroups: around the seams of the
+    launches the bits of a call on those rows alone."""
+    from erfnet_pytorch_amd import train_ops as TO
+    buf = torch.randn(rows + classes, device="cuda").to(torch.bfloat16)
+    z, t = buf.as_strided((rows, classes), (1, 1)), torch.randint(0, classes, (rows,), device="cuda")
+    lp, ent, stats, top, idx = TO.class_log_probs_fwd(z, t, k, -100)
+    seam = rows - 500
+    here = slice(seam - 40, seam + 40)
+    part = TO.class_log_probs_fwd(z[here], t[here], k, -100)
+    for whole, alone in ((lp[here], part[0]), (ent[here], part[1]), (stats[:, here], part[2]), (top[here], part[3]), (idx[here], part[4])):
+        assert torch.equal(whole, alone)
+    assert not torch.isnan(lp).any() and float(lp.max()) <= 0
+    if classes > 60:                                        # (of a gradient of 16 GB a sample is enough)
+        return
+    g = torch.randn(rows, device="cuda")
+    dz = TO.class_log_probs_bwd(z, t, stats, ent, idx, g, None, None, -100)
+    assert torch.equal(dz[here], TO.class_log_probs_bwd(z[here], t[here], part[2], part[1], part[4], g[here], None, None, -100))
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     from erfnet_pytorch_amd.loss import class_log_probs
     z = _logits((3, 30), torch.float32, "plain", 17).requires_grad_()

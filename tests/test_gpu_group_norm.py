@@ -241,6 +241,24 @@ def test_captured_calls_and_another_stream(shape, groups):
 
 
 @pytest.mark.gpu
+def test_more_groups_than_one_launch_has_workgroups():
+    """1.06 million groups: whole images from both sides of the 2^20th group against the formula."""
+    from erfnet_pytorch_amd import train_ops as TO
+    n, p, c = 1024, 600, 1040
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, dy = (torch.randn(n, p, c, generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    w, b = (torch.randn(c, generator=gen, device="cuda") for _ in range(2))
+    y, stats = TO.group_norm_act_fwd(x, w, b, c, 1e-5, "silu")
+    dx = TO.group_norm_act_bwd(dy, x, w, b, stats, c, "silu")[0]
+    for i in (0, 2 ** 20 // c, 2 ** 20 // c + 1, n - 1):
+        xd, wd, bd, dyd = x[i:i + 1].cpu().double().requires_grad_(), w.cpu().double(), b.cpu().double(), dy[i:i + 1].cpu().double()
+        yd = _ref(xd, wd, bd, c, 1e-5, "silu")
+        tol = _tolerances(xd.detach(), wd, bd, dyd, c, 1e-5, "silu", torch.bfloat16)
+        assert ((y[i:i + 1].cpu().double() - yd.detach()).abs() <= tol[0]).all()
+        assert ((dx[i:i + 1].cpu().double() - torch.autograd.grad(yd, xd, dyd)[0]).abs() <= tol[1]).all()
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     from erfnet_pytorch_amd.norm import group_norm_act
     x, w, b, dy = _inputs((1, 8, 4, 4), torch.float32, 12)
