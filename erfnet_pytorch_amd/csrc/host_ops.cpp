@@ -24,7 +24,17 @@ static int dtype_code(const Tensor& t, const char* who) {
     TORCH_CHECK_TYPE(false, who, ": float32 or bfloat16 tensors, got ", t.dtype());
 }
 
-static bool shape_only(const Tensor& t) { return t.is_meta() || t.key_set().has(c10::DispatchKey::Python); }
+// Whether there is no memory behind a tensor: meta and fake ones.  Other tensors that dispatch to Python have memory of their own
+// making, which the kernels do not see: refused.
+static bool shape_only(const Tensor& t) {
+    if (t.is_meta()) return true;
+    if (!t.key_set().has(c10::DispatchKey::Python)) return false;
+    py::gil_scoped_acquire gil;
+    const py::object o = py::reinterpret_steal<py::object>(THPVariable_Wrap(t));
+    const bool fake = py::isinstance(o, py::module_::import("torch._subclasses.fake_tensor").attr("FakeTensor"));
+    TORCH_CHECK_TYPE(fake, "erfnet_pytorch_amd's operators take plain tensors, got ", std::string(py::str(py::type::of(o))));
+    return true;
+}
 
 static void require_gpu(const Tensor& t, const char* who) {
     TORCH_CHECK(t.is_cuda(), who, ": erfnet_pytorch_amd runs on MI355X (gfx950) device tensors only; got a CPU tensor and there is no CPU path in this package");
@@ -59,7 +69,9 @@ static int64_t activation_code(const std::string& a) {
 static Tensor channels_last(const Tensor& x) {
     Tensor last = x.dim() > 2 ? x.movedim(1, -1) : x;
     if (last.is_contiguous()) return last;
-    if (x.dim() == 4 && x.is_contiguous() && x.numel() && x.is_cuda() && !shape_only(x)) {
+    auto tiles = [](int64_t n) { return (n + 31) / 32; };
+    if (x.dim() == 4 && x.is_contiguous() && x.numel() && x.is_cuda() && !shape_only(x) &&
+        x.size(0) * tiles(x.size(1)) * tiles(x.size(2) * x.size(3)) < (1 << 24)) {              // what one launch takes
         const int code = dtype_code(x, "group_norm_act");
         Tensor out = at::empty({x.size(0), x.size(2), x.size(3), x.size(1)}, x.options());
         c10::DeviceGuard guard(x.device());
@@ -70,6 +82,18 @@ static Tensor channels_last(const Tensor& x) {
     return last.contiguous();
 }
 static Tensor channels_first(const Tensor& y) { return y.dim() > 2 ? y.movedim(-1, 1) : y; }
+// [N, C, ...] in channels-last memory.  No view: a view made inside an autograd node may not be written in place.
+static Tensor empty_channels_last(at::IntArrayRef sizes, const at::TensorOptions& options) {
+    std::vector<int64_t> strides(sizes.size());
+    int64_t step = sizes[1];
+    for (size_t d = sizes.size() - 1; d >= 2; --d) {
+        strides[d] = step;
+        step *= std::max<int64_t>(sizes[d], 1);
+    }
+    strides[0] = std::max<int64_t>(step, 1);
+    strides[1] = 1;
+    return at::empty_strided(sizes, strides, options);
+}
 
 static Tensor fp32(const OptTensor& t) { return t ? t->to(at::kFloat).contiguous() : Tensor(); }
 
@@ -81,6 +105,7 @@ static GnShape gn_check(const Tensor& x, const OptTensor& weight, const OptTenso
     TORCH_CHECK_VALUE(x.dim() >= 2 && x.is_contiguous(), who, ": a contiguous channels-last tensor [N, ..., C], got shape ", x.sizes(), " strides ", x.strides());
     const int64_t c = x.size(-1), n = x.size(0);
     TORCH_CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0, who, ": ", c, " channels do not split into ", groups, " groups");
+    TORCH_CHECK_VALUE(n <= INT_MAX && c <= INT_MAX, who, ": shape ", x.sizes(), " is too large");
     for (const auto& [t, name] : {std::make_pair(&weight, "weight"), std::make_pair(&bias, "bias")})
         if (*t) {
             TORCH_CHECK_VALUE((*t)->dim() == 1 && (*t)->size(0) == c, who, ": ", name, " has shape [", c, "], got ", (*t)->sizes());
@@ -97,11 +122,13 @@ static Tensor gn_workspace(const Tensor& x, const GnShape& s, int64_t groups) {
     return at::empty({(int64_t)erf_group_norm_workspace_bytes(s.code, s.n, s.hw, s.c, (int)groups)}, x.options().dtype(at::kByte));
 }
 
-// (y, stats [2, N, groups]) of a contiguous channels-last x
-static std::tuple<Tensor, Tensor> group_norm_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps, int64_t act) {
+// (y, stats [2, N, groups]) of a contiguous channels-last x; y [N, ..., C], or as `first` [N, C, ...] in the same memory
+static std::tuple<Tensor, Tensor> group_norm_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps, int64_t act,
+                                                 bool first) {
     const GnShape s = gn_check(x, weight, bias, groups);
     TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "group_norm_act: invalid eps ", eps);
-    Tensor y = at::empty(x.sizes(), x.options()), stats = at::empty({2, s.n, groups}, x.options().dtype(at::kFloat));
+    Tensor y = first && x.dim() > 2 ? empty_channels_last(x.movedim(-1, 1).sizes(), x.options()) : at::empty(x.sizes(), x.options());
+    Tensor stats = at::empty({2, s.n, groups}, x.options().dtype(at::kFloat));
     if (x.numel() && !shape_only(x)) {
         require_gpu(x, "group_norm_act");
         const Tensor w = fp32(weight), b = fp32(bias);
@@ -146,11 +173,11 @@ static std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor& dy, const
 struct GroupNormActFn : public torch::autograd::Function<GroupNormActFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps, int64_t act) {
         const Tensor last = channels_last(x);
-        auto [y, stats] = group_norm_fwd(last, weight, bias, groups, eps, act);
+        auto [y, stats] = group_norm_fwd(last, weight, bias, groups, eps, act, true);
         ctx->save_for_backward({last, weight.value_or(Tensor()), bias.value_or(Tensor()), stats});
         ctx->saved_data["groups"] = groups;
         ctx->saved_data["act"] = act;
-        return channels_first(y);
+        return y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         once_only("group_norm_act");
@@ -169,7 +196,7 @@ static Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& w
     const int64_t act = activation_code(activation);
     if (c10::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
         return GroupNormActFn::apply(x, weight, bias, groups, eps, act);
-    return channels_first(std::get<0>(group_norm_fwd(channels_last(x), weight, bias, groups, eps, act)));
+    return std::get<0>(group_norm_fwd(channels_last(x), weight, bias, groups, eps, act, true));
 }
 
 // ------------------------------------------------------------------------------------------------ label log probabilities
@@ -229,12 +256,8 @@ static Tensor check_target(const OptTensor& target, const Layout& q) {
 // Memory of [N, k, ...] that follows the logits: k last for rows
 static Tensor like_layout(const Layout& q, int64_t k, at::ScalarType type) {
     std::vector<int64_t> s = q.shape;
-    if (q.rows && s.size() > 1) {
-        s.push_back(k);
-        return at::empty(s, q.z.options().dtype(type)).movedim(-1, 1);
-    }
     s.insert(s.begin() + 1, k);
-    return at::empty(s, q.z.options().dtype(type));
+    return q.rows && s.size() > 2 ? empty_channels_last(s, q.z.options().dtype(type)) : at::empty(s, q.z.options().dtype(type));
 }
 // ... of a tensor [N, k, ...] given from outside
 static Tensor to_layout(const Tensor& t, const Layout& q) { return q.rows && t.dim() > 2 ? t.movedim(1, -1).contiguous() : t.contiguous(); }
@@ -336,7 +359,7 @@ static std::tuple<Tensor, Tensor, Tensor, Tensor> class_log_probs(const Tensor& 
 // What the device tables of an optimizer describe: which parameters have a gradient, and where both lie.  look() compares that with
 // the present; it keeps no gradient alive.
 struct ParamWatch {
-    struct Entry { const void *param, *grad; bool on, copied; };
+    struct Entry { const void *param, *grad; bool on, copied; at::ScalarType type; at::DimVector shape; };          // shape: sizes, then strides
     std::vector<Entry> entries;
     std::vector<Tensor> params;                 // those with a gradient, in the order of the groups
 
@@ -349,6 +372,12 @@ struct ParamWatch {
         TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.scalar_type() == p.scalar_type() && g.device() == p.device() && g.sizes() == p.sizes(),
                           "AdamW: a gradient of a parameter ", p.dtype(), " ", p.sizes(), " has to be a dense tensor of the same type, shape and device, got ",
                           g.dtype(), " ", g.sizes());
+    }
+
+    static bool same_shape(const Tensor& p, const Entry& e) {
+        const at::IntArrayRef seen(e.shape);
+        const size_t d = p.dim();
+        return seen.size() == 2 * d && p.sizes() == seen.slice(0, d) && p.strides() == seen.slice(d);
     }
 
     // 0: all as before; 1: the same parameters, gradients elsewhere (noted); 2: other parameters, or parameters elsewhere.
@@ -365,9 +394,9 @@ struct ParamWatch {
                 Entry& e = entries[i++];
                 if (on != e.on) return 2;
                 if (!on) continue;
-                if (p.data_ptr() != e.param) return 2;
+                if (p.data_ptr() != e.param || p.scalar_type() != e.type || !same_shape(p, e)) return 2;
                 const bool strided = g.layout() == at::kStrided;
-                if (strided && g.data_ptr() == e.grad && g.strides() == p.strides() && g.scalar_type() == p.scalar_type() && !e.copied) continue;
+                if (strided && g.data_ptr() == e.grad && g.sizes() == p.sizes() && g.strides() == p.strides() && g.scalar_type() == e.type && !e.copied) continue;
                 check_grad(p, g);
                 e.grad = g.data_ptr();
                 e.copied = g.strides() != p.strides() && !(g.is_contiguous() && p.is_contiguous());
@@ -385,7 +414,8 @@ struct ParamWatch {
                 const Tensor& p = tensor(h.ptr());
                 const bool on = p.grad().defined() && p.numel();
                 if (on) check_grad(p, p.grad());
-                entries.push_back({on ? p.data_ptr() : nullptr, nullptr, on, false});
+                entries.push_back({on ? p.data_ptr() : nullptr, nullptr, on, false, p.scalar_type(), at::DimVector(p.sizes())});
+                entries.back().shape.append(p.strides().begin(), p.strides().end());
                 if (on) params.push_back(p);
             }
     }
@@ -469,7 +499,7 @@ static void adamw_no_overlap(const std::vector<Tensor>& params) {
 
 static std::tuple<Tensor, Tensor> group_norm_act_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps,
                                                      const std::string& activation) {
-    return group_norm_fwd(x, weight, bias, groups, eps, activation_code(activation));
+    return group_norm_fwd(x, weight, bias, groups, eps, activation_code(activation), false);
 }
 static std::tuple<Tensor, Tensor, Tensor> group_norm_act_bwd(const Tensor& dy, const Tensor& x, const OptTensor& weight, const OptTensor& bias, const Tensor& stats,
                                                              int64_t groups, const std::string& activation) {

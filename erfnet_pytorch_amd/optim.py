@@ -78,7 +78,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"invalid eps {group['eps']}")
         if not 0.0 <= group["weight_decay"] < float("inf"):
             raise ValueError(f"invalid weight decay {group['weight_decay']}")
-        for p in group["params"]:
+        self._check_params(group["params"])
+
+    @staticmethod
+    def _check_params(params):
+        for p in params:
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError(f"AdamW updates float32 or bfloat16 parameters, got {p.dtype}")
             if not _dense(p):
@@ -160,6 +164,7 @@ class AdamW(torch.optim.Optimizer):
     # -- device tables --------------------------------------------------------------------------
     def _build(self, groups):
         live = [p for g in groups for p in g if p.grad is not None and p.numel()]
+        self._check_params(live)                        # they may have changed, or been put into a group by hand
         for p in live:
             ops.require_gpu(p, "AdamW")
         if live and torch.cuda.is_current_stream_capturing():

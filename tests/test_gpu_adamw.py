@@ -96,6 +96,30 @@ def test_the_watch_reports_what_changed():
         w.look([ps])
 
 
+def test_the_watch_sees_other_shapes_at_the_same_place():
+    """p.data replaced by a part or another order of itself: the tables describe something else then."""
+    from erfnet_pytorch_amd.optim import _host
+    for other in (lambda t: t[:2], lambda t: t.view(3, 4), lambda t: t.view(3, 4).t()):
+        p = torch.nn.Parameter(torch.zeros(4, 3))
+        p.grad = torch.zeros(4, 3)
+        w = _host.ParamWatch()
+        w.bind([[p]])
+        assert [w.look([[p]]) for _ in range(2)] == [1, 0]
+        p.grad = None
+        p.data = other(p.data)
+        p.grad = torch.zeros_like(p)
+        assert w.look([[p]]) == 2
+
+
+def test_parameters_put_into_a_group_by_hand_are_checked():
+    p, h = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4, dtype=torch.float16))
+    opt = _adamw([p])
+    opt.param_groups[0]["params"].append(h)
+    h.grad = torch.zeros_like(h)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        opt.step()
+
+
 def test_parameters_that_share_memory_are_found():
     from erfnet_pytorch_amd.optim import _host
     t = torch.zeros(10)

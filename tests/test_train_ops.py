@@ -76,6 +76,39 @@ def test_cpu_tensors_are_refused():
         T.class_log_probs_fwd(torch.zeros(3, 4), None, 0, -100)
 
 
+def test_tensors_that_dispatch_to_python_are_refused():
+    """Their memory is not the one they show (outputs would be left unwritten); fake tensors are the exception."""
+    class Wrapped(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError
+    for call in (lambda: TO.group_norm_act_fwd(Wrapped(torch.zeros(2, 3, 4)), None, None, 2, 1e-5, "none"),
+                 lambda: TO.class_log_probs_fwd(Wrapped(torch.zeros(3, 4)), None, 0, -100)):
+        with pytest.raises(TypeError, match="plain tensors"):
+            call()
+
+
+@pytest.mark.gpu
+def test_outputs_may_be_written_in_place():
+    """As torch's own: h = norm(x); h += residual."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    from erfnet_pytorch_amd.norm import group_norm_act
+    x, r, dy = (torch.randn(2, 8, 6, 10, device="cuda").contiguous(memory_format=torch.channels_last) for _ in range(3))
+    grads = []
+    for inplace in (False, True):
+        xs = x.clone().requires_grad_()
+        y = group_norm_act(xs, 2)
+        y = y.add_(r).mul_(2.0) if inplace else (y + r) * 2.0
+        out = class_log_probs(xs, torch.zeros(2, 6, 10, dtype=torch.int64, device="cuda"), top_k=2)
+        lp, top = (out.log_prob.mul_(3.0), out.top_log_probs.mul_(2.0)) if inplace else (out.log_prob * 3.0, out.top_log_probs * 2.0)
+        grads.append(torch.autograd.grad((y * dy).sum() + lp.sum() + top.sum(), xs)[0])
+    assert torch.equal(*grads)
+
+
 @pytest.mark.gpu
 def test_opcheck_against_the_device_kernels():
     checks = ("test_schema", "test_faketensor")
