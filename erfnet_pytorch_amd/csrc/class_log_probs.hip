@@ -315,14 +315,18 @@ __global__ __launch_bounds__(256) void lp_position_kernel(const LpArgs a) {
 
 // ------------------------------------------------------------------------------------------------ a team of threads per row
 // A row is cut at the 16-byte boundaries of memory into chunks of EPC classes, the first and the last possibly partial; thread r of
-// the team takes chunks r, r + TEAM, ...  UNROLL of them are in flight and share one change of the maximum.  Teams of 8, 16 or 64
-// lanes have the whole row in registers then; a workgroup goes on along a longer row.
+// the team takes chunks r, r + TEAM, ...  U of them are in flight and share one change of the maximum; those behind the row's end are
+// skipped by the whole wave (20000 x 2048 bf16 38 us against 59).  Teams of 8, 16 or 64 lanes have the whole row in registers then; a
+// workgroup goes on along a longer row.
 //
 // Alternatives: the k-th largest of the threads' own maxima is a bound that the k best classes reach, and few others do.  What
 // reaches it is collected -- from the registers, or by the whole workgroup from the chunks of the threads whose maximum reaches it --
 // and put in its place by counting.  Rows with NaN, and rows where more values tie than the collection holds, go through k rounds
 // over the row.
-#define UNROLL 4
+//
+// Bound by the memory where rows are long (4096 x 32000 bf16 52 us, 5.0 TB/s; fp32 93 us, 5.6 TB/s), by the arithmetic where the
+// logits come out of the cache (8 instructions a value, one of them an exp), and by the selection, 0.5 ns a row: 100000 x 1000 fp32
+// 68 us, with 5 alternatives 123; bf16 43 and 80.  The loads of the next set ahead of the work on this one gained nothing here.
 
 template <int TEAM> struct TeamShared {
     enum { CAND = TEAM == 256 ? 512 : TEAM == 64 ? 256 : 64 };
@@ -343,21 +347,28 @@ template <int TEAM> __device__ __forceinline__ void team_sync() {
     }
 }
 
-// Chunk q of a row whose first class lies `off` classes behind a boundary, as it lies in memory; what is not part of the row is -inf.
+// Where the logits begin and end.  A row's first and last chunk may hold classes of its neighbours: within these bounds they are read
+// whole all the same (100000 x 1001 bf16 75 us against 95 where they are gathered), and what is not the row's is masked afterwards.
+template <typename T> struct Span { const T *first, *last; };
+template <typename T, typename ARGS>
+__device__ __forceinline__ Span<T> span_of(const ARGS& a) { return Span<T>{(const T*)a.z, (const T*)a.z + (a.N - 1) * a.sn + a.C}; }
+
+// Chunk q of a row whose first class lies `off` classes behind a boundary, as it lies in memory.
 // It is taken apart by chunk_values, after all loads of a set: taken apart behind the branch, each load would be waited for alone.
 template <typename T>
-__device__ __forceinline__ i32x4 load_chunk(const T* row, int off, int C, int q) {
+__device__ __forceinline__ i32x4 load_chunk(const Span<T>& span, const T* row, int off, int C, int q) {
     constexpr int E = Elem<T>::EPC;
     const int c0 = q * E - off;
-    if (c0 >= 0 && c0 + E <= C) return *(const i32x4*)(row + c0);
+    const T* p = row + c0;
+    if (p >= span.first && p + E <= span.last) return *(const i32x4*)p;
     i32x4 r;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         if constexpr (E == 4) {
-            r[w] = c0 + w >= 0 && c0 + w < C ? __float_as_int(row[c0 + w]) : (int)0xFF800000u;
+            r[w] = c0 + w >= 0 && c0 + w < C ? __float_as_int(row[c0 + w]) : 0;
         } else {
             const int c = c0 + 2 * w;
-            const unsigned lo = c >= 0 && c < C ? row[c] : 0xFF80u, hi = c + 1 >= 0 && c + 1 < C ? row[c + 1] : 0xFF80u;
+            const unsigned lo = c >= 0 && c < C ? row[c] : 0u, hi = c + 1 >= 0 && c + 1 < C ? row[c + 1] : 0u;
             r[w] = (int)(lo | hi << 16);
         }
     }
@@ -373,6 +384,17 @@ __device__ __forceinline__ void chunk_values(const i32x4& r, float* f) {
     }
 }
 #define NO_CLASSES(T) (Elem<T>::EPC == 4 ? (int)0xFF800000u : (int)0xFF80FF80u)          // -inf in every place of a word
+// ... with -inf for what is not the row's
+template <typename T>
+__device__ __forceinline__ void row_values(const i32x4& r, int off, int C, int q, float* f) {
+    constexpr int E = Elem<T>::EPC;
+    const int c0 = q * E - off;
+    chunk_values<T>(r, f);
+    if (c0 < 0 || c0 + E > C) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = c0 + e >= 0 && c0 + e < C ? f[e] : -INFINITY;
+    }
+}
 
 // How many of n ranks in LDS are above r; 8 reads are in flight together
 __device__ __forceinline__ int count_above(const u64* ranks, int n, u64 r) {
@@ -433,8 +455,8 @@ __device__ __forceinline__ float kth_largest(float* v, int k, int tid) {
     return m;
 }
 
-template <typename T, int TEAM, bool TOP>
-__global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
+template <typename T, int TEAM, int U, bool TOP>
+__global__ __launch_bounds__(256, TEAM == 256 ? 7 : U == 4 ? 5 : 4) void lp_rows_kernel(const LpArgs a) {
     constexpr int E = Elem<T>::EPC;
     __shared__ TeamShared<TOP || TEAM == 256 ? TEAM : 8> shared[TOP || TEAM == 256 ? 256 / TEAM : 1];
     const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
@@ -446,26 +468,34 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
     const int chunks = (a.C + off + E - 1) / E, per = (chunks + a.segments - 1) / a.segments;
     const int seg = blockIdx.y, q0 = min(seg * per, chunks), q1 = min(q0 + per, chunks);
 
+    const Span<T> span = span_of<T>(a);
     LpTarget target{};
     if (tid == 0 && a.segments == 1) target = lp_target(a, row, i);
     Stat st{-INFINITY, 0.f, 0.f};
-    float f[UNROLL][E];
-    for (int q = q0 + tid; q < (TEAM < 256 ? q0 + TEAM : q1); q += TEAM * UNROLL) {
-        i32x4 raw[UNROLL];
+    float f[U][E];
+    const int end = TEAM < 256 ? (a.C + 2 * (E - 1)) / E : q1;                // the chunks of any row: one bound for the whole wave
+    for (int q = q0; q < (TEAM < 256 ? 1 : q1); q += TEAM * U) {
+        i32x4 raw[U];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             raw[u] = i32x4{NO_CLASSES(T), NO_CLASSES(T), NO_CLASSES(T), NO_CLASSES(T)};
-            if (q + u * TEAM < q1) raw[u] = load_chunk(row, off, a.C, q + u * TEAM);
+            if (q + u * TEAM + tid < q1) raw[u] = load_chunk(span, row, off, a.C, q + u * TEAM + tid);
         }
+        float most = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) chunk_values<T>(raw[u], f[u]);
-        const float most = largest<UNROLL * E>([&](int n) { return f[n / E][n % E]; });
+        for (int u = 0; u < U; ++u)
+            if (q + u * TEAM < end) {
+                row_values<T>(raw[u], off, a.C, q + u * TEAM + tid, f[u]);
+                most = __builtin_elementwise_maximum(most, largest<E>([&](int e) { return f[u][e]; }));
+            }
         if (most > st.m) stat_move(st, most);
         const float base = base_of(st.m);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < U; ++u)
+            if (q + u * TEAM < end) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) stat_add(st, base, f[u][e]);
+                for (int e = 0; e < E; ++e) stat_add(st, base, f[u][e]);
+            }
     }
     float own[1] = {st.m};                                             // this thread's largest value
     constexpr int WAVE = TEAM < 256 ? TEAM : 64;
@@ -522,7 +552,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
                 const float least = kth_largest<TEAM, 1>(own, a.k, tid);
                 team_sync<TEAM>();
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u)
+                for (int u = 0; u < U; ++u)
                     if (q0 + tid + u * TEAM < q1) collect(f[u], q0 + tid + u * TEAM, least);
             } else {
                 sh.max[tid] = own[0];
@@ -544,7 +574,7 @@ __global__ __launch_bounds__(256) void lp_rows_kernel(const LpArgs a) {
                     const int q = q0 + sh.winner[p / each] + p % each * TEAM;
                     if (q >= q1) continue;
                     float v[E];
-                    chunk_values<T>(load_chunk(row, off, a.C, q), v);
+                    chunk_values<T>(load_chunk(span, row, off, a.C, q), v);
                     collect(v, q, least);
                 }
             }
@@ -777,10 +807,11 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     if (gh != 0.f) pull = fmaf(gh, a.entropy[i], pull);
     {
         const int q = q0 + tid;
+        const Span<T> span = span_of<T>(a);
         i32x4 raw[BWD_UNROLL];
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u)
-            if (any && q + u * TEAM < q1) raw[u] = load_chunk(row, off, a.C, q + u * TEAM);
+            if (any && q + u * TEAM < q1) raw[u] = load_chunk(span, row, off, a.C, q + u * TEAM);
 #pragma unroll
         for (int u = 0; u < BWD_UNROLL; ++u) {
             if (q + u * TEAM >= q1) break;
@@ -836,22 +867,28 @@ static inline int lp_positions(int dtype, long long N, long long L, long long sc
 }
 
 // Rows of more classes than a thread walks through by itself are taken by the smallest team that has the whole row in registers
-// wherever it starts (and lanes for the alternatives), or by a workgroup; few rows of very many classes are split so that about 1024 workgroups have work.
+// wherever it starts (and lanes for the alternatives), or by a workgroup.  8 chunks a thread let a smaller team have a row, fewer
+// waves stay on a SIMD: forward, 8 / 4 chunks, 100000 x 1000 bf16 42 / 65 us, 20000 x 2049 25 / 39, 100000 x 200 15 / 13, 20000 x 2000
+// 23 / 19: 8 where 4 would need the larger team.  Few rows of very many classes are split so that about 1024 workgroups have work.
 static inline int lp_epc(int dtype) { return dtype == ERF_BF16 ? 8 : 4; }
 // A thread takes a whole row of up to `alone` classes: up to there a wave's rows fill the cache lines that its loads touch.  1000000
 // rows by threads / by teams, us: forward fp32 24 classes 59 / 53, 32 88 / 54, bf16 40 51 / 75, 48 101 / 80; with 2 alternatives fp32 32
 // 90 / 90, 40 129 / 107, bf16 56 99 / 129, 64 162 / 127; backward fp32 12 49 / 51, 16 88 / 57; bf16 12 27 / 68, 16 55 / 48, 24 91 / 48.
 #define ALONE_FWD(dtype, k) ((dtype) == ERF_BF16 ? ((k) ? 56 : 44) : ((k) ? 32 : 24))
 #define ALONE_BWD 12
-static inline int lp_team(int dtype, int C, int k, int alone) {
-    if (C <= alone) return 1;
-    for (int team = 8; team <= 64; team = team == 16 ? 64 : 2 * team)
-        if (k <= team && C <= (team * UNROLL - 1) * lp_epc(dtype) + 1) return team;
-    return 256;
+struct LpTeam { int team, each; };     // team 1: a thread; each: chunks in flight per thread
+static inline LpTeam lp_team(int dtype, int C, int k, int alone, int most) {
+    static const LpTeam teams[] = {{8, 4}, {16, 4}, {16, 8}, {64, 4}, {64, 8}};
+    if (C <= alone) return {1, 0};
+    for (const LpTeam& t : teams)
+        if (t.each <= most && k <= t.team && C <= (t.team * t.each - 1) * lp_epc(dtype) + 1) return t;
+    return {256, 4};
 }
+static inline LpTeam lp_fwd_team(int dtype, int C, int k) { return lp_team(dtype, C, k, ALONE_FWD(dtype, k), 8); }
+static inline LpTeam lp_bwd_team(int dtype, int C) { return lp_team(dtype, C, 0, ALONE_BWD, BWD_UNROLL); }
 static inline int lp_segments(int dtype, long long N, int C, int k) {
-    if (lp_team(dtype, C, k, ALONE_FWD(dtype, k)) < 256) return 1;
-    const long long most = ((long long)C + 256 * UNROLL * lp_epc(dtype) - 1) / (256 * UNROLL * lp_epc(dtype)), want = (1024 + N - 1) / N;
+    if (lp_fwd_team(dtype, C, k).team < 256) return 1;
+    const long long most = ((long long)C + 1024 * lp_epc(dtype) - 1) / (1024 * lp_epc(dtype)), want = (1024 + N - 1) / N;
     return (int)(want < most ? want : most);
 }
 
@@ -860,21 +897,23 @@ static inline int lp_segments(int dtype, long long N, int C, int k) {
 
 template <typename T, bool TOP>
 static void lp_rows_launch(LpArgs a, int dtype, hipStream_t s) {
-    const int team = lp_team(dtype, a.C, a.k, ALONE_FWD(dtype, a.k));
+    const auto [team, each] = lp_fwd_team(dtype, a.C, a.k);
     for (a.first = 0; a.first < a.N; a.first += ROWS_PER_LAUNCH(team)) {
         const long long rows = a.N - a.first < ROWS_PER_LAUNCH(team) ? a.N - a.first : ROWS_PER_LAUNCH(team);
         const dim3 grid((unsigned)((rows * team + 255) / 256), (unsigned)a.segments), block(256);
-        if (team == 8) hipLaunchKernelGGL((lp_rows_kernel<T, 8, TOP>), grid, block, 0, s, a);
-        else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, TOP>), grid, block, 0, s, a);
-        else if (team == 64) hipLaunchKernelGGL((lp_rows_kernel<T, 64, TOP>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((lp_rows_kernel<T, 256, TOP>), grid, block, 0, s, a);
+        if (team == 8) hipLaunchKernelGGL((lp_rows_kernel<T, 8, 4, TOP>), grid, block, 0, s, a);
+        else if (team == 16 && each == 4) hipLaunchKernelGGL((lp_rows_kernel<T, 16, 4, TOP>), grid, block, 0, s, a);
+        else if (team == 16) hipLaunchKernelGGL((lp_rows_kernel<T, 16, 8, TOP>), grid, block, 0, s, a);
+        else if (team == 64 && each == 4) hipLaunchKernelGGL((lp_rows_kernel<T, 64, 4, TOP>), grid, block, 0, s, a);
+        else if (team == 64) hipLaunchKernelGGL((lp_rows_kernel<T, 64, 8, TOP>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((lp_rows_kernel<T, 256, 4, TOP>), grid, block, 0, s, a);
     }
     if (a.segments > 1) hipLaunchKernelGGL(lp_join_kernel<T>, dim3((unsigned)a.N), dim3(256), 0, s, a);
 }
 
 template <typename T>
 static void lp_rows_bwd_launch(LpBwdArgs a, int dtype, hipStream_t s) {
-    const int team = lp_team(dtype, a.C, 0, ALONE_BWD), per = 256 * BWD_UNROLL;
+    const int team = lp_bwd_team(dtype, a.C).team, per = 256 * BWD_UNROLL;
     const int chunks = (a.C + 2 * (lp_epc(dtype) - 1)) / lp_epc(dtype);              // of a row that starts just before a boundary
     for (a.first = 0; a.first < a.N; a.first += ROWS_PER_LAUNCH(team)) {
         const long long rows = a.N - a.first < ROWS_PER_LAUNCH(team) ? a.N - a.first : ROWS_PER_LAUNCH(team);
@@ -903,7 +942,7 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         return ERF_EINVAL;
     LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, 0, (u64*)workspace};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && lp_team(dtype, C, top_k, ALONE_FWD(dtype, top_k)) > 1) {
+    if (stride_c == 1 && lp_fwd_team(dtype, C, top_k).team > 1) {
         a.segments = lp_segments(dtype, N, C, top_k);
         if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
         else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
@@ -937,7 +976,7 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
                       g_log_prob, g_entropy, g_top, top_indices, dlogits, 0};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && lp_team(dtype, C, 0, ALONE_BWD) > 1) {
+    if (stride_c == 1 && lp_bwd_team(dtype, C).team > 1) {
         if (dtype == ERF_BF16) lp_rows_bwd_launch<bf16raw>(a, dtype, s);
         else lp_rows_bwd_launch<float>(a, dtype, s);
     } else {

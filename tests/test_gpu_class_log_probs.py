@@ -149,6 +149,18 @@ def test_rows(shape, layout, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("classes", [25, 44, 45, 56, 57, 125, 126, 249, 250, 253, 254, 505, 509, 510, 1017, 1018, 1021, 1022, 2041, 2045, 4089, 4090])
+def test_rows_at_the_ends_of_every_plan(classes, dtype):
+    """The largest and smallest rows of the threads and of each team, between NaN: what lies beside a row has no effect on it."""
+    z = _logits((9, classes), dtype, "plain", classes)
+    room = torch.full((9, classes + 3), float("nan"), dtype=dtype, device="cuda")
+    room[:, 1:classes + 1] = z
+    for k in (0, 3):
+        _check(room[:, 1:classes + 1], _targets(z, classes), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("layout", ["plain", "channels_last", "sliced", "transposed"])
 @pytest.mark.parametrize("shape", MAPS)
 def test_maps(shape, layout, dtype):
@@ -277,9 +289,9 @@ def test_without_target_and_partial_gradients():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("classes,k,rows", [(60, 0, 2 ** 27 + 500), (600, 2, 2 ** 24 + 500), (2500, 1, 2 ** 22 + 500)])
+@pytest.mark.parametrize("classes,k,rows", [(60, 0, 2 ** 27 + 500), (600, 2, 2 ** 26 + 500), (1500, 1, 2 ** 24 + 500), (4500, 1, 2 ** 22 + 500)])
 def test_more_rows_than_one_launch_takes(classes, k, rows):
-    """Rows that overlap in memory (the next one starts a class later), by teams of 8 and 64 and by workgroups: around the seams of the
+    """Rows that overlap in memory (the next one starts a class later), by teams of 8, 16 and 64 and by workgroups: around the seams of the
     launches the bits of a call on those rows alone."""
     from erfnet_pytorch_amd import train_ops as TO
     buf = torch.randn(rows + classes, device="cuda").to(torch.bfloat16)
