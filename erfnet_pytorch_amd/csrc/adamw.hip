@@ -12,6 +12,10 @@
 // by 0.1 % a step and half an e4m3 step is 3 % to 6 %, so rounding to nearest would never let v fall.  sqrt(v) > 0 never
 // becomes 0 (its smallest code stands in): the next update divides by it.  The update of p uses the new moments before they
 // are rounded.
+//
+// 32 bits: the memory bounds it (fp32: 28 bytes an element).  8 bits: 97 M elements in bf16 (10 bytes each) 216 us, 4.5 TB/s, memory and
+// arithmetic about even.  A network's 228 small tensors (2.1 M elements): 13 us in either, one launch's latency and the tail of
+// the tensors that fill no chunk.
 #include "../../include/erfnet_mi355.h"
 #include "common.cuh"
 #include <type_traits>

@@ -339,6 +339,23 @@ def test_nothing_beside_the_tensors_is_written(bits):
 
 
 @pytest.mark.gpu
+def test_a_tensor_of_more_than_2_to_the_32_elements():
+    """Its last elements get the bits that a small tensor of the same values gets."""
+    n, tail = 2 ** 32 + 5000, 9000
+    gen = torch.Generator().manual_seed(9)
+    end, grad = (torch.randn(tail, generator=gen).bfloat16().cuda() for _ in range(2))
+    p, q = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda")), torch.nn.Parameter(end.clone())
+    p.data[-tail:] = end
+    p.grad, q.grad = torch.zeros_like(p), grad
+    p.grad[-tail:] = grad
+    opt = _adamw([p, q], lr=1e-2)
+    opt.step()
+    assert torch.equal(p.detach()[-tail:], q.detach()) and float(p.detach()[:-tail].abs().max()) == 0.0
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(opt.state[p][k][-tail:], opt.state[q][k])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_groups_missing_gradients_and_layouts(bits):
     """Groups with settings of their own, parameters without a gradient (left alone, with their own step count), channels-last

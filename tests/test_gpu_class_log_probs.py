@@ -311,6 +311,22 @@ def test_more_rows_than_one_launch_takes(classes, k, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,stride", [((4, 1000), (2 ** 31, 1)), ((4, 40), (2 ** 31, 1)), ((2, 20, 64), (20 * 2 ** 27, 2 ** 27, 1))])
+def test_offsets_that_pass_32_bits(shape, stride):
+    """Rows, and planes, so far apart: the bits of a compact copy."""
+    from erfnet_pytorch_amd import train_ops as TO
+    room = torch.empty(sum((n - 1) * s for n, s in zip(shape, stride)) + 1, dtype=torch.bfloat16, device="cuda")
+    small = _logits(shape, torch.bfloat16, "plain", 3)
+    z = room.as_strided(shape, stride).copy_(small)
+    t = torch.randint(0, shape[1], (shape[0], *shape[2:]), device="cuda")
+    outs = [TO.class_log_probs_fwd(v, t, 3, -100) for v in (z, small)]
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    g, top = torch.randn(t.shape, device="cuda"), torch.randn(outs[0][3].shape, device="cuda")
+    dz = [TO.class_log_probs_bwd(v, t, o[2], o[1], o[4], g, g, top, -100) for v, o in zip((z, small), outs)]
+    assert torch.equal(*dz)
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     from erfnet_pytorch_amd.loss import class_log_probs
     z = _logits((3, 30), torch.float32, "plain", 17).requires_grad_()

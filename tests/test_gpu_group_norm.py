@@ -259,6 +259,30 @@ def test_more_groups_than_one_launch_has_workgroups():
 
 
 @pytest.mark.gpu
+def test_offsets_that_pass_32_bits():
+    """A map of 2^32 + 2^23 values whose pixels repeat with period 64: mean, variance and gradient means are those of one period.
+
+    At most 4096 additions one after another (1024 workgroups share a map's pixels, two pixel lanes each: 2052 pixels a thread, and some
+    tens to join them), d U = 2^-12.  In the forward pass 4 pixels are summed before they are joined: 2^-14 of the mean size 0.8 and of
+    rstd, so off(u) <= 2^-14 (1 + |xhat|) <= 6 * 2^-14 for |xhat| <= 5, and y is off by 1.1 of that and half a step: 2^-10 + 2^-8 |y|.
+    dx: |dy| off(u) / 2 <= 2^-10, the two means 2^-12 * 0.8 (1 + |xhat|) <= 2^-9, and half a step: 2^-8 + 2^-8 |dx|."""
+    from erfnet_pytorch_amd import train_ops as TO
+    n, p, c, groups = 8, 2 ** 19 + 2 ** 10, 1024, 8
+    gen = torch.Generator().manual_seed(6)
+    x, dy = (torch.randn(1, 64, c, generator=gen).bfloat16() for _ in range(2))
+    big, dbig = (t.cuda().expand(n * p // 64, 64, c).reshape(n, p, c) for t in (x, dy))
+    y, stats = TO.group_norm_act_fwd(big, None, None, groups, 1e-5, "silu")
+    xd = x.double().requires_grad_()
+    want = _ref(xd, torch.ones(c, dtype=torch.float64), torch.zeros(c, dtype=torch.float64), groups, 1e-5, "silu")
+    dwant = torch.autograd.grad(want, xd, dy.double())[0]
+    dx = TO.group_norm_act_bwd(dbig, big, None, None, stats, groups, "silu")[0]
+    for i, at in ((0, 0), (n - 1, p - 64)):
+        assert ((y[i, at:at + 64].cpu().double() - want.detach()[0]).abs() <= 2.0 ** -10 + 2.0 ** -8 * want.detach()[0].abs()).all()
+        assert ((dx[i, at:at + 64].cpu().double() - dwant[0]).abs() <= 2.0 ** -8 * (1 + dwant[0].abs())).all()
+        assert torch.equal(y[i, at:at + 64], y[0, :64]) and torch.equal(dx[i, at:at + 64], dx[0, :64])
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     from erfnet_pytorch_amd.norm import group_norm_act
     x, w, b, dy = _inputs((1, 8, 4, 4), torch.float32, 12)
