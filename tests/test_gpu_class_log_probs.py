@@ -327,6 +327,33 @@ def test_offsets_that_pass_32_bits(shape, stride):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,k", [((40, 9), 5), ((40, 60), 3), ((40, 60), 20), ((9, 300), 32), ((9, 1200), 32), ((5, 5000), 32), ((2, 20, 4, 6), 2), ((2, 20, 4, 6), 12)])
+def test_alternatives_that_name_a_class_more_than_once(shape, k):
+    """The backward pass takes the classes as they are given: the same one several times, and the target's, get every gradient.
+
+    p is off by at most (2 |log p| + 8) U of itself, the sums of k gradients by k U: in all (2 max |log p| + k + 16) U of
+    (|gl| + sum |gk|) (1 + p) + |gh| p (|log p| + H)."""
+    from erfnet_pytorch_amd import train_ops as TO
+    z = _logits(shape, torch.float32, "plain", 21, spread=1.0)
+    n, c = shape[:2]
+    pos = (n, *shape[2:])
+    gen = torch.Generator().manual_seed(22)
+    t = torch.randint(0, c, pos, generator=gen)
+    idx = torch.randint(0, c, (n, k, *shape[2:]), generator=gen)
+    idx[:, 1] = idx[:, 0]
+    idx[: n // 2, k - 1] = t[: n // 2]
+    gl, gh, gk = torch.randn(pos, generator=gen), torch.randn(pos, generator=gen), torch.randn(idx.shape, generator=gen)
+    _, ent, stats, _, _ = TO.class_log_probs_fwd(z, t.cuda(), 0, -100)
+    got = _to_rows(TO.class_log_probs_bwd(z, t.cuda(), stats, ent, idx.cuda(), gl.cuda(), gh.cuda(), gk.cuda(), -100).cpu().double(), True)
+    lp = torch.log_softmax(_to_rows(z.cpu().double(), True), -1)
+    p, h = lp.exp(), -(lp.exp() * lp).sum(-1, keepdim=True)
+    tr, ir, lr, hr, kr = t.reshape(-1, 1), _to_rows(idx, True), gl.double().reshape(-1, 1), gh.double().reshape(-1, 1), _to_rows(gk.double(), True)
+    want = torch.zeros_like(p).scatter_add_(1, tr, lr).scatter_add_(1, ir, kr) - p * (lr + kr.sum(-1, keepdim=True)) - hr * p * (lp + h)
+    size = (lr.abs() + kr.abs().sum(-1, keepdim=True)) * (1 + p) + hr.abs() * p * (lp.abs() + h)
+    assert ((got - want).abs() <= (2 * float(lp.abs().max()) + k + 16) * U * size).all()
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     from erfnet_pytorch_amd.loss import class_log_probs
     z = _logits((3, 30), torch.float32, "plain", 17).requires_grad_()
