@@ -783,9 +783,68 @@ __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a)
     }
 }
 
+// Many rows of few classes that lie one behind the other: 256 rows are brought to LDS and back as one stretch of memory, and a thread
+// works off a row there.  Rows of an even number of classes are begun at another class in each lane, which spreads the lanes over
+// LDS's banks.
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void lp_rows_lds_bwd_kernel(const LpBwdArgs a) {
+    constexpr int K = KT > 0 ? KT : 1, E = Elem<T>::EPC;
+    extern __shared__ i32x4 stage[];
+    T* lds = (T*)stage;
+    const long long first = (long long)blockIdx.x * 256, i = first + threadIdx.x;
+    const int rows = (int)(a.N - first < 256 ? a.N - first : 256), count = rows * a.C;
+    const T* z = (const T*)a.z + first * a.C;
+    T* dz = (T*)a.dz + first * a.C;
+    for (int q = threadIdx.x; q < count / E; q += 256) stage[q] = ((const i32x4*)z)[q];
+    for (int e = count / E * E + threadIdx.x; e < count; e += 256) lds[e] = z[e];
+    float gl = 0.f, gh = 0.f, pull, base = 0.f, logs = 0.f, gk[K];
+    int t = -1, jk[K];
+    bool any = false;
+    if (i < a.N) {
+        if (a.g_log_prob) {
+            const long long v = a.target[i];
+            t = v >= 0 && v < a.C ? (int)v : -1;
+            gl = v == a.ignore ? 0.f : t >= 0 ? a.g_log_prob[i] : __builtin_nanf("");
+        }
+        if (a.g_entropy) gh = a.g_entropy[i];
+        base = a.stats[i];
+        logs = a.stats[a.N + i];
+    }
+    pull = gl;
+    any = gl != 0.f || gh != 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        gk[k] = 0.f;
+        jk[k] = -1;
+        if (KT > 0 && k < a.k && i < a.N) {
+            gk[k] = a.g_top[i * a.k + k];
+            load_indices<1>(a.top_index + i * a.k + k, &jk[k]);
+            pull += gk[k];
+            any = any || gk[k] != 0.f;
+        }
+    }
+    if (gh != 0.f) pull = fmaf(gh, a.entropy[i], pull);
+    __syncthreads();
+    if (i < a.N) {
+        T* row = lds + threadIdx.x * a.C;
+        int c = a.C % 2 ? 0 : threadIdx.x % a.C;
+        for (int n = 0; n < a.C; ++n) {
+            float own = t == c ? gl : 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) own += KT > 0 && jk[k] == c ? gk[k] : 0.f;
+            Elem<T>::st(row + c, any ? lp_grad(Elem<T>::ld(row + c), base, logs, gh, pull) + own : 0.f);
+            c = c + 1 == a.C ? 0 : c + 1;
+        }
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < count / E; q += 256) ((i32x4*)dz)[q] = stage[q];
+    for (int e = count / E * E + threadIdx.x; e < count; e += 256) dz[e] = lds[e];
+}
+
 // Rows by teams (4096 x 32001 bf16 86 us, 6.1 TB/s: the memory bounds it): chunks at the 16-byte boundaries as in the forward pass;
 // the target and the alternatives are written once more after the rest.  A gradient row that lies differently to the boundaries than the logits' row is stored class by class.
 #define BWD_UNROLL 4
+#define LDS_ROW 160       // bytes of a row
 template <typename T, int TEAM>
 __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     constexpr int E = Elem<T>::EPC;
@@ -926,6 +985,15 @@ static inline int lp_segments(int dtype, long long N, int C, int k) {
     return (int)(want < most ? want : most);
 }
 
+// Rows through LDS: compact, on 16-byte boundaries, few enough classes that 4 workgroups fit a CU's LDS, enough rows to fill the chip.
+// LDS against threads or teams, us: 3145728 x 20 fp32 115 / 248, bf16 68 / 275; 1000000 x 9 18 / 30 and 13 / 18; 1000000 x 24 41 / 75 and
+// 24 / 48; with 5 alternatives 61 / 118 and 42 / 72; 65536 x 20 5.7 / 6.8 and 5.2 / 6.4.
+static inline bool lp_bwd_in_lds(const LpBwdArgs& a, int dtype, long long sc) {
+    const int size = dtype == ERF_BF16 ? 2 : 4;
+    return sc == 1 && a.sn == a.C && a.dn == a.C && !(((unsigned long long)a.z | (unsigned long long)a.dz) % 16) && a.C * size <= LDS_ROW &&
+           a.N >= (1 << 16) && a.k <= 8;
+}
+
 // A launch has less than 2^32 threads: very many rows are several launches' work
 #define ROWS_PER_LAUNCH(team) ((1ll << 30) / (team))
 
@@ -1010,7 +1078,18 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
                       g_log_prob, g_entropy, g_top, top_indices, dlogits, 0};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && lp_bwd_team(dtype, C).team > 1) {
+    if (lp_bwd_in_lds(a, dtype, stride_c)) {
+        const dim3 grid((unsigned)((N + 255) / 256)), block(256);
+        const size_t lds = (size_t)256 * C * (dtype == ERF_BF16 ? 2 : 4);
+#define LP_KT(T)                                                                                            \
+    do {                                                                                                    \
+        if (a.k == 0) hipLaunchKernelGGL((lp_rows_lds_bwd_kernel<T, 0>), grid, block, lds, s, a);           \
+        else if (a.k <= 2) hipLaunchKernelGGL((lp_rows_lds_bwd_kernel<T, 2>), grid, block, lds, s, a);      \
+        else hipLaunchKernelGGL((lp_rows_lds_bwd_kernel<T, 8>), grid, block, lds, s, a);                    \
+    } while (0)
+        if (dtype == ERF_BF16) LP_KT(bf16raw); else LP_KT(float);
+#undef LP_KT
+    } else if (stride_c == 1 && lp_bwd_team(dtype, C).team > 1) {
         if (dtype == ERF_BF16) lp_rows_bwd_launch<bf16raw>(a, dtype, s);
         else lp_rows_bwd_launch<float>(a, dtype, s);
     } else {

@@ -161,6 +161,24 @@ def test_rows_at_the_ends_of_every_plan(classes, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(65536, 1), (65537, 2), (65700, 9), (65791, 20), (65536, 40), (65536, 41), (65600, 80), (1, 20, 256, 257)])
+def test_many_rows_of_few_classes(shape, dtype):
+    """The workgroup that works 256 rows off in LDS, its last one in part, and rows just too long or too many alternatives for it;
+    channels-last maps are such rows.  Ignored positions full of NaN get 0 and leave their neighbours alone."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits(shape, dtype, "channels_last" if len(shape) > 2 else "plain", 31)
+    t = _targets(z, 32)
+    for k in sorted({0, min(2, shape[1]), min(5, shape[1]), min(9, shape[1])}):
+        _check(z, t, k, seed=k)
+    rows = z.movedim(1, -1).reshape(-1, shape[1])
+    want = torch.autograd.grad(class_log_probs(z.requires_grad_(), t).log_prob.sum(), z)[0]
+    holes = torch.where((t == -100).reshape(-1, 1), torch.full_like(rows, float("nan")), rows).view(shape[0], *shape[2:], shape[1]).movedim(-1, 1)
+    got = torch.autograd.grad(class_log_probs(holes.requires_grad_(), t).log_prob.sum(), holes)[0]
+    assert torch.equal(got, want) and bool((t == -100).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("layout", ["plain", "channels_last", "sliced", "transposed"])
 @pytest.mark.parametrize("shape", MAPS)
 def test_maps(shape, layout, dtype):
