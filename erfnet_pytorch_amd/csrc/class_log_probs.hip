@@ -662,6 +662,78 @@ __global__ __launch_bounds__(256) void lp_join_kernel(const LpArgs a) {
     }
 }
 
+// Many rows of few classes that lie one behind the other: 256 rows are brought to LDS as one stretch of memory, and a thread works off
+// a row there, once for the maximum and once for the sums.  Rows of an even number of classes are begun at another class in each lane,
+// which spreads the lanes over LDS's banks.  Alternatives as in lp_position_kernel, equal values by their classes.
+#define LDS_ROW 160       // bytes of a row at most: 4 workgroups fit a CU's LDS
+template <typename T>
+__device__ __forceinline__ void rows_to_lds(const T* z, int count, i32x4* stage) {
+    constexpr int E = Elem<T>::EPC;
+    for (int q = threadIdx.x; q < count / E; q += 256) stage[q] = ((const i32x4*)z)[q];
+    for (int e = count / E * E + threadIdx.x; e < count; e += 256) ((T*)stage)[e] = z[e];
+}
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void lp_rows_lds_kernel(const LpArgs a) {
+    constexpr int K = KT > 0 ? KT : 1;
+    extern __shared__ i32x4 stage[];
+    const long long first = (long long)blockIdx.x * 256, i = first + threadIdx.x;
+    rows_to_lds<T>((const T*)a.z + first * a.C, (int)(a.N - first < 256 ? a.N - first : 256) * a.C, stage);
+    __syncthreads();
+    if (i >= a.N) return;
+    const T* row = (const T*)stage + threadIdx.x * a.C;
+    const int begin = a.C % 2 ? 0 : threadIdx.x % a.C;
+    const LpTarget target = lp_target(a, row, i);
+    Stat st{-INFINITY, 0.f, 0.f};
+    for (int c = 0; c < a.C; ++c) st.m = fmaxf(st.m, Elem<T>::ld(row + (c + begin < a.C ? c + begin : c + begin - a.C)));
+    const float base = base_of(st.m);
+    float tv[K];
+    int tc[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) { tv[k] = -INFINITY; tc[k] = -1; }
+    for (int n = 0; n < a.C; ++n) {
+        const int c = n + begin < a.C ? n + begin : n + begin - a.C;
+        const float z = Elem<T>::ld(row + c);
+        stat_add(st, base, z);
+        if (KT > 0) {
+            bool up[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) up[k] = z > tv[k] || (z == tv[k] && c < tc[k]);
+#pragma unroll
+            for (int k = K - 1; k >= 0; --k) {
+                const bool from_above = k > 0 && up[k > 0 ? k - 1 : 0];
+                tv[k] = from_above ? tv[k > 0 ? k - 1 : 0] : up[k] ? z : tv[k];
+                tc[k] = from_above ? tc[k > 0 ? k - 1 : 0] : up[k] ? c : tc[k];
+            }
+        }
+    }
+    const float logs = logf(st.s);
+    lp_finish(a, target, i, st, logs);
+    if (KT == 0) return;
+    bool rounds = logs != logs;
+#pragma unroll
+    for (int k = 0; k < K; ++k) rounds = rounds || (k < a.k && tc[k] < 0);
+    if (!rounds) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k < a.k) {
+                a.top[i * a.k + k] = (tv[k] - base) - logs;
+                a.top_index[i * a.k + k] = tc[k];
+            }
+        return;
+    }
+    u64 last = ~0ull;
+    for (int k = 0; k < a.k; ++k) {
+        u64 best = 0;
+        for (int c = 0; c < a.C; ++c) {
+            const u64 r = rank_of(Elem<T>::ld(row + c), c);
+            best = r < last && r > best ? r : best;
+        }
+        last = best;
+        a.top[i * a.k + k] = (rank_value(best) - base) - logs;
+        a.top_index[i * a.k + k] = rank_index(best);
+    }
+}
+
 struct LpBwdArgs {
     const void* z;
     const long long* target;
@@ -783,9 +855,7 @@ __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a)
     }
 }
 
-// Many rows of few classes that lie one behind the other: 256 rows are brought to LDS and back as one stretch of memory, and a thread
-// works off a row there.  Rows of an even number of classes are begun at another class in each lane, which spreads the lanes over
-// LDS's banks.
+// Many rows of few classes, brought to LDS and back as lp_rows_lds_kernel brings them there
 template <typename T, int KT>
 __global__ __launch_bounds__(256) void lp_rows_lds_bwd_kernel(const LpBwdArgs a) {
     constexpr int K = KT > 0 ? KT : 1, E = Elem<T>::EPC;
@@ -795,8 +865,7 @@ __global__ __launch_bounds__(256) void lp_rows_lds_bwd_kernel(const LpBwdArgs a)
     const int rows = (int)(a.N - first < 256 ? a.N - first : 256), count = rows * a.C;
     const T* z = (const T*)a.z + first * a.C;
     T* dz = (T*)a.dz + first * a.C;
-    for (int q = threadIdx.x; q < count / E; q += 256) stage[q] = ((const i32x4*)z)[q];
-    for (int e = count / E * E + threadIdx.x; e < count; e += 256) lds[e] = z[e];
+    rows_to_lds<T>(z, count, stage);
     float gl = 0.f, gh = 0.f, pull, base = 0.f, logs = 0.f, gk[K];
     int t = -1, jk[K];
     bool any = false;
@@ -844,7 +913,6 @@ __global__ __launch_bounds__(256) void lp_rows_lds_bwd_kernel(const LpBwdArgs a)
 // Rows by teams (4096 x 32001 bf16 86 us, 6.1 TB/s: the memory bounds it): chunks at the 16-byte boundaries as in the forward pass;
 // the target and the alternatives are written once more after the rest.  A gradient row that lies differently to the boundaries than the logits' row is stored class by class.
 #define BWD_UNROLL 4
-#define LDS_ROW 160       // bytes of a row
 template <typename T, int TEAM>
 __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     constexpr int E = Elem<T>::EPC;
@@ -986,12 +1054,12 @@ static inline int lp_segments(int dtype, long long N, int C, int k) {
 }
 
 // Rows through LDS: compact, on 16-byte boundaries, few enough classes that 4 workgroups fit a CU's LDS, enough rows to fill the chip.
-// LDS against threads or teams, us: 3145728 x 20 fp32 115 / 248, bf16 68 / 275; 1000000 x 9 18 / 30 and 13 / 18; 1000000 x 24 41 / 75 and
-// 24 / 48; with 5 alternatives 61 / 118 and 42 / 72; 65536 x 20 5.7 / 6.8 and 5.2 / 6.4.
-static inline bool lp_bwd_in_lds(const LpBwdArgs& a, int dtype, long long sc) {
-    const int size = dtype == ERF_BF16 ? 2 : 4;
-    return sc == 1 && a.sn == a.C && a.dn == a.C && !(((unsigned long long)a.z | (unsigned long long)a.dz) % 16) && a.C * size <= LDS_ROW &&
-           a.N >= (1 << 16) && a.k <= 8;
+// LDS against threads or teams, us, backward: 3145728 x 20 fp32 115 / 248, bf16 68 / 275; 1000000 x 9 18 / 30 and 13 / 18; 1000000 x 24 41
+// / 75 and 24 / 48; with 5 alternatives 61 / 118 and 42 / 72; 65536 x 20 5.7 / 6.8 and 5.2 / 6.4.  Forward, from 13 classes on: 3145728 x 20
+// 69 / 124 and 49 / 65, 1000000 x 9 14 / 13 and 12 / 13, 1000000 x 32 37 / 53 and 26 / 60; with 2 alternatives 55 / 91 and 36 / 63,
+// with 5 113 / 106 and 83 / 77.
+static inline bool lp_in_lds(int dtype, long long N, int C, long long sn, long long sc, int k, int most_k, unsigned long long addresses) {
+    return sc == 1 && sn == C && addresses % 16 == 0 && C * (dtype == ERF_BF16 ? 2 : 4) <= LDS_ROW && N >= (1 << 16) && k <= most_k;
 }
 
 // A launch has less than 2^32 threads: very many rows are several launches' work
@@ -1044,7 +1112,17 @@ int erf_class_log_probs_fwd(const void* logits, int dtype, long long N, int C, l
         return ERF_EINVAL;
     LpArgs a{logits, target, N, L, stride_n, stride_c, C, top_k, ignore_index, log_prob, entropy, stats, top_log_probs, top_indices, 1, 0, (u64*)workspace};
     hipStream_t s = (hipStream_t)stream;
-    if (stride_c == 1 && lp_fwd_team(dtype, C, top_k).team > 1) {
+    if (C > 12 && lp_in_lds(dtype, N, C, stride_n, stride_c, top_k, 2, (unsigned long long)logits)) {
+        const dim3 grid((unsigned)((N + 255) / 256)), block(256);
+        const size_t lds = (size_t)256 * C * (dtype == ERF_BF16 ? 2 : 4);
+#define LP_KT(T)                                                                                            \
+    do {                                                                                                    \
+        if (top_k == 0) hipLaunchKernelGGL((lp_rows_lds_kernel<T, 0>), grid, block, lds, s, a);             \
+        else hipLaunchKernelGGL((lp_rows_lds_kernel<T, 2>), grid, block, lds, s, a);                        \
+    } while (0)
+        if (dtype == ERF_BF16) LP_KT(bf16raw); else LP_KT(float);
+#undef LP_KT
+    } else if (stride_c == 1 && lp_fwd_team(dtype, C, top_k).team > 1) {
         a.segments = lp_segments(dtype, N, C, top_k);
         if (dtype == ERF_BF16) { if (top_k) lp_rows_launch<bf16raw, true>(a, dtype, s); else lp_rows_launch<bf16raw, false>(a, dtype, s); }
         else { if (top_k) lp_rows_launch<float, true>(a, dtype, s); else lp_rows_launch<float, false>(a, dtype, s); }
@@ -1078,7 +1156,7 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
                       g_log_prob, g_entropy, g_top, top_indices, dlogits, 0};
     hipStream_t s = (hipStream_t)stream;
-    if (lp_bwd_in_lds(a, dtype, stride_c)) {
+    if (lp_in_lds(dtype, N, C, stride_n, stride_c, a.k, 8, (unsigned long long)logits | (unsigned long long)dlogits) && dstride_n == C) {
         const dim3 grid((unsigned)((N + 255) / 256)), block(256);
         const size_t lds = (size_t)256 * C * (dtype == ERF_BF16 ? 2 : 4);
 #define LP_KT(T)                                                                                            \
