@@ -237,7 +237,7 @@ int erf_weighted_ce_bwd(const void* logits, int dtype, const long long* target, 
 /* ---- group normalisation with an activation on channels-last maps x, y [N][HW][C] (contiguous; y and dx may not alias x or dy).
  * y = act((x - mean) * rstd * gamma + beta), mean / rstd [N][groups] over HW x C / groups values (rstd = 1 / sqrt(var + eps)).
  * gamma, beta: fp32 [C] or NULL (1, 0).  bwd: dx, and dgamma / dbeta fp32 [C] (each may be NULL), from the forward pass's x, mean
- * and rstd.  workspace: erf_group_norm_workspace_bytes (0: unsupported arguments), 16-byte aligned, not shared by calls that may
+ * and rstd.  N <= 2^23, C <= 2^20, HW * C <= 2^40.  workspace: erf_group_norm_workspace_bytes (0: unsupported arguments), 16-byte aligned, not shared by calls that may
  * overlap; it need not be cleared. */
 #define ERF_ACT_NONE 0
 #define ERF_ACT_RELU 1
@@ -254,10 +254,12 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
  *   rows: L = 1, stride_c = 1 (tokens, classifier outputs, channels-last maps);  planes: stride_c >= max(L, 2) (NCHW maps).
  * All other arrays are contiguous: [N][L], and [N][k][L] for the alternatives (top_k <= min(ERF_TOP_MAX, C)).
  * fwd: log_prob = log softmax(z)[target] (0 where target == ignore_index, NaN for a target outside [0, C)); target and log_prob are
- *   both given or both NULL; entropy = -sum p log p; stats [2][N][L]: max z and log sum e^{z - max}, for bwd (NULL where none follows); alternatives in falling
- *   order of their value, equal ones by index, NaN first.
+ *   both given or both NULL; entropy = -sum p log p; stats [2][N][L]: max z and log sum e^{z - max}, for bwd (NULL where none
+ *   follows); alternatives in falling order of their value, equal ones by index, NaN first.
  * bwd: dlogits (same type, own strides, same kind of layout) = gl ([j = t] - p) - gh p (log p + entropy) + sum_k gk ([j = i_k] - p);
- *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits hold. */
+ *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits hold.  dlogits may
+ *   not alias logits.
+ * Rows further apart than C: what lies between the first and the last of them may be read, and has no effect; it is not written. */
 #define ERF_TOP_MAX 32
 /* workspace of fwd: erf_class_log_probs_workspace_bytes (0: none needed, NULL is fine), 16-byte aligned, not shared by calls that may
  * overlap; it need not be cleared. */
