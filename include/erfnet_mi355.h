@@ -237,8 +237,8 @@ int erf_weighted_ce_bwd(const void* logits, int dtype, const long long* target, 
 /* ---- group normalisation with an activation on channels-last maps x, y [N][HW][C] (contiguous; y and dx may not alias x or dy).
  * y = act((x - mean) * rstd * gamma + beta), mean / rstd [N][groups] over HW x C / groups values (rstd = 1 / sqrt(var + eps)).
  * gamma, beta: fp32 [C] or NULL (1, 0).  bwd: dx, and dgamma / dbeta fp32 [C] (each may be NULL), from the forward pass's x, mean
- * and rstd.  N <= 2^23, C <= 2^20, HW * C <= 2^40.  workspace: erf_group_norm_workspace_bytes (0: unsupported arguments), 16-byte aligned, not shared by calls that may
- * overlap; it need not be cleared. */
+ * and rstd.  N <= 2^23, C <= 2^20, HW * C <= 2^40.  workspace: erf_group_norm_workspace_bytes (0: unsupported arguments), 16-byte
+ * aligned, not shared by calls that may overlap; it need not be cleared. */
 #define ERF_ACT_NONE 0
 #define ERF_ACT_RELU 1
 #define ERF_ACT_SILU 2
