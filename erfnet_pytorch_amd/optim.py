@@ -61,8 +61,11 @@ class AdamW(torch.optim.Optimizer):
         return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed}
 
     def __setstate__(self, state):
+        # unpickling and copying start without tables; torch's load_state_dict comes here too, with an optimizer whose tables captured
+        # launches may read: load_state_dict below puts those aside
         super().__setstate__(state)
-        self._reset()
+        if "_watch" not in self.__dict__:
+            self._reset()
 
     # -- argument checks ------------------------------------------------------------------------
     def _check_group(self, group):
