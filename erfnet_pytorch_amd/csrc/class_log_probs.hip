@@ -844,6 +844,7 @@ __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a)
             if (!any[p]) continue;
             for (int k = 0; k < a.k; ++k) {
                 const long long j = a.top_index[(n * a.k + k) * a.L + l + p];
+                if (j < 0 || j >= a.C) continue;                       // no class: pull has its gradient, as in the other kernels
                 float own = j == t[p] ? gl[p] : 0.f;
                 for (int o = 0; o < a.k; ++o) {
                     const long long at = (n * a.k + o) * a.L + l + p;

@@ -1,5 +1,7 @@
 """Group norm, label log probabilities and AdamW together: as registered ops (schema, fake kernels, no CPU kernel) and as the pieces
 of one training step."""
+import math
+
 import pytest
 import torch
 
@@ -122,6 +124,38 @@ def test_opcheck_against_the_device_kernels():
         torch.library.opcheck(T.class_log_probs_fwd.default, (z, t, 3, -100), test_utils=checks)
         lp, ent, st, top, idx = T.class_log_probs_fwd(z, t, 3, -100)
         torch.library.opcheck(T.class_log_probs_bwd.default, (z, t, st, ent, idx, lp, ent, top, -100), test_utils=checks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 40, 5, 7), (50, 12), (50, 100), (9, 1200), (66000, 20), (2, 40, 4, 6)])
+@pytest.mark.parametrize("k", [4, 12])
+def test_alternatives_outside_the_classes_have_no_class_of_their_own(shape, k):
+    """dz_j = gl ([j = t] - p) + sum_k gk ([j = i_k] - p): such a k gives -p gk alone, in every plan, and nothing beside dz is written.
+    Zero logits: p = 1 / C.  Their stats are set here (0, and log C rounded once), so a term's only errors are the exponential's
+    (|log p| 3 U + 4 U) p, and one rounding per addition: k + 3 of them."""
+    n, c = shape[:2]
+    last = shape == (2, 40, 4, 6)
+    z = torch.zeros(shape, device="cuda")
+    z = z.contiguous(memory_format=torch.channels_last) if last else z
+    pos = (n, *shape[2:])
+    gen = torch.Generator().manual_seed(5)
+    t = torch.randint(0, c, pos, generator=gen)
+    gl, gk = torch.randn(pos, generator=gen), torch.randn((n, k, *shape[2:]), generator=gen)
+    index = torch.randint(0, c, gk.shape, generator=gen)
+    for value, place in ((-1, 1), (c, 2), (2 ** 40, 3), (-2 ** 40, 0)):
+        index[:, place] = value
+    stats = torch.stack([torch.zeros(pos), torch.full(pos, float(c)).log()])
+    dz = T.class_log_probs_bwd(z, t.cuda(), stats.cuda(), torch.zeros(pos, device="cuda"), index.cuda(), gl.cuda(), None, gk.cuda(), -100)
+    rows = lambda x: x.movedim(1, -1).reshape(-1, x.shape[1])                                                      # noqa: E731
+    want, size = torch.zeros(t.numel(), c, dtype=torch.float64), torch.zeros(t.numel(), c, dtype=torch.float64)
+    own = torch.cat([gl.reshape(-1, 1), rows(gk)], 1).double()
+    at = torch.cat([t.reshape(-1, 1), rows(index)], 1)
+    live = (at >= 0) & (at < c)
+    want.scatter_add_(1, torch.where(live, at, 0), torch.where(live, own, 0.0))
+    size.scatter_add_(1, torch.where(live, at, 0), torch.where(live, own.abs(), 0.0))
+    want, size = want - own.sum(1, keepdim=True) / c, size + own.abs().sum(1, keepdim=True) / c
+    assert dz.is_contiguous(memory_format=torch.channels_last) if last else dz.is_contiguous()
+    assert ((rows(dz).cpu().double() - want).abs() <= (k + 3 + 4 + 3 * math.log(c)) * U * size).all()
 
 
 def _step_reference(x, params, t, groups):
