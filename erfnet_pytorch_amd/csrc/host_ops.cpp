@@ -360,7 +360,9 @@ static std::tuple<Tensor, Tensor, Tensor, Tensor> class_log_probs(const Tensor& 
 // the present; it keeps no gradient alive.
 struct ParamWatch {
     struct Entry { const void *param, *grad; bool on, copied; at::ScalarType type; at::DimVector shape; };          // shape: sizes, then strides
+    struct Move { size_t at; const void* grad; bool copied; };
     std::vector<Entry> entries;
+    std::vector<Move> moves;                    // of the present look
     std::vector<Tensor> params;                 // those with a gradient, in the order of the groups
 
     static const Tensor& tensor(PyObject* o) {
@@ -382,27 +384,31 @@ struct ParamWatch {
 
     // 0: all as before; 1: the same parameters, gradients elsewhere (noted); 2: other parameters, or parameters elsewhere.
     // A gradient whose strides are not its parameter's counts as elsewhere every time: it is copied into the parameter's order.
+    // Nothing is noted before every gradient has been checked: after a refusal the next look finds the same changes.
     int look(const std::vector<py::list>& groups) {
         size_t i = 0;
-        bool moved = false;
+        moves.clear();
         for (const py::list& group : groups)
             for (py::handle h : group) {
                 const Tensor& p = tensor(h.ptr());
                 const Tensor& g = p.grad();
                 const bool on = g.defined() && p.numel();
                 if (i >= entries.size()) return 2;
-                Entry& e = entries[i++];
+                const Entry& e = entries[i++];
                 if (on != e.on) return 2;
                 if (!on) continue;
                 if (p.data_ptr() != e.param || p.scalar_type() != e.type || !same_shape(p, e)) return 2;
                 const bool strided = g.layout() == at::kStrided;
                 if (strided && g.data_ptr() == e.grad && g.sizes() == p.sizes() && g.strides() == p.strides() && g.scalar_type() == e.type && !e.copied) continue;
                 check_grad(p, g);
-                e.grad = g.data_ptr();
-                e.copied = g.strides() != p.strides() && !(g.is_contiguous() && p.is_contiguous());
-                moved = true;
+                moves.push_back({i - 1, g.data_ptr(), g.strides() != p.strides() && !(g.is_contiguous() && p.is_contiguous())});
             }
-        return i != entries.size() ? 2 : moved ? 1 : 0;
+        if (i != entries.size()) return 2;
+        for (const Move& m : moves) {
+            entries[m.at].grad = m.grad;
+            entries[m.at].copied = m.copied;
+        }
+        return moves.empty() ? 0 : 1;
     }
 
     // Takes the parameters as they are; look() then reports the gradients as moved once

@@ -39,6 +39,7 @@ class _Plan:
         self.device, self.code = device, code
         self.params, self.bases, self.which = [], [], []        # which: places among all parameters with a gradient
         self.captured = False                           # a captured launch may write the grad fields at any time
+        self.stale = True                               # the table lacks the gradients' present addresses
 
 
 class AdamW(torch.optim.Optimizer):
@@ -54,6 +55,7 @@ class AdamW(torch.optim.Optimizer):
         self._lr = []                                   # per group: [value on the devices, {device: double tensor}]
         self._kept = []                                 # what captured launches still read
         self._copies, self._copies_captured = {}, False
+        self._moved = False                             # gradients moved, and the copies' places do not follow yet
         self._watch = _host.ParamWatch()
 
     def __getstate__(self):
@@ -82,6 +84,14 @@ class AdamW(torch.optim.Optimizer):
         if not 0.0 <= group["weight_decay"] < float("inf"):
             raise ValueError(f"invalid weight decay {group['weight_decay']}")
         self._check_params(group["params"])
+
+    @staticmethod
+    def _settings(group):
+        """The group's numbers as a launch takes them; they may have been changed by hand."""
+        b1, b2, eps = float(group["betas"][0]), float(group["betas"][1]), float(group["eps"])
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
+            raise ValueError(f"betas lie in [0, 1) and eps is not negative, got {group['betas']} and {group['eps']}")
+        return b1, b2, eps, float(group["weight_decay"])
 
     @staticmethod
     def _check_params(params):
@@ -257,14 +267,26 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        settings = [self._settings(g) for g in self.param_groups]              # a refused step updates no group
         groups = [g["params"] for g in self.param_groups]
         seen = 2 if self._plans is None else self._watch.look(groups)
-        if seen:
+        if seen == 2:
             with torch.no_grad():
-                if seen == 2:
-                    self._build(groups)
-                    self._watch.look(groups)
+                self._build(groups)
+            try:
+                self._watch.look(groups)
+            except BaseException:
+                self._plans = None
+                raise
+        if seen:
+            self._moved = True                          # until the copies have their places, and each table its addresses
+            for plans in self._plans:
+                for plan in plans:
+                    plan.stale = True
+        if self._moved:
+            with torch.no_grad():
                 self._copy_places()
+            self._moved = False
         if not any(self._plans):
             return loss
         capturing = torch.cuda.is_current_stream_capturing()
@@ -274,13 +296,13 @@ class AdamW(torch.optim.Optimizer):
                 for own, p in self._copies.values():
                     own.copy_(p.grad)
         self.refresh_lr()
-        for group, where, plans in zip(self.param_groups, self._lr, self._plans):
+        for numbers, where, plans in zip(settings, self._lr, self._plans):
             for plan in plans:
                 if plan.device.index == torch._C._cuda_getDevice():
-                    self._launch(group, where[1][plan.device], plan, seen, capturing)
+                    self._launch(numbers, where[1][plan.device], plan, capturing)
                 else:
                     with torch.cuda.device(plan.device):
-                        self._launch(group, where[1][plan.device], plan, seen, capturing)
+                        self._launch(numbers, where[1][plan.device], plan, capturing)
         self._watch.bump()
         ops.bump_param_epoch()                          # the parameters changed through raw pointers
         return loss
@@ -294,15 +316,16 @@ class AdamW(torch.optim.Optimizer):
 
     step.hooked = True                                  # torch's wrapper (hooks and a profiler range, 8 us) is used where a hook asks for it
 
-    def _launch(self, group, lr, plan, seen, capturing):
+    def _launch(self, numbers, lr, plan, capturing):
         stream = ops._stream()
         table = plan.table.data_ptr()
-        if seen or plan.captured or capturing:
-            self._watch.set_grads(table, plan.which, plan.copies, stream)
+        if plan.stale or plan.captured or capturing:
             plan.captured = plan.captured or capturing
-        b1, b2 = group["betas"]
+            self._watch.set_grads(table, plan.which, plan.copies, stream)
+            if not capturing:                           # a captured launch writes its addresses when it is replayed
+                plan.stale = False
         call("erf_adamw_step", table, plan.chunks.data_ptr(), plan.steps.data_ptr(), plan.chunks.shape[0], lr.data_ptr(),
-             b1, b2, group["eps"], group["weight_decay"], plan.code, self.state_bits, self.seed, stream)
+             *numbers, plan.code, self.state_bits, self.seed, stream)
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

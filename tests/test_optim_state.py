@@ -3,6 +3,7 @@ not reach a table are sent again.  Tables are stand-ins here; the launches thems
 import copy
 
 import numpy as np
+import pytest
 import torch
 
 from erfnet_pytorch_amd import optim
@@ -46,3 +47,120 @@ def test_copies_start_without_tables():
     q, = other.param_groups[0]["params"]
     assert other._plans is None and other._kept == [] and other._lr == [] and other._copies == {} and opt._plans == [[plan]]
     assert float(other.state[q]["step"]) == 3
+
+
+def test_a_look_that_refuses_a_gradient_notes_none():
+    a, b = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    a.grad, b.grad = torch.zeros(3), torch.zeros(3)
+    w = optim._host.ParamWatch()
+    w.bind([[a, b]])
+    assert [w.look([[a, b]]) for _ in range(2)] == [1, 0]
+    old, a.grad = (a.grad, b.grad), torch.zeros(3)
+    b.grad = torch.sparse_coo_tensor(torch.tensor([[0]]), torch.tensor([1.0]), (3,))
+    with pytest.raises(ValueError, match="gradient"):
+        w.look([[a, b]])
+    b.grad = old[1]
+    assert [w.look([[a, b]]) for _ in range(2)] == [1, 0]               # a's is noted now
+
+
+class _Recorder:
+    """The launches of an optimizer, in place of the device: (addresses sent to a table, step launched), in order."""
+
+    def __init__(self, monkeypatch, opt):
+        self.sent, self.steps, self.fail_step = [], [], None
+        recorder = self
+
+        class Watch:
+            def __init__(self):
+                self.w = optim._host.ParamWatch()
+
+            def __getattr__(self, name):
+                return getattr(self.w, name)
+
+            def set_grads(self, table, which, copies, stream):
+                recorder.sent.append(table)
+        opt._watch = Watch()
+
+        def call(name, table, chunks, steps, n, lr, *rest):
+            assert name == "erf_adamw_step"
+            if recorder.fail_step == len(recorder.steps):
+                recorder.fail_step = None
+                raise RuntimeError("refused")
+            recorder.steps.append(table)
+        monkeypatch.setattr(optim, "call", call)
+        monkeypatch.setattr(optim.ops, "require_gpu", lambda *a: None)
+        monkeypatch.setattr(optim.ops, "_stream", lambda: 0)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: None, raising=False)                # a CPU device has index None
+
+
+def _two_groups(monkeypatch):
+    a, b = (torch.nn.Parameter(torch.ones(5)) for _ in range(2))
+    opt = optim.AdamW([{"params": [a]}, {"params": [b]}])
+    a.grad, b.grad = torch.zeros(5), torch.zeros(5)
+    return opt, a, b, _Recorder(monkeypatch, opt)
+
+
+def test_a_refused_launch_leaves_the_later_tables_to_be_filled(monkeypatch):
+    opt, a, b, rec = _two_groups(monkeypatch)
+    rec.fail_step = 0
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    tables = [plans[0].table.data_ptr() for plans in opt._plans]
+    assert rec.steps == [] and tables[1] not in rec.sent
+    opt.step()
+    assert rec.steps == tables and tables[1] in rec.sent
+    rec.sent.clear()
+    opt.step()
+    assert rec.sent == [] and rec.steps == 2 * tables                   # nothing moved
+    a.grad = torch.zeros(5)
+    rec.fail_step = len(rec.steps)
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    opt.step()
+    assert tables[0] in rec.sent and tables[1] in rec.sent
+
+
+def test_a_learning_rate_that_is_refused_leaves_the_tables_to_be_filled(monkeypatch):
+    opt, a, b, rec = _two_groups(monkeypatch)
+    opt.step()
+    rec.sent.clear()
+    a.grad = torch.zeros(5)
+    opt.param_groups[1]["lr"] = "fast"
+    with pytest.raises(ValueError):
+        opt.step()
+    opt.param_groups[1]["lr"] = 1e-3
+    opt.step()
+    assert set(rec.sent) == {plans[0].table.data_ptr() for plans in opt._plans}
+
+
+@pytest.mark.parametrize("key,value", [("betas", (0.9, 1.0)), ("eps", -1.0), ("eps", float("nan")), ("weight_decay", "much")])
+def test_settings_that_are_refused_update_no_group(monkeypatch, key, value):
+    opt, a, b, rec = _two_groups(monkeypatch)
+    good, opt.param_groups[1][key] = opt.param_groups[1][key], value
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            opt.step()
+    assert rec.steps == [] and a._version == 0
+    opt.param_groups[1][key] = good
+    opt.step()
+    tables = [plans[0].table.data_ptr() for plans in opt._plans]
+    assert rec.steps == tables and set(rec.sent) == set(tables) and a._version == 1
+
+
+def test_places_for_copies_that_could_not_be_made_are_made_by_the_next_step(monkeypatch):
+    p = torch.nn.Parameter(torch.ones(4, 5))
+    opt = optim.AdamW([p])
+    p.grad = torch.zeros(4, 5)
+    rec = _Recorder(monkeypatch, opt)
+    opt.step()
+    p.grad = torch.zeros(5, 4).t()
+    with monkeypatch.context() as m:
+        def full(*a, **k):
+            raise torch.OutOfMemoryError("full")
+        m.setattr(torch, "empty_like", full)
+        with pytest.raises(torch.OutOfMemoryError):
+            opt.step()
+    opt.step()
+    plan, = opt._plans[0]
+    assert len(opt._copies) == 1 and plan.copies == [opt._copies[0][0].data_ptr()] and rec.sent[-1] == plan.table.data_ptr()
