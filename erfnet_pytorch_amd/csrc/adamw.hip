@@ -252,6 +252,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
     constexpr int PER_WAVE = CHUNK / QB / 4;
     const int2 ch = a.chunks[blockIdx.x];
     const erf_adamw_tensor t = a.table[ch.x];
+    if (!t.grad) return;                                      // the whole workgroup: no gradient, no step of this tensor
     const int step = a.steps[blockIdx.x] + 1;
     const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const long long start = (long long)ch.y * CHUNK;
@@ -321,10 +322,7 @@ int erf_adamw_set_grads(erf_adamw_tensor* table, const void* const* grads, int c
     for (int i = 0; i < count; i += GRADS_PER_LAUNCH) {
         const int n = count - i < GRADS_PER_LAUNCH ? count - i : GRADS_PER_LAUNCH;
         AdamwGrads a = {};
-        for (int k = 0; k < n; ++k) {
-            if (!grads[i + k]) return ERF_EINVAL;
-            a.g[k] = grads[i + k];
-        }
+        for (int k = 0; k < n; ++k) a.g[k] = grads[i + k];
         hipLaunchKernelGGL(adamw_grads_kernel, dim3(1), dim3(GRADS_PER_LAUNCH), 0, (hipStream_t)stream, table + i, n, a);
     }
     return erf_check_launch();

@@ -356,14 +356,19 @@ static std::tuple<Tensor, Tensor, Tensor, Tensor> class_log_probs(const Tensor& 
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW's parameters
-// What the device tables of an optimizer describe: which parameters have a gradient, and where both lie.  look() compares that with
+// What the device tables of an optimizer describe: which parameters they hold, which of these have a gradient, and where both lie.  look() compares that with
 // the present; it keeps no gradient alive.
 struct ParamWatch {
-    struct Entry { const void *param, *grad; bool on, copied; at::ScalarType type; at::DimVector shape; };          // shape: sizes, then strides
+    struct Entry {
+        const void *param, *grad;
+        bool on, has, copied;                   // in a table; with a gradient, which is copied
+        at::ScalarType type;
+        at::DimVector shape;                    // sizes, then strides
+    };
     struct Move { size_t at; const void* grad; bool copied; };
     std::vector<Entry> entries;
     std::vector<Move> moves;                    // of the present look
-    std::vector<Tensor> params;                 // those with a gradient, in the order of the groups
+    std::vector<Tensor> params;                 // those in tables, in the order of the groups
 
     static const Tensor& tensor(PyObject* o) {
         TORCH_CHECK_TYPE(THPVariable_Check(o), "AdamW: parameters are tensors");
@@ -382,7 +387,8 @@ struct ParamWatch {
         return seen.size() == 2 * d && p.sizes() == seen.slice(0, d) && p.strides() == seen.slice(d);
     }
 
-    // 0: all as before; 1: the same parameters, gradients elsewhere (noted); 2: other parameters, or parameters elsewhere.
+    // 0: all as before; 1: the same parameters, gradients elsewhere, come or gone (noted); 2: other parameters, parameters elsewhere, or
+    // a gradient of one that is in no table.
     // A gradient whose strides are not its parameter's counts as elsewhere every time: it is copied into the parameter's order.
     // Nothing is noted before every gradient has been checked: after a refusal the next look finds the same changes.
     int look(const std::vector<py::list>& groups) {
@@ -392,12 +398,17 @@ struct ParamWatch {
             for (py::handle h : group) {
                 const Tensor& p = tensor(h.ptr());
                 const Tensor& g = p.grad();
-                const bool on = g.defined() && p.numel();
                 if (i >= entries.size()) return 2;
                 const Entry& e = entries[i++];
-                if (on != e.on) return 2;
-                if (!on) continue;
+                if (!e.on) {
+                    if (g.defined() && p.numel()) return 2;
+                    continue;
+                }
                 if (p.data_ptr() != e.param || p.scalar_type() != e.type || !same_shape(p, e)) return 2;
+                if (!g.defined()) {
+                    if (e.has) moves.push_back({i - 1, nullptr, false});
+                    continue;
+                }
                 const bool strided = g.layout() == at::kStrided;
                 if (strided && g.data_ptr() == e.grad && g.sizes() == p.sizes() && g.strides() == p.strides() && g.scalar_type() == e.type && !e.copied) continue;
                 check_grad(p, g);
@@ -406,33 +417,46 @@ struct ParamWatch {
         if (i != entries.size()) return 2;
         for (const Move& m : moves) {
             entries[m.at].grad = m.grad;
+            entries[m.at].has = m.grad != nullptr;
             entries[m.at].copied = m.copied;
         }
         return moves.empty() ? 0 : 1;
     }
 
-    // Takes the parameters as they are; look() then reports the gradients as moved once
-    void bind(const std::vector<py::list>& groups) {
+    // Takes the parameters as they are: those with a gradient, and those whose places among all parameters `more` names, are in the
+    // tables.  look() then reports the gradients as moved once.
+    void bind(const std::vector<py::list>& groups, const std::vector<int64_t>& more) {
         entries.clear();
         params.clear();
+        auto next = more.begin();
         for (const py::list& group : groups)
             for (py::handle h : group) {
                 const Tensor& p = tensor(h.ptr());
-                const bool on = p.grad().defined() && p.numel();
-                if (on) check_grad(p, p.grad());
-                entries.push_back({on ? p.data_ptr() : nullptr, nullptr, on, false, p.scalar_type(), at::DimVector(p.sizes())});
+                const bool named = next != more.end() && *next == (int64_t)entries.size();
+                if (named) ++next;
+                const bool on = (p.grad().defined() || named) && p.numel();
+                if (on && p.grad().defined()) check_grad(p, p.grad());
+                entries.push_back({on ? p.data_ptr() : nullptr, nullptr, on, on && p.grad().defined(), false, p.scalar_type(), at::DimVector(p.sizes())});
                 entries.back().shape.append(p.strides().begin(), p.strides().end());
                 if (on) params.push_back(p);
             }
     }
 
-    // The gradients' addresses are written to the table records of one launch; which: places among the parameters with a gradient
+    // The gradients' addresses, NULL for none, are written to the table records of one launch; which: places among the parameters in tables
     void set_grads(int64_t table, const std::vector<int>& which, const std::vector<int64_t>& copies, int64_t stream) const {
         std::vector<const void*> at, all;
         for (const Entry& e : entries)
             if (e.on) all.push_back(e.grad);
         for (size_t i = 0; i < which.size(); ++i) at.push_back(copies[i] ? (const void*)copies[i] : all.at(which[i]));
         check_status(erf_adamw_set_grads((erf_adamw_tensor*)table, at.data(), (int)at.size(), (void*)stream), "erf_adamw_set_grads");
+    }
+
+    // Which of them have a gradient
+    std::vector<bool> present() const {
+        std::vector<bool> r;
+        for (const Entry& e : entries)
+            if (e.on) r.push_back(e.has);
+        return r;
     }
 
     // Places of the gradients that need a copy in their parameter's order
@@ -447,9 +471,14 @@ struct ParamWatch {
         return r;
     }
 
-    // The parameters changed through their addresses
+    // The parameters with a gradient changed through their addresses
     void bump() {
-        for (Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+        size_t i = 0;
+        for (const Entry& e : entries)
+            if (e.on) {
+                if (e.has) params[i].unsafeGetTensorImpl()->bump_version();
+                ++i;
+            }
     }
 };
 
@@ -536,7 +565,8 @@ PYBIND11_MODULE(_host, m) {
     py::class_<ParamWatch>(m, "ParamWatch")
         .def(py::init<>())
         .def("look", wrap_pybind_function(&ParamWatch::look))
-        .def("bind", wrap_pybind_function(&ParamWatch::bind))
+        .def("bind", wrap_pybind_function(&ParamWatch::bind), py::arg("groups"), py::arg("more") = std::vector<int64_t>())
+        .def("present", wrap_pybind_function(&ParamWatch::present))
         .def("set_grads", wrap_pybind_function(&ParamWatch::set_grads))
         .def("copied", wrap_pybind_function(&ParamWatch::copied))
         .def("bump", wrap_pybind_function(&ParamWatch::bump));

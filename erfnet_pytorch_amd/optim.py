@@ -33,11 +33,13 @@ from .train_ops import _host
 
 
 class _Plan:
-    """The device tables of one launch: parameters of one group, device and type that have a gradient."""
+    """The device tables of one launch: parameters of one group, device and type.  A parameter comes in with its first gradient and
+    stays; where it has none its address is NULL and the launch leaves it alone, so its step count is in one place for all launches."""
 
-    def __init__(self, device, code):
-        self.device, self.code = device, code
-        self.params, self.bases, self.which = [], [], []        # which: places among all parameters with a gradient
+    def __init__(self, group, device, code):
+        self.group, self.device, self.code = group, device, code
+        self.params, self.bases, self.which = [], [], []        # which: places among all parameters in tables
+        self.live = True                                # one of them has a gradient
         self.captured = False                           # a captured launch may write the grad fields at any time
         self.stale = True                               # the table lacks the gradients' present addresses
 
@@ -183,42 +185,73 @@ class AdamW(torch.optim.Optimizer):
         if live and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the first step with these parameters builds device tables and cannot be captured: "
                                "run one step before the capture")
+        known = [plan for plans in self._plans or () for plan in plans] + [k for k in self._kept if isinstance(k, _Plan)] if live else []
+        known = {id(p): (p.device, plan.code) for plan in known for p in plan.params}
         self._drop_plans()
-        chunk, block = size_query("erf_adamw_chunk_elements"), size_query("erf_adamw_scale_block")
-        plans, base, place = [], 0, 0
-        for group in groups:
-            mine = {}
+
+        def held(p):                                    # with a gradient, or as it was in a table before
+            return p.numel() and (p.grad is not None or (known.get(id(p)) == (p.device, _code(p)) and _dense(p)))
+        _host.adamw_no_overlap(live)
+        try:
+            _host.adamw_no_overlap([p for g in groups for p in g if held(p)])
+        except ValueError:                              # with one that has no gradient now
+            known = {}
+        block = size_query("erf_adamw_scale_block")
+        plans, more, base, place, at = [], [], 0, 0, 0
+        for number, group in enumerate(groups):
+            rows = {}                                   # per device and type: parameter -> (random base, place)
             for p in group:
-                if p.grad is not None and p.numel():
-                    key = (p.device, F32 if p.dtype == torch.float32 else BF16)
-                    plan = mine.get(key)
-                    if plan is None:
-                        plan = mine[key] = _Plan(*key)
-                    plan.params.append(p)
-                    plan.bases.append(base)
-                    plan.which.append(place)
+                if held(p):
+                    if p.grad is None:
+                        more.append(at)
+                    rows.setdefault((p.device, _code(p)), {})[p] = (base, place)
                     place += 1
                 base += -(-p.numel() // block) * block
-            plans.append(list(mine.values()))
-        _host.adamw_no_overlap(live)
-        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
-        for ps in plans:
-            for plan in ps:
-                states = [self._state_of(p) for p in plan.params]
-                try:
-                    states, steps = [[st[k] for k in names] for st in states], np.array([int(st["step"]) for st in states], dtype=np.int32)
-                except KeyError as e:
-                    raise ValueError(f"AdamW: a parameter's state lacks {e} (state_bits={self.state_bits})") from None
-                rows, plan.holds = _host.adamw_table(plan.params, states, plan.bases)
-                per = -(-rows[:, 6].numpy() // chunk)   # chunks of each tensor
-                plan.first_chunk = np.cumsum(per) - per
-                which = np.repeat(np.arange(len(per)), per)
-                where = np.stack([which, np.arange(len(which)) - plan.first_chunk[which]], 1).astype(np.int32)
-                plan.table = rows.to(plan.device)
-                plan.chunks = torch.from_numpy(where).to(plan.device)
-                plan.steps = torch.from_numpy(steps[which]).to(plan.device)
-        self._watch.bind(groups)
+                at += 1
+            plans.append([plan for key, mine in rows.items() for plan in self._tables(number, *key, mine)])
+        self._watch.bind(groups, more)
         self._plans = plans
+        self._kept = [k for k in self._kept if not any(k is plan for ps in plans for plan in ps)]
+
+    def _tables(self, number, device, code, mine):
+        """Plans for these parameters.  Captured ones that describe some of them as they are now are taken up again, with the counts of
+        `state`: a captured launch and the next step then move the same counts.  The rest come into one new plan."""
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
+        chunk = size_query("erf_adamw_chunk_elements")
+
+        def describe(params):
+            states = [self._state_of(p) for p in params]
+            try:
+                states, steps = [[st[k] for k in names] for st in states], np.array([int(st["step"]) for st in states], dtype=np.int32)
+            except KeyError as e:
+                raise ValueError(f"AdamW: a parameter's state lacks {e} (state_bits={self.state_bits})") from None
+            rows, holds = _host.adamw_table(params, states, [mine[p][0] for p in params])
+            return rows, holds, steps
+        plans, rest = [], dict(mine)
+        for plan in reversed([k for k in self._kept if isinstance(k, _Plan)]):
+            if (plan.group, plan.device, plan.code) != (number, device, code) or any(p not in rest for p in plan.params):
+                continue
+            rows, _, steps = describe(plan.params)
+            if not torch.equal(rows, plan.rows):
+                continue
+            plan.steps.copy_(torch.from_numpy(steps[plan.owner]))
+            plan.which, plan.stale = [mine[p][1] for p in plan.params], True
+            plans.append(plan)
+            for p in plan.params:
+                del rest[p]
+        if rest:
+            plan = _Plan(number, device, code)
+            plan.params, plan.bases, plan.which = list(rest), [b for b, _ in rest.values()], [w for _, w in rest.values()]
+            plan.rows, plan.holds, steps = describe(plan.params)
+            per = -(-plan.rows[:, 6].numpy() // chunk)  # chunks of each tensor
+            plan.first_chunk = np.cumsum(per) - per
+            plan.owner = np.repeat(np.arange(len(per)), per)
+            where = np.stack([plan.owner, np.arange(len(plan.owner)) - plan.first_chunk[plan.owner]], 1).astype(np.int32)
+            plan.table = plan.rows.to(device)
+            plan.chunks = torch.from_numpy(where).to(device)
+            plan.steps = torch.from_numpy(steps[plan.owner]).to(device)
+            plans.append(plan)
+        return plans
 
     def _copy_places(self):
         """Gradients with other strides than their parameter's are copied into its order every step; where the copies lie."""
@@ -280,14 +313,15 @@ class AdamW(torch.optim.Optimizer):
                 raise
         if seen:
             self._moved = True                          # until the copies have their places, and each table its addresses
+            present = self._watch.present()
             for plans in self._plans:
                 for plan in plans:
-                    plan.stale = True
+                    plan.stale, plan.live = True, any(present[i] for i in plan.which)
         if self._moved:
             with torch.no_grad():
                 self._copy_places()
             self._moved = False
-        if not any(self._plans):
+        if not any(plan.live for plans in self._plans for plan in plans):
             return loss
         capturing = torch.cuda.is_current_stream_capturing()
         if self._copies:
@@ -298,6 +332,8 @@ class AdamW(torch.optim.Optimizer):
         self.refresh_lr()
         for numbers, where, plans in zip(settings, self._lr, self._plans):
             for plan in plans:
+                if not plan.live:
+                    continue
                 if plan.device.index == torch._C._cuda_getDevice():
                     self._launch(numbers, where[1][plan.device], plan, capturing)
                 else:
@@ -329,6 +365,10 @@ class AdamW(torch.optim.Optimizer):
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
+
+
+def _code(t):
+    return {torch.float32: F32, torch.bfloat16: BF16}.get(t.dtype)
 
 
 def _dense(t):

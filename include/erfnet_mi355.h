@@ -282,6 +282,7 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
  *   rounded up or down at random: the bits come from (seed, step, base + element) alone, so a run can be repeated.
  * chunks: device int pairs (tensor, chunk), every chunk of erf_adamw_chunk_elements() elements of every tensor exactly once;
  * steps: device int per chunk, the steps taken so far; each launch adds 1.  lr: device double.
+ * A tensor whose grad is NULL takes no step: its values, moments and counts stay as they are.
  * Tensors of one launch must not overlap.
  * erf_adamw_set_grads writes the grad fields of records 0..count-1; grads: HOST array, read before the call returns. */
 typedef struct {

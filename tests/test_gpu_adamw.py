@@ -565,3 +565,71 @@ def test_gradients_made_inside_the_capture_and_another_stream():
         torch.cuda.synchronize()
         one(q, qo)
         assert torch.equal(p.detach(), q.detach())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_between_steps_with_other_gradients_count_on(bits):
+    """Eager steps without one of the captured step's gradients, without any, and with one more, between its replays: the bits and the
+    counts of launched steps."""
+    def run(graphed):
+        ps = [torch.nn.Parameter(p) for p, _ in _tensors([300, 9000, 77], torch.float32, 41)]
+        opt = _adamw(ps, lr=1e-3, state_bits=bits)
+        static = [torch.zeros_like(p) for p in ps]
+
+        def fill(k, which):
+            for i, (p, s) in enumerate(zip(ps, static)):
+                s.copy_(torch.cos(torch.arange(s.numel(), device="cuda") * (k + 0.5) + i))
+                p.grad = s if i in which else None
+        fill(0, (0, 1))
+        opt.step()
+        graph = torch.cuda.CUDAGraph()
+        if graphed:
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+                opt.step()
+
+        def go(k):
+            fill(k, (0, 1))
+            if graphed:
+                graph.replay()
+                opt.note_replay()
+            else:
+                opt.step()
+            torch.cuda.synchronize()
+        go(1)
+        for k, which in enumerate(((0,), (), (1,), (0, 2), (2,), (0, 1, 2))):
+            fill(10 + k, which)
+            opt.step()
+            go(20 + 2 * k)
+            go(21 + 2 * k)
+        return [p.detach().clone() for p in ps], [float(s["step"]) for s in opt.state_dict()["state"].values()], \
+            [v for p in ps for k, v in opt.state[p].items() if k != "step"]
+    (a, ca, sa), (b, cb, sb) = run(False), run(True)
+    assert ca == cb == [17.0, 16.0, 3.0] and all(torch.equal(x, y) for x, y in zip(a, b))
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(sa, sb))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_without_a_gradient_is_left_alone(bits):
+    """Its address in the table is NULL: values, moments and count stay, and it goes on where it was."""
+    ps = [torch.nn.Parameter(p) for p, _ in _tensors([5000, 5000], torch.float32, 51)]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt, other = _adamw(ps, lr=LR, state_bits=bits), _adamw(qs[:1], lr=LR, state_bits=bits)
+
+    def mine():
+        return [ps[0].detach()] + [v for k, v in opt.state[ps[0]].items() if k != "step"]
+    for k in range(4):
+        g = torch.cos(torch.arange(5000, device="cuda") * (k + 1.5))
+        ps[0].grad, ps[1].grad = (g if k != 2 else None), g
+        if k == 2:
+            before = [t.clone() for t in mine()]
+        opt.step()
+        if k == 2:
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(before, mine()))
+            continue
+        qs[0].grad = g
+        other.step()
+    assert torch.equal(ps[0].detach(), qs[0].detach())
+    assert [float(opt.state_dict()["state"][i]["step"]) for i in (0, 1)] == [3, 4]

@@ -14,7 +14,7 @@ def _with_plan(captured):
     p = torch.nn.Parameter(torch.ones(6))
     opt = optim.AdamW([p], lr=1e-2)
     opt.state[p].update(step=torch.zeros(()), exp_avg=torch.zeros(6), exp_avg_sq=torch.zeros(6))
-    plan = optim._Plan(p.device, 0)
+    plan = optim._Plan(0, p.device, 0)
     plan.params, plan.first_chunk, plan.steps, plan.captured = [p], np.array([0]), torch.tensor([3], dtype=torch.int32), captured
     opt._plans = [[plan]]
     opt._lr = [[1e-2, {p.device: torch.full((1,), 1e-2, dtype=torch.float64)}]]
@@ -164,3 +164,89 @@ def test_places_for_copies_that_could_not_be_made_are_made_by_the_next_step(monk
     opt.step()
     plan, = opt._plans[0]
     assert len(opt._copies) == 1 and plan.copies == [opt._copies[0][0].data_ptr()] and rec.sent[-1] == plan.table.data_ptr()
+
+
+# ------------------------------------------------------------------------------------------------ gradients that come and go
+def test_the_watch_tells_gradients_that_come_and_go():
+    ps = [torch.nn.Parameter(torch.zeros(3)) for _ in range(4)]
+    ps[0].grad, ps[1].grad = torch.zeros(3), torch.zeros(3)
+    w = optim._host.ParamWatch()
+    w.bind([ps[:2], ps[2:]], [2])                                       # the third is in the tables without a gradient
+    assert w.present() == [True, True, False] and [w.look([ps]) for _ in range(2)] == [1, 0]
+    old, ps[1].grad = ps[1].grad, None
+    assert [w.look([ps]) for _ in range(2)] == [1, 0] and w.present() == [True, False, False]
+    before = [p._version for p in ps]
+    w.bump()
+    assert [p._version - b for p, b in zip(ps, before)] == [1, 0, 0, 0]
+    ps[1].grad, ps[2].grad = old, torch.zeros(3)
+    assert [w.look([ps]) for _ in range(2)] == [1, 0] and w.present() == [True, True, True]
+    ps[2].grad = torch.zeros(6)[::2]
+    assert w.look([ps]) == 1 and w.copied() == [2]
+    ps[2].grad = None
+    assert [w.look([ps]) for _ in range(2)] == [1, 0] and w.copied() == []
+    ps[3].grad = torch.zeros(3)
+    assert w.look([ps]) == 2
+
+
+def _three(monkeypatch):
+    ps = [torch.nn.Parameter(torch.ones(n)) for n in (5, 9000, 7)]
+    opt = optim.AdamW(ps)
+    ps[0].grad, ps[1].grad = (torch.zeros_like(p) for p in ps[:2])
+    rec = _Recorder(monkeypatch, opt)
+    opt.step()
+    return opt, ps, rec, opt._plans[0][0]
+
+
+def test_gradients_that_come_and_go_leave_the_tables_in_place(monkeypatch):
+    opt, ps, rec, plan = _three(monkeypatch)
+    for gone in ([1], [0, 1], [0], []):
+        for i in (0, 1):
+            ps[i].grad = None if i in gone else torch.zeros_like(ps[i])
+        n = len(rec.steps)
+        opt.step()
+        assert opt._plans == [[plan]] and len(rec.steps) - n == (len(gone) < 2)
+
+
+def test_a_first_gradient_beside_a_captured_table_gets_a_table_of_its_own(monkeypatch):
+    opt, ps, rec, plan = _three(monkeypatch)
+    plan.captured = True
+    plan.steps += torch.tensor([1, 4, 4, 4], dtype=torch.int32)         # what launches would count
+    ps[0].grad = None
+    ps[2].grad = torch.zeros_like(ps[2])
+    opt.step()
+    assert len(opt._plans[0]) == 2 and opt._plans[0][0] is plan and opt._plans[0][1].params == [ps[2]] and opt._kept == []
+    assert plan.steps.tolist() == [1, 4, 4, 4] and rec.steps[-2:] == [q.table.data_ptr() for q in opt._plans[0]]
+    assert [float(opt.state_dict()["state"][i]["step"]) for i in range(3)] == [1, 4, 0]
+    opt.refresh()                                                       # nothing was replaced: the captured table is taken up again
+    opt.step()
+    assert plan in opt._plans[0] and plan.steps.tolist() == [1, 4, 4, 4]
+    ps[1].data = ps[1].data.clone()                                     # elsewhere now: the captured launch has the old place
+    ps[1].grad = torch.zeros_like(ps[1])
+    opt.step()
+    assert not any(q is plan for q in opt._plans[0]) and any(q is plan for q in opt._kept)
+    assert sorted(id(p) for q in opt._plans[0] for p in q.params) == sorted(map(id, ps))
+
+
+def test_a_first_gradient_without_captured_tables_makes_one_table_of_all(monkeypatch):
+    opt, ps, rec, plan = _three(monkeypatch)
+    plan.steps += 3
+    ps[0].grad = None
+    ps[2].grad = torch.zeros_like(ps[2])
+    opt.step()
+    q, = opt._plans[0]
+    assert q.params == ps and q.steps.tolist() == [3, 3, 3, 3, 0] and opt._kept == []
+
+
+def test_parameters_that_share_memory_take_steps_in_turn(monkeypatch):
+    """As long as only one of them has a gradient."""
+    t = torch.ones(10)
+    a, b = torch.nn.Parameter(t[:6]), torch.nn.Parameter(t[4:])
+    opt = optim.AdamW([a, b])
+    rec = _Recorder(monkeypatch, opt)
+    for p, q in ((a, b), (b, a), (a, b)):
+        p.grad, q.grad = torch.zeros(6), None
+        opt.step()
+        assert [r.params for r in opt._plans[0]] == [[p]]
+    b.grad = torch.zeros(6)
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
