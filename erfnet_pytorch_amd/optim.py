@@ -128,11 +128,15 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def _write_back_steps(self):
+        """The device's counts into `state`, except where the count there was changed by hand (or the state taken away) since the last time."""
         for plans in self._plans or ():
             for plan in plans:
                 counts = plan.steps.cpu()
-                for p, first in zip(plan.params, plan.first_chunk):
-                    self.state[p]["step"] = counts[int(first)].float()
+                for i, (p, first) in enumerate(zip(plan.params, plan.first_chunk)):
+                    st = self.state.get(p, {})
+                    if "step" in st and float(st["step"]) == plan.counts[i]:
+                        st["step"] = counts[int(first)].float()
+                        plan.counts[i] = float(st["step"])
 
     def _drop_plans(self):
         """Forget the device tables: the next step builds them anew from `state` and the parameters."""
@@ -142,7 +146,8 @@ class AdamW(torch.optim.Optimizer):
         self._plans = None
 
     def refresh(self):
-        """To be called after entries of `state` were replaced by hand between two steps."""
+        """To be called after entries of `state` were replaced or removed by hand between two steps.  Counts too: state_dict() brings
+        those in `state` up to date, and a count that differs from what it wrote is taken over."""
         self._drop_plans()
 
     def state_dict(self):
@@ -235,6 +240,7 @@ class AdamW(torch.optim.Optimizer):
             if not torch.equal(rows, plan.rows):
                 continue
             plan.steps.copy_(torch.from_numpy(steps[plan.owner]))
+            plan.counts = self._counts(plan.params)
             plan.which, plan.stale = [mine[p][1] for p in plan.params], True
             plans.append(plan)
             for p in plan.params:
@@ -250,8 +256,13 @@ class AdamW(torch.optim.Optimizer):
             plan.table = plan.rows.to(device)
             plan.chunks = torch.from_numpy(where).to(device)
             plan.steps = torch.from_numpy(steps[plan.owner]).to(device)
+            plan.counts = self._counts(plan.params)
             plans.append(plan)
         return plans
+
+    def _counts(self, params):
+        """The counts as they stand in `state`."""
+        return [float(self.state[p]["step"]) for p in params]
 
     def _copy_places(self):
         """Gradients with other strides than their parameter's are copied into its order every step; where the copies lie."""

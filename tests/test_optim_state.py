@@ -16,6 +16,7 @@ def _with_plan(captured):
     opt.state[p].update(step=torch.zeros(()), exp_avg=torch.zeros(6), exp_avg_sq=torch.zeros(6))
     plan = optim._Plan(0, p.device, 0)
     plan.params, plan.first_chunk, plan.steps, plan.captured = [p], np.array([0]), torch.tensor([3], dtype=torch.int32), captured
+    plan.counts = [0.0]
     opt._plans = [[plan]]
     opt._lr = [[1e-2, {p.device: torch.full((1,), 1e-2, dtype=torch.float64)}]]
     opt._copies, opt._copies_captured = {0: (torch.zeros(6), p)}, captured
@@ -250,3 +251,35 @@ def test_parameters_that_share_memory_take_steps_in_turn(monkeypatch):
     b.grad = torch.zeros(6)
     with pytest.raises(ValueError, match="share memory"):
         opt.step()
+
+
+# ------------------------------------------------------------------------------------------------ state changed by hand
+def test_counts_changed_by_hand_are_taken_over(monkeypatch):
+    opt, ps, rec, plan = _three(monkeypatch)
+    plan.steps += 4
+    assert [float(opt.state_dict()["state"][i]["step"]) for i in (0, 1)] == [4, 4]
+    opt.state[ps[0]]["step"] = torch.tensor(10.0)
+    opt.refresh()
+    opt.step()
+    q, = opt._plans[0]
+    assert q.steps.tolist() == [10, 4, 4, 4]
+    opt.state[ps[1]]["step"] = opt.state[ps[1]]["step"].clone()         # moved about, not changed
+    q.steps += 1
+    assert [float(opt.state_dict()["state"][i]["step"]) for i in (0, 1)] == [11, 5]
+    opt.state[ps[1]]["step"].fill_(2.0)
+    opt.refresh()
+    assert [float(opt.state_dict()["state"][i]["step"]) for i in (0, 1)] == [11, 2]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_state_taken_away_starts_anew(monkeypatch, captured):
+    opt, ps, rec, plan = _three(monkeypatch)
+    plan.steps += 4
+    plan.captured = captured
+    del opt.state[ps[0]]
+    opt.state[ps[1]] = {}
+    opt.refresh()
+    opt.step()
+    q, = opt._plans[0]
+    assert q is not plan and q.steps.tolist() == [0, 0, 0, 0] and opt._kept == ([plan] if captured else [])
+    assert set(opt.state[ps[0]]) == {"step", "exp_avg", "exp_avg_sq"}
