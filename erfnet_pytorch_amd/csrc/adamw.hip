@@ -158,7 +158,8 @@ struct Lane4 {
     }
 };
 
-struct AdamwScalars { float step_size, decay, inv_bc2, b1, omb1, b2, omb2, eps; unsigned key; };
+// plain_div: eps is not in fast_div's range (sqrt(v) / sqrt(1 - b2^t) stays below 2^120)
+struct AdamwScalars { float step_size, decay, inv_bc2, b1, omb1, b2, omb2, eps; unsigned key; bool plain_div; };
 
 // sqrt(v), v >= 0, to half a step but for one case in a million: y = v / sqrt(v) from the hardware's reciprocal root, then
 // y + (v - y^2) / (2 sqrt(v)).  A v below the smallest normal number has no digits left and loses some more.
@@ -166,7 +167,8 @@ __device__ __forceinline__ float fast_sqrt(float v) {
     const float s = __builtin_amdgcn_rsqf(fmaxf(v, 1.17549435e-38f)), y = v * s;
     return fmaf(fmaf(-y, y, v), 0.5f * s, y);
 }
-// m / d, d finite and not 0, in the same way
+// m / d in the same way, for 2^-126 <= d <= 2^125: outside that 1 / d has no digits, or is infinite.  |m / d| is finite there: m came
+// from gradients of which sqrt(v), in d, has its share
 __device__ __forceinline__ float fast_div(float m, float d) {
     const float r = __builtin_amdgcn_rcpf(d), q = m * r;
     return fmaf(fmaf(-q, d, m), r, q);
@@ -205,7 +207,7 @@ __device__ __forceinline__ void adamw_update(Lane4<T, 8>& x, const AdamwScalars&
         br[e] = __float_as_uint(r[e]);
     }
     unsigned most_m = wave_umax(max(max(bm[0], bm[1]), max(bm[2], bm[3]))), most_r = wave_umax(max(max(br[0], br[1]), max(br[2], br[3])));
-    const bool odd = most_m >= 0x7F800000u || most_r >= 0x7F800000u || k.eps == 0.f;
+    const bool odd = most_m >= 0x7F800000u || most_r >= 0x7F800000u || k.plain_div;
     if (!odd) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) x.p[e] = x.p[e] * k.decay - fast_div(m[e], r[e] * k.inv_bc2 + k.eps) * k.step_size;
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwArgs a) {
     const double lr = *a.lr;
     const AdamwScalars k{(float)(lr / (1.0 - ipow(a.b1, step))), (float)(1.0 - lr * a.wd), (float)(1.0 / sqrt(1.0 - ipow(a.b2, step))),
                          (float)a.b1, (float)(1.0 - a.b1), (float)a.b2, (float)(1.0 - a.b2), (float)a.eps,
-                         ((unsigned)step * 0x9E3779B9u) ^ a.seed};
+                         ((unsigned)step * 0x9E3779B9u) ^ a.seed, !(a.eps >= 0x1p-126 && a.eps <= 0x1p100)};
     const unsigned counter = (unsigned)(t.base + start);
     if (whole) {
 #pragma unroll

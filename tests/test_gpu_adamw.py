@@ -633,3 +633,27 @@ def test_a_tensor_without_a_gradient_is_left_alone(bits):
         other.step()
     assert torch.equal(ps[0].detach(), qs[0].detach())
     assert [float(opt.state_dict()["state"][i]["step"]) for i in (0, 1)] == [3, 4]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-39, 2.0 ** -126, 1e-8, 1.0, 1e30, 1e38, 1e300])
+def test_every_size_of_eps(bits, eps):
+    """Elements whose moments are 0 (their update is 0 / eps) only decay; the others follow the formula with eps as the fp32 value that
+    the kernel has.  With eps = 0 an element without moments has no update: 0 / 0."""
+    gen = torch.Generator().manual_seed(61)
+    start = torch.randn(5000, generator=gen).cuda()
+    g = (1e-2 * torch.randn(5000, generator=gen)).cuda()
+    g[::3] = 0
+    p = torch.nn.Parameter(start.clone())
+    opt = _adamw([p], lr=LR, betas=BETAS, eps=eps, weight_decay=WD, state_bits=bits)
+    p.grad = g
+    opt.step()
+    zero = torch.zeros(5000, device="cuda")
+    rp, _, _, tp, _, _ = _reference(start, g, zero, zero, 1, eps=float(torch.tensor(eps, dtype=torch.float64).float()))
+    if eps == 0.0:
+        assert torch.equal(torch.isnan(p.detach()), g == 0)
+        rp, tp = rp[g != 0], tp[g != 0]
+        assert ((p.detach()[g != 0].double() - rp).abs() <= tp).all()
+        return
+    assert ((p.detach().double() - rp).abs() <= tp).all()
