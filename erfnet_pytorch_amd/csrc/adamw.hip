@@ -162,7 +162,7 @@ struct Lane4 {
 struct AdamwScalars { float step_size, decay, inv_bc2, b1, omb1, b2, omb2, eps; unsigned key; bool plain_div; };
 
 // sqrt(v), v >= 0, to half a step but for one case in a million: y = v / sqrt(v) from the hardware's reciprocal root, then
-// y + (v - y^2) / (2 sqrt(v)).  A v below the smallest normal number has no digits left and loses some more.
+// y + (v - y^2) / (2 sqrt(v)).  For 0 and normal v: the hardware's reciprocal root does not take subnormal ones.
 __device__ __forceinline__ float fast_sqrt(float v) {
     const float s = __builtin_amdgcn_rsqf(fmaxf(v, 1.17549435e-38f)), y = v * s;
     return fmaf(fmaf(-y, y, v), 0.5f * s, y);
@@ -188,7 +188,7 @@ __device__ __forceinline__ void adamw_update(Lane4<T, 32>& x, const AdamwScalars
 }
 
 // ... in 8 bits, of one wave's scale block; sm, sr: its scales, replaced by the new ones.  The arithmetic, not the memory, bounds
-// this kernel: what handles values that are not finite stands in a branch of its own that a wave takes when it has met one (bits
+// this kernel: what handles values that are not finite, or v that are subnormal, stands in a branch of its own that a wave takes when it has met one (bits
 // of NaN and infinity, as integers, are above all others, so the maximum finds them).
 template <typename T>
 __device__ __forceinline__ void adamw_update(Lane4<T, 8>& x, const AdamwScalars& k, unsigned counter, float& sm, float& sr) {
@@ -197,6 +197,7 @@ __device__ __forceinline__ void adamw_update(Lane4<T, 8>& x, const AdamwScalars&
     const f32x2 r0 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(x.cr, true);
     float m[4] = {m0[0], m0[1], m1[0], m1[1]}, r[4] = {r0[0], r0[1], r1[0], r1[1]}, v[4];
     unsigned bm[4], br[4];
+    bool subnormal = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float old = r[e] * sr;
@@ -205,9 +206,10 @@ __device__ __forceinline__ void adamw_update(Lane4<T, 8>& x, const AdamwScalars&
         r[e] = fast_sqrt(v[e]);
         bm[e] = __float_as_uint(m[e]) & 0x7FFFFFFFu;
         br[e] = __float_as_uint(r[e]);
+        subnormal |= __builtin_amdgcn_classf(v[e], 0x80);     // above 0
     }
     unsigned most_m = wave_umax(max(max(bm[0], bm[1]), max(bm[2], bm[3]))), most_r = wave_umax(max(max(br[0], br[1]), max(br[2], br[3])));
-    const bool odd = most_m >= 0x7F800000u || most_r >= 0x7F800000u || k.plain_div;
+    const bool odd = most_m >= 0x7F800000u || most_r >= 0x7F800000u || k.plain_div || __any(subnormal);
     if (!odd) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) x.p[e] = x.p[e] * k.decay - fast_div(m[e], r[e] * k.inv_bc2 + k.eps) * k.step_size;

@@ -657,3 +657,28 @@ def test_every_size_of_eps(bits, eps):
         assert ((p.detach()[g != 0].double() - rp).abs() <= tp).all()
         return
     assert ((p.detach().double() - rp).abs() <= tp).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-17, 2e-18, 1e-18, 1e-19, 1e-20])
+def test_8_bit_moments_of_tiny_gradients(size):
+    """v = (1 - b2) g^2 is subnormal below |g| of about 3e-18, a multiple of 2^-149: sqrt(v) is that of the v that fp32 holds, to a
+    half step (U), and its code is off by less than a step.  Gradients of ordinary size beside them, in another scale block, and
+    among them, where the tiny ones' codes are the smallest."""
+    p = torch.nn.Parameter(torch.zeros(768, device="cuda"))
+    opt = _adamw([p], lr=LR, betas=BETAS, eps=EPS, weight_decay=0.0, state_bits=8)
+    g = size * (1 + torch.arange(768, device="cuda") / 768)
+    g[256:512] = 0.5
+    g[600] = 0.25
+    p.grad = g
+    opt.step()
+    omb2 = torch.tensor(1 - BETAS[1], dtype=torch.float64).float().cuda()
+    v = g * g * omb2                                          # as the kernel rounds them
+    want = v.double().sqrt()
+    got = _decoded(opt, p, "exp_avg_sq_root")
+    each = opt.state[p]["exp_avg_sq_root_scale"].double().repeat_interleave(256)
+    assert ((got - want).abs() <= torch.maximum(want * 2.0 ** -3, each * 2.0 ** -9) * (1 + 1e-6) + U * want).all()
+    assert ((got > 0) == (v > 0)).all()
+    first = want[:256].max()
+    if float(first) > 0:
+        assert 224 * (1 - 1e-5) <= float(first / each[0]) <= 448 * (1 + 1e-5)
