@@ -753,6 +753,9 @@ __device__ __forceinline__ float lp_grad(float z, float base, float logs, float 
     return -__builtin_amdgcn_exp2f(lp * LOG2E) * fmaf(gh, fmaxf(lp, -200.f), pull);          // p = 0: 0 * -inf
 }
 
+// gl of a target that is not ignored: one outside [0, C) has log p = NaN, and so has its gradient unless nothing comes in
+__device__ __forceinline__ float target_grad(bool inside, float g) { return inside || g == 0.f ? g : __builtin_nanf(""); }
+
 // One thread per P positions, as in the forward pass (6 x 20 x 512 x 1024 fp32 with 2 alternatives 123 us, 5.3 TB/s).  The target's
 // term and those of up to KT alternatives are added on the way; where there are more (KT < 0), the classes that are alternatives are
 // written once more.
@@ -776,7 +779,7 @@ __global__ __launch_bounds__(256) void lp_position_bwd_kernel(const LpBwdArgs a)
             for (int p = 0; p < P; ++p) {
                 const long long v = a.target[i + p];
                 t[p] = v >= 0 && v < a.C ? (int)v : -1;
-                gl[p] = v == a.ignore ? 0.f : t[p] >= 0 ? gl[p] : __builtin_nanf("");
+                gl[p] = v == a.ignore ? 0.f : target_grad(t[p] >= 0, gl[p]);
             }
         }
         if (a.g_entropy) load_positions<float, P>(a.g_entropy + i, gh);
@@ -874,7 +877,7 @@ __global__ __launch_bounds__(256) void lp_rows_lds_bwd_kernel(const LpBwdArgs a)
         if (a.g_log_prob) {
             const long long v = a.target[i];
             t = v >= 0 && v < a.C ? (int)v : -1;
-            gl = v == a.ignore ? 0.f : t >= 0 ? a.g_log_prob[i] : __builtin_nanf("");
+            gl = v == a.ignore ? 0.f : target_grad(t >= 0, a.g_log_prob[i]);
         }
         if (a.g_entropy) gh = a.g_entropy[i];
         base = a.stats[i];
@@ -925,7 +928,7 @@ __global__ __launch_bounds__(256) void lp_rows_bwd_kernel(const LpBwdArgs a) {
     const int off = (int)(((unsigned long long)row / sizeof(T)) % E), dist = (int)(((unsigned long long)out / sizeof(T)) % E);
     const int chunks = (a.C + off + E - 1) / E, q0 = blockIdx.y * TEAM * BWD_UNROLL, q1 = min(q0 + TEAM * BWD_UNROLL, chunks);
     const long long t = a.g_log_prob ? a.target[i] : a.ignore;
-    const float gl = t == a.ignore ? 0.f : t >= 0 && t < a.C ? a.g_log_prob[i] : __builtin_nanf(""), gh = a.g_entropy ? a.g_entropy[i] : 0.f;
+    const float gl = t == a.ignore ? 0.f : target_grad(t >= 0 && t < a.C, a.g_log_prob[i]), gh = a.g_entropy ? a.g_entropy[i] : 0.f;
     float pull = gl;
     bool any = gl != 0.f || gh != 0.f;
     // alternative wl + r W is lane wl's of every wave (W lanes of it): its gradient, its class and that class's logit, all on their way

@@ -91,7 +91,7 @@ def class_log_probs(logits, target=None, top_k=0, ignore_index=-100):
       top_log_probs [N, k, ...]    the k <= 32 largest log probabilities in falling order, equal ones by index, NaN before all
       top_indices [N, k, ...]      their classes (int64); both None for top_k = 0
     Differentiable in the logits through log_prob, entropy and top_log_probs (once).  A position whose incoming gradients are all 0
-    gets the gradient 0 whatever its logits hold, so padding that is ignored cannot spread NaN.
+    gets the gradient 0 whatever its logits and target hold, so padding that is ignored or masked cannot spread NaN.
     A logit of -inf has probability 0 and takes no part.  A position without any finite logit, or with +inf or NaN among its
     logits, has no distribution: its log_prob (if not ignored), entropy and top_log_probs are NaN, as log_softmax's.
     """

@@ -258,7 +258,7 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
  *   follows); alternatives in falling order of their value, equal ones by index, NaN first.
  * bwd: dlogits (same type, own strides, same kind of layout) = gl ([j = t] - p) - gh p (log p + entropy) + sum_k gk ([j = i_k] - p);
  *   i_k outside [0, C) is no class: its gradient enters only as -p gk.
- *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits hold.  dlogits may
+ *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits and target hold.  dlogits may
  *   not alias logits.
  * Rows further apart than C: what lies between the first and the last of them may be read, and has no effect; it is not written. */
 #define ERF_TOP_MAX 32

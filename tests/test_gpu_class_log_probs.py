@@ -289,6 +289,29 @@ def test_targets_outside_the_classes_give_nan_and_another_ignore_index():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(5, 9), (5, 50), (5, 5000), (65600, 20), (1, 20, 1, 5), (2, 9, 640, 512)])
+@pytest.mark.parametrize("last", [False, True])
+def test_targets_outside_the_classes_without_a_gradient_give_none(shape, last):
+    """Such positions masked by the caller: exactly 0 in every plan, or what the other outputs' gradients give alone."""
+    from erfnet_pytorch_amd.loss import class_log_probs
+    z = _logits(shape, torch.float32, "channels_last" if last and len(shape) == 4 else "plain", 15).requires_grad_()
+    pos = (shape[0], *shape[2:])
+    t = torch.zeros(pos, dtype=torch.int64, device="cuda")
+    flat = t.view(-1)
+    flat[0], flat[1], flat[2], flat[-1] = -1, shape[1], 2 ** 40, -7
+    g = torch.ones(pos, device="cuda")
+    for i in (0, 2, -1):
+        g.view(-1)[i] = 0
+    h = torch.zeros(pos, device="cuda")
+    h.view(-1)[2] = 1.0
+    out = class_log_probs(z, t)
+    dz, = torch.autograd.grad([out.log_prob, out.entropy], z, [g, h])
+    dh, = torch.autograd.grad(class_log_probs(z).entropy, z, h)
+    dz, dh = (d.movedim(1, -1).reshape(-1, shape[1]) for d in (dz, dh))
+    assert (dz[0] == 0).all() and dz[1].isnan().all() and torch.equal(dz[2], dh[2]) and (dz[-1] == 0).all() and dz[3].isfinite().all()
+
+
+@pytest.mark.gpu
 def test_without_target_and_partial_gradients():
     from erfnet_pytorch_amd.loss import class_log_probs
     z = _logits((3, 30), torch.float32, "plain", 14).requires_grad_()
