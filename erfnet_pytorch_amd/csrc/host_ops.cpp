@@ -58,6 +58,11 @@ static void once_only(const char* who) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), who, " is differentiable once: backward with create_graph=True is not supported");
 }
 
+// ... and forward-mode differentiation would find no tangent on the outputs, which counts as a derivative of 0
+static void reverse_only(const Tensor& t, const char* who) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), who, " has no forward-mode derivative");
+}
+
 // ------------------------------------------------------------------------------------------------ group norm + activation
 static int64_t activation_code(const std::string& a) {
     const int64_t code = a == "none" ? ERF_ACT_NONE : a == "relu" ? ERF_ACT_RELU : a == "silu" ? ERF_ACT_SILU : -1;
@@ -194,6 +199,7 @@ static Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& w
     require_gpu(x, "group_norm_act");
     TORCH_CHECK_VALUE(x.dim() >= 2, "group_norm_act: x has shape [N, C, ...], got ", x.sizes());
     const int64_t act = activation_code(activation);
+    for (const Tensor& t : {x, weight.value_or(Tensor()), bias.value_or(Tensor())}) reverse_only(t, "group_norm_act");
     if (c10::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
         return GroupNormActFn::apply(x, weight, bias, groups, eps, act);
     return std::get<0>(group_norm_fwd(channels_last(x), weight, bias, groups, eps, act, true));
@@ -347,6 +353,7 @@ struct ClassLogProbsFn : public torch::autograd::Function<ClassLogProbsFn> {
 
 static std::tuple<Tensor, Tensor, Tensor, Tensor> class_log_probs(const Tensor& logits, const OptTensor& target, int64_t top_k, int64_t ignore_index) {
     require_gpu(logits, "class_log_probs");
+    reverse_only(logits, "class_log_probs");
     if (c10::GradMode::is_enabled() && logits.requires_grad()) {
         const variable_list r = ClassLogProbsFn::apply(logits, target, top_k, ignore_index);
         return {r[0], r[1], r[2], r[3]};

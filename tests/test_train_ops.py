@@ -94,6 +94,24 @@ def test_tensors_that_dispatch_to_python_are_refused():
             call()
 
 
+def test_forward_mode_differentiation_is_refused():
+    """No tangent on the outputs would count as a derivative of 0."""
+    import torch.autograd.forward_ad as fa
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from erfnet_pytorch_amd.loss import class_log_probs
+    from erfnet_pytorch_amd.norm import group_norm_act
+    with FakeTensorMode(), fa.dual_level():
+        x, w = torch.empty(2, 8, 4, 4, device="cuda"), torch.empty(8, device="cuda")
+        for leaf in (False, True):
+            dx, dw = (fa.make_dual(t.clone().requires_grad_(leaf), torch.empty_like(t)) for t in (x, w))
+            for call in (lambda: group_norm_act(dx, 2), lambda: group_norm_act(x, 2, dw, w), lambda: group_norm_act(x, 2, w, dw),
+                         lambda: class_log_probs(dx, top_k=1)):
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        call()
+        assert group_norm_act(x, 2, w).shape == x.shape and class_log_probs(x).entropy.shape == (2, 4, 4)
+
+
 @pytest.mark.gpu
 def test_outputs_may_be_written_in_place():
     """As torch's own: h = norm(x); h += residual."""
