@@ -51,6 +51,8 @@ static const OptTensor& on_device(const OptTensor& t, const Tensor& x, const cha
     return t;
 }
 
+// Views that torch negates when they are read (the imaginary part of a conjugate) hold the negative of their values: resolve_neg()
+// copies those, and gives every other tensor as it is.
 static void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // backward with create_graph=True would record nothing of what these passes do
@@ -71,7 +73,8 @@ static int64_t activation_code(const std::string& a) {
 }
 
 // Logical [N, C, ...] as a contiguous [N, ..., C]; zero-copy where the memory is channels-last
-static Tensor channels_last(const Tensor& x) {
+static Tensor channels_last(const Tensor& given) {
+    const Tensor x = given.resolve_neg();
     Tensor last = x.dim() > 2 ? x.movedim(1, -1) : x;
     if (last.is_contiguous()) return last;
     auto tiles = [](int64_t n) { return (n + 31) / 32; };
@@ -100,7 +103,7 @@ static Tensor empty_channels_last(at::IntArrayRef sizes, const at::TensorOptions
     return at::empty_strided(sizes, strides, options);
 }
 
-static Tensor fp32(const OptTensor& t) { return t ? t->to(at::kFloat).contiguous() : Tensor(); }
+static Tensor fp32(const OptTensor& t) { return t ? t->resolve_neg().to(at::kFloat).contiguous() : Tensor(); }
 
 struct GnShape { int code, n, c; int64_t hw; };
 static GnShape gn_check(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups) {
@@ -216,7 +219,8 @@ struct Layout {
     std::vector<int64_t> shape;        // [N, ...]
 };
 
-static Layout class_layout(const Tensor& logits) {
+static Layout class_layout(const Tensor& given) {
+    const Tensor logits = given.resolve_neg();
     TORCH_CHECK_VALUE(logits.dim() >= 2 && logits.size(1) >= 1, "class_log_probs: logits have shape [N, C, ...] with at least one class, got ", logits.sizes());
     Layout q;
     q.z = logits;
@@ -256,7 +260,7 @@ static Tensor check_target(const OptTensor& target, const Layout& q) {
     TORCH_CHECK_TYPE(target->scalar_type() == at::kLong, "class_log_probs: targets are int64 class indices, got ", target->dtype());
     TORCH_CHECK_VALUE(target->sizes() == at::IntArrayRef(q.shape), "class_log_probs: expected targets of shape ", at::IntArrayRef(q.shape), ", got ", target->sizes());
     on_device(target, q.z, "class_log_probs", "target");
-    return target->contiguous();
+    return target->resolve_neg().contiguous();
 }
 
 // Memory of [N, k, ...] that follows the logits: k last for rows
@@ -266,7 +270,10 @@ static Tensor like_layout(const Layout& q, int64_t k, at::ScalarType type) {
     return q.rows && s.size() > 2 ? empty_channels_last(s, q.z.options().dtype(type)) : at::empty(s, q.z.options().dtype(type));
 }
 // ... of a tensor [N, k, ...] given from outside
-static Tensor to_layout(const Tensor& t, const Layout& q) { return q.rows && t.dim() > 2 ? t.movedim(1, -1).contiguous() : t.contiguous(); }
+static Tensor to_layout(const Tensor& given, const Layout& q) {
+    const Tensor t = given.resolve_neg();
+    return q.rows && t.dim() > 2 ? t.movedim(1, -1).contiguous() : t.contiguous();
+}
 
 // (log_prob, entropy, stats [2, N, ...], top_log_probs, top_indices); stats undefined where no backward pass follows
 static std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> class_log_probs_fwd(const Tensor& logits, const OptTensor& target_, int64_t top_k, int64_t ignore_index,
@@ -396,7 +403,7 @@ struct ParamWatch {
 
     // 0: all as before; 1: the same parameters, gradients elsewhere, come or gone (noted); 2: other parameters, parameters elsewhere, or
     // a gradient of one that is in no table.
-    // A gradient whose strides are not its parameter's counts as elsewhere every time: it is copied into the parameter's order.
+    // A gradient whose strides are not its parameter's (or that holds its negative) counts as elsewhere every time: it is copied.
     // Nothing is noted before every gradient has been checked: after a refusal the next look finds the same changes.
     int look(const std::vector<py::list>& groups) {
         size_t i = 0;
@@ -417,9 +424,9 @@ struct ParamWatch {
                     continue;
                 }
                 const bool strided = g.layout() == at::kStrided;
-                if (strided && g.data_ptr() == e.grad && g.sizes() == p.sizes() && g.strides() == p.strides() && g.scalar_type() == e.type && !e.copied) continue;
+                if (strided && g.data_ptr() == e.grad && g.sizes() == p.sizes() && g.strides() == p.strides() && g.scalar_type() == e.type && !e.copied && !g.is_neg()) continue;
                 check_grad(p, g);
-                moves.push_back({i - 1, g.data_ptr(), g.strides() != p.strides() && !(g.is_contiguous() && p.is_contiguous())});
+                moves.push_back({i - 1, g.data_ptr(), g.is_neg() || (g.strides() != p.strides() && !(g.is_contiguous() && p.is_contiguous()))});
             }
         if (i != entries.size()) return 2;
         for (const Move& m : moves) {
@@ -541,11 +548,11 @@ static void adamw_no_overlap(const std::vector<Tensor>& params) {
 
 static std::tuple<Tensor, Tensor> group_norm_act_fwd(const Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps,
                                                      const std::string& activation) {
-    return group_norm_fwd(x, weight, bias, groups, eps, activation_code(activation), false);
+    return group_norm_fwd(x.resolve_neg(), weight, bias, groups, eps, activation_code(activation), false);
 }
 static std::tuple<Tensor, Tensor, Tensor> group_norm_act_bwd(const Tensor& dy, const Tensor& x, const OptTensor& weight, const OptTensor& bias, const Tensor& stats,
                                                              int64_t groups, const std::string& activation) {
-    return group_norm_bwd(dy, x, weight, bias, stats, groups, activation_code(activation));
+    return group_norm_bwd(dy.resolve_neg(), x.resolve_neg(), weight, bias, stats, groups, activation_code(activation));
 }
 static std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> class_log_probs_with_stats(const Tensor& logits, const OptTensor& target, int64_t top_k, int64_t ignore_index) {
     return class_log_probs_fwd(logits, target, top_k, ignore_index, true);

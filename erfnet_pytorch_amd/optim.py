@@ -100,6 +100,8 @@ class AdamW(torch.optim.Optimizer):
         for p in params:
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError(f"AdamW updates float32 or bfloat16 parameters, got {p.dtype}")
+            if p.is_neg():
+                raise ValueError("AdamW updates parameters in memory of their own, got a view that holds their negative")
             if not _dense(p):
                 raise ValueError(f"AdamW updates parameters whose memory has no gaps or overlaps, got shape {tuple(p.shape)} strides {p.stride()}")
 

@@ -94,6 +94,50 @@ def test_tensors_that_dispatch_to_python_are_refused():
             call()
 
 
+def _negated(t):
+    """t as a view whose memory holds -t."""
+    v = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_views_that_hold_their_negative_are_copied_or_refused():
+    from erfnet_pytorch_amd import optim
+    z = torch.randn(3, 5)
+    assert torch.equal(TO.class_layout(_negated(z))[0], z) and not TO.class_layout(_negated(z))[0].is_neg()
+    p = torch.nn.Parameter(torch.zeros(6))
+    w = optim._host.ParamWatch()
+    p.grad = torch.view_as_real(torch.complex(torch.zeros(6), torch.ones(6)))[:, 1].contiguous()
+    w.bind([[p]])
+    assert [w.look([[p]]) for _ in range(2)] == [1, 0] and w.copied() == []
+    p.grad = torch._neg_view(p.grad)                        # the same address
+    assert w.look([[p]]) == 1 and w.copied() == [0] and w.look([[p]]) == 1
+    with pytest.raises(ValueError, match="negative"):
+        optim.AdamW([torch.nn.Parameter(_negated(torch.ones(4)))])
+
+
+@pytest.mark.gpu
+def test_views_that_hold_their_negative_give_what_their_values_give():
+    from erfnet_pytorch_amd.loss import class_log_probs
+    from erfnet_pytorch_amd.norm import group_norm_act
+    from erfnet_pytorch_amd.optim import AdamW
+    x, dy, w, b = (torch.randn(*s, device="cuda") for s in ((2, 8, 6, 10), (2, 8, 6, 10), (8,), (8,)))
+    t = torch.randint(0, 8, (2, 6, 10), device="cuda")
+
+    def run(view):
+        xs, ws, bs = (view(v).detach().requires_grad_() for v in (x, w, b))
+        y = group_norm_act(xs, 2, ws, bs, activation="silu")
+        out = class_log_probs(xs, t, top_k=2)
+        g = torch.autograd.grad([y, out.log_prob, out.top_log_probs], [xs, ws, bs], [view(dy), view(dy[:, 0].clone()), view(dy[:, :2].clone())])
+        p = torch.nn.Parameter(b.clone())
+        p.grad = view(w)
+        AdamW([p]).step()
+        return [y, *out, *g, p, *TO.group_norm_act_fwd(view(x.movedim(1, -1).contiguous()), view(w), view(b), 2, 1e-5, "none")]
+    want = run(lambda v: v)
+    for view in (lambda v: torch._neg_view(-v), lambda v: torch._neg_view(-v.repeat_interleave(2, -1))[..., ::2]):
+        assert all(torch.equal(u, v) for u, v in zip(want, run(view)))
+
+
 def test_forward_mode_differentiation_is_refused():
     """No tangent on the outputs would count as a derivative of 0."""
     import torch.autograd.forward_ad as fa
