@@ -38,6 +38,15 @@ def _samples(dev, dtype=torch.bfloat16):
     }
 
 
+def _one_pixel(dev):
+    """The same for maps of one pixel."""
+    def t(*shape, dt=torch.float32):
+        return torch.empty(shape, dtype=dt, device=dev)
+    f, i, z = torch.float32, torch.int64, t(6, 20, 1, 1)
+    return {"class_log_probs_fwd": [((z, None, 3, -100), [((0,), f), ((6, 1, 1), f), ((2, 6, 1, 1), f), ((6, 3, 1, 1), f), ((6, 3, 1, 1), i)])],
+            "class_log_probs_bwd": [((z, t(6, 1, 1, dt=i), t(2, 6, 1, 1), t(6, 1, 1), t(6, 0, 1, 1, dt=i), t(6, 1, 1), None, None, -100), [((6, 20, 1, 1), f)])]}
+
+
 def _outs(res):
     return list(res) if isinstance(res, (tuple, list)) else [res]
 
@@ -69,6 +78,52 @@ def test_ops_trace_under_fake_tensor_mode():
     assert tuple(y.shape) == (4, 64, 128, 64) and y.device.type == "cuda" and tuple(stats.shape) == (2, 4, 8)
     assert tuple(top.shape) == (4, 3, 64, 128) and top.stride() == idx.stride() == (64 * 128 * 3, 1, 128 * 3, 3)
     assert dz.is_contiguous(memory_format=torch.channels_last)
+
+
+@pytest.mark.parametrize("name", sorted(_samples("meta")))
+def test_ops_trace_with_dynamic_shapes(name):
+    """Sizes as symbols: shapes, types and strides of the fixed sizes they stand for."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+    op = getattr(T, name)
+    samples = list(_samples("meta")[name])
+    if name.startswith("class_log_probs"):                  # one pixel a map: rows, whatever the strides
+        samples += [s for s in _one_pixel("meta")[name]]
+    for args, want in samples:
+        fixed = _outs(op(*args))
+        mode = FakeTensorMode(shape_env=ShapeEnv())
+
+        def symbols(t):
+            if not isinstance(t, torch.Tensor):
+                return t
+            return mode.from_tensor(t, symbolic_context=StatelessSymbolicContext(dynamic_sizes=[DimDynamic.DYNAMIC] * t.dim()))
+        args = [symbols(a) for a in args]
+        with mode:
+            got = _outs(op(*args))
+        assert any(isinstance(n, torch.SymInt) for o in got for n in o.shape)
+        assert [(tuple(int(n) for n in o.shape), o.dtype) for o in got] == want
+        for o, f in zip(got, fixed):
+            assert all(int(a) == b for a, b, n in zip(o.stride(), f.stride(), f.shape) if n > 1)
+
+
+def test_dynamic_shapes_that_do_not_fit_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+    mode = FakeTensorMode(shape_env=ShapeEnv())
+
+    def symbols(*shape, dtype=torch.float32):
+        t = torch.empty(shape, dtype=dtype, device="meta")
+        return mode.from_tensor(t, symbolic_context=StatelessSymbolicContext(dynamic_sizes=[DimDynamic.DYNAMIC] * t.dim()))
+    x, z = symbols(2, 8, 16, 24), symbols(4, 30, 5)
+    with mode:
+        for call in (lambda: T.group_norm_act_fwd(x, None, None, 5, 1e-5, "relu"), lambda: T.group_norm_act_fwd(x, None, None, 4, 1e-5, "gelu"),
+                     lambda: T.group_norm_act_fwd(x, symbols(25), None, 4, 1e-5, "relu"), lambda: T.group_norm_act_fwd(x.transpose(1, 2), None, None, 4, 1e-5, "relu"),
+                     lambda: T.group_norm_act_bwd(symbols(2, 8, 16, 12), x, None, None, symbols(2, 2, 4), 4, "relu"),
+                     lambda: T.class_log_probs_fwd(z, None, 31, -100), lambda: T.class_log_probs_fwd(z, symbols(4, 6, dtype=torch.int64), 0, -100)):
+            with pytest.raises(ValueError):
+                call()
+        with pytest.raises(TypeError):
+            T.class_log_probs_fwd(symbols(4, 30, dtype=torch.float16), None, 0, -100)
 
 
 def test_cpu_tensors_are_refused():
