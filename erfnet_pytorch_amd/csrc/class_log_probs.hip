@@ -1016,6 +1016,11 @@ static inline bool lp_shape_ok(int dtype, long long N, int C, long long L, long 
     return (sc == 1 && L == 1) || (sc >= L && sc >= 2);
 }
 
+// Whether no two elements of dlogits share a place: images one behind the other, or images side by side within a class
+static inline bool lp_apart(long long N, int C, long long L, long long dn, long long dc) {
+    return N == 1 || (__int128)dn >= (__int128)(C - 1) * dc + L || (dn >= L && (__int128)dc >= (__int128)(N - 1) * dn + L);
+}
+
 static inline unsigned lp_grid(long long total) {
     const long long g = (total + 255) / 256;
     return (unsigned)(g > 65536 ? 65536 : g);
@@ -1155,7 +1160,8 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
                             const float* g_log_prob, const float* g_entropy, int top_k, const long long* top_indices, const float* g_top,
                             void* dlogits, long long dstride_n, long long dstride_c, void* stream) {
     if (!logits || !stats || !entropy || !dlogits || (g_log_prob && !target) || !lp_shape_ok(dtype, N, C, L, stride_n, stride_c, top_k) ||
-        (g_top && (!top_indices || !top_k)) || dstride_n < 0 || (dstride_c == 1) != (stride_c == 1) || (dstride_c != 1 && dstride_c < L))
+        (g_top && (!top_indices || !top_k)) || dstride_n < 0 || (dstride_c == 1) != (stride_c == 1) || (dstride_c != 1 && dstride_c < L) ||
+        !lp_apart(N, C, L, dstride_n, dstride_c))
         return ERF_EINVAL;
     const LpBwdArgs a{logits, target, N, L, stride_n, stride_c, dstride_n, dstride_c, C, g_top ? top_k : 0, ignore_index, stats, entropy,
                       g_log_prob, g_entropy, g_top, top_indices, dlogits, 0};

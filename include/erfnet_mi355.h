@@ -259,7 +259,7 @@ int erf_group_norm_bwd(const void* x, const void* dy, void* dx, int dtype, int N
  * bwd: dlogits (same type, own strides, same kind of layout) = gl ([j = t] - p) - gh p (log p + entropy) + sum_k gk ([j = i_k] - p);
  *   i_k outside [0, C) is no class: its gradient enters only as -p gk.
  *   g_log_prob, g_entropy, g_top may each be NULL; a position whose gradients are all 0 gets 0 whatever its logits and target hold.  dlogits may
- *   not alias logits.
+ *   not alias logits, and its strides may not let two of its elements share a place (refused).
  * Rows further apart than C: what lies between the first and the last of them may be read, and has no effect; it is not written. */
 #define ERF_TOP_MAX 32
 /* workspace of fwd: erf_class_log_probs_workspace_bytes (0: none needed, NULL is fine), 16-byte aligned, not shared by calls that may

@@ -533,6 +533,23 @@ def test_abi_refuses_bad_arguments_without_a_gpu():
         assert _lib.query("erf_class_log_probs_bwd", *args) == -1, i
 
 
+def test_abi_refuses_gradients_that_share_memory_without_a_gpu():
+    """Rows closer than C, planes or images on top of each other: two threads would write one place.  (Accepted strides reach a launch,
+    which there is no device for here: another status.)"""
+    from erfnet_pytorch_amd import _lib
+    if torch.cuda.is_available():
+        pytest.skip("the accepted calls have no memory behind them")
+
+    def status(n, c, length, dn, dc):
+        rows = dc == 1
+        return _lib.query("erf_class_log_probs_bwd", 16, 0, n, c, length, c * length, 1 if rows else max(length, 2), 16, -100, 16, 16, 16, 0, 0, 0, 0, 16, dn, dc, 0)
+    for bad in ((2, 5, 1, 0, 1), (2, 5, 1, 4, 1), (2, 5, 6, 29, 6), (2, 5, 6, 0, 6), (2, 5, 6, 5, 100), (3, 5, 6, 6, 17), (2, 1, 6, 5, 6),
+                (2, 2 ** 28, 6, 2 ** 62, 2 ** 62)):
+        assert status(*bad) == -1, bad
+    for good in ((1, 5, 1, 0, 1), (2, 5, 1, 5, 1), (2, 5, 1, 9, 1), (2, 5, 6, 30, 6), (1, 5, 6, 0, 6), (3, 5, 6, 6, 18), (2, 1, 6, 6, 6), (2, 2 ** 28, 6, 2 ** 61, 2 ** 62)):
+        assert status(*good) == -3, good
+
+
 def test_layouts_are_recognised():
     from erfnet_pytorch_amd.train_ops import class_layout as whole
 
