@@ -17,9 +17,14 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import ops, train_ops
+from . import ops
 from ._lib import call, query
 from .dp import global_weighted_mean
+
+try:
+    from . import train_ops
+except ImportError as e:                  # the cross entropy needs the library alone
+    train_ops, _lacking = None, e
 
 
 def _stream():
@@ -95,5 +100,7 @@ def class_log_probs(logits, target=None, top_k=0, ignore_index=-100):
     A logit of -inf has probability 0 and takes no part.  A position without any finite logit, or with +inf or NaN among its
     logits, has no distribution: its log_prob (if not ignored), entropy and top_log_probs are NaN, as log_softmax's.
     """
+    if train_ops is None:
+        raise _lacking
     log_prob, entropy, top, index = train_ops._host.class_log_probs(logits, target, top_k, ignore_index)
     return ClassLogProbs(None if target is None else log_prob, entropy, top if top_k else None, index if top_k else None)
