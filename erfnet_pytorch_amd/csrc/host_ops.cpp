@@ -375,7 +375,8 @@ static std::tuple<Tensor, Tensor, Tensor, Tensor> class_log_probs(const Tensor& 
 struct ParamWatch {
     struct Entry {
         const void *param, *grad;
-        bool on, has, copied;                   // in a table; with a gradient, which is copied
+        bool on, copied;                        // in a table; its gradient is copied
+        size_t place;                           // among those in tables
         at::ScalarType type;
         at::DimVector shape;                    // sizes, then strides
     };
@@ -383,6 +384,7 @@ struct ParamWatch {
     std::vector<Entry> entries;
     std::vector<Move> moves;                    // of the present look
     std::vector<Tensor> params;                 // those in tables, in the order of the groups
+    std::vector<char> given;                    // which of them have a gradient
 
     static const Tensor& tensor(PyObject* o) {
         TORCH_CHECK_TYPE(THPVariable_Check(o), "AdamW: parameters are tensors");
@@ -420,7 +422,7 @@ struct ParamWatch {
                 }
                 if (p.data_ptr() != e.param || p.scalar_type() != e.type || !same_shape(p, e)) return 2;
                 if (!g.defined()) {
-                    if (e.has) moves.push_back({i - 1, nullptr, false});
+                    if (given[e.place]) moves.push_back({i - 1, nullptr, false});
                     continue;
                 }
                 const bool strided = g.layout() == at::kStrided;
@@ -431,7 +433,7 @@ struct ParamWatch {
         if (i != entries.size()) return 2;
         for (const Move& m : moves) {
             entries[m.at].grad = m.grad;
-            entries[m.at].has = m.grad != nullptr;
+            given[entries[m.at].place] = m.grad != nullptr;
             entries[m.at].copied = m.copied;
         }
         return moves.empty() ? 0 : 1;
@@ -442,6 +444,7 @@ struct ParamWatch {
     void bind(const std::vector<py::list>& groups, const std::vector<int64_t>& more) {
         entries.clear();
         params.clear();
+        given.clear();
         auto next = more.begin();
         for (const py::list& group : groups)
             for (py::handle h : group) {
@@ -450,9 +453,12 @@ struct ParamWatch {
                 if (named) ++next;
                 const bool on = (p.grad().defined() || named) && p.numel();
                 if (on && p.grad().defined()) check_grad(p, p.grad());
-                entries.push_back({on ? p.data_ptr() : nullptr, nullptr, on, on && p.grad().defined(), false, p.scalar_type(), at::DimVector(p.sizes())});
+                entries.push_back({on ? p.data_ptr() : nullptr, nullptr, on, false, params.size(), p.scalar_type(), at::DimVector(p.sizes())});
                 entries.back().shape.append(p.strides().begin(), p.strides().end());
-                if (on) params.push_back(p);
+                if (on) {
+                    params.push_back(p);
+                    given.push_back(p.grad().defined());
+                }
             }
     }
 
@@ -465,13 +471,7 @@ struct ParamWatch {
         check_status(erf_adamw_set_grads((erf_adamw_tensor*)table, at.data(), (int)at.size(), (void*)stream), "erf_adamw_set_grads");
     }
 
-    // Which of them have a gradient
-    std::vector<bool> present() const {
-        std::vector<bool> r;
-        for (const Entry& e : entries)
-            if (e.on) r.push_back(e.has);
-        return r;
-    }
+    std::vector<bool> present() const { return {given.begin(), given.end()}; }
 
     // Places of the gradients that need a copy in their parameter's order
     std::vector<int> copied() const {
@@ -487,12 +487,8 @@ struct ParamWatch {
 
     // The parameters with a gradient changed through their addresses
     void bump() {
-        size_t i = 0;
-        for (const Entry& e : entries)
-            if (e.on) {
-                if (e.has) params[i].unsafeGetTensorImpl()->bump_version();
-                ++i;
-            }
+        for (size_t i = 0; i < params.size(); ++i)
+            if (given[i]) params[i].unsafeGetTensorImpl()->bump_version();
     }
 };
 

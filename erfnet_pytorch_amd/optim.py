@@ -39,7 +39,6 @@ class _Plan:
     def __init__(self, group, device, code):
         self.group, self.device, self.code = group, device, code
         self.params, self.bases, self.which = [], [], []        # which: places among all parameters in tables
-        self.live = True                                # one of them has a gradient
         self.captured = False                           # a captured launch may write the grad fields at any time
         self.stale = True                               # the table lacks the gradients' present addresses
 
@@ -54,6 +53,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _reset(self):
         self._plans = None                              # [[_Plan, ...] per group], None: to be built
+        self._active = []                               # those with a gradient in them
         self._lr = []                                   # per group: [value on the devices, {device: double tensor}]
         self._kept = []                                 # what captured launches still read
         self._copies, self._copies_captured = {}, False
@@ -329,12 +329,13 @@ class AdamW(torch.optim.Optimizer):
             present = self._watch.present()
             for plans in self._plans:
                 for plan in plans:
-                    plan.stale, plan.live = True, any(present[i] for i in plan.which)
+                    plan.stale = True
+            self._active = [plan for plans in self._plans for plan in plans if any(present[i] for i in plan.which)]
         if self._moved:
             with torch.no_grad():
                 self._copy_places()
             self._moved = False
-        if not any(plan.live for plans in self._plans for plan in plans):
+        if not self._active:
             return loss
         capturing = torch.cuda.is_current_stream_capturing()
         if self._copies:
@@ -343,15 +344,14 @@ class AdamW(torch.optim.Optimizer):
                 for own, p in self._copies.values():
                     own.copy_(p.grad)
         self.refresh_lr()
-        for numbers, where, plans in zip(settings, self._lr, self._plans):
-            for plan in plans:
-                if not plan.live:
-                    continue
-                if plan.device.index == torch._C._cuda_getDevice():
-                    self._launch(numbers, where[1][plan.device], plan, capturing)
-                else:
-                    with torch.cuda.device(plan.device):
-                        self._launch(numbers, where[1][plan.device], plan, capturing)
+        here = torch._C._cuda_getDevice()
+        for plan in self._active:
+            numbers, lr = settings[plan.group], self._lr[plan.group][1][plan.device]
+            if plan.device.index == here:
+                self._launch(numbers, lr, plan, capturing)
+            else:
+                with torch.cuda.device(plan.device):
+                    self._launch(numbers, lr, plan, capturing)
         self._watch.bump()
         ops.bump_param_epoch()                          # the parameters changed through raw pointers
         return loss
