@@ -385,6 +385,7 @@ struct ParamWatch {
     std::vector<Move> moves;                    // of the present look
     std::vector<Tensor> params;                 // those in tables, in the order of the groups
     std::vector<char> given;                    // which of them have a gradient
+    bool changed = false;                       // whether the last look found that one came or went
 
     static const Tensor& tensor(PyObject* o) {
         TORCH_CHECK_TYPE(THPVariable_Check(o), "AdamW: parameters are tensors");
@@ -431,10 +432,13 @@ struct ParamWatch {
                 moves.push_back({i - 1, g.data_ptr(), g.is_neg() || (g.strides() != p.strides() && !(g.is_contiguous() && p.is_contiguous()))});
             }
         if (i != entries.size()) return 2;
+        changed = false;
         for (const Move& m : moves) {
-            entries[m.at].grad = m.grad;
-            given[entries[m.at].place] = m.grad != nullptr;
-            entries[m.at].copied = m.copied;
+            Entry& e = entries[m.at];
+            e.grad = m.grad;
+            e.copied = m.copied;
+            changed = changed || given[e.place] != (m.grad != nullptr);
+            given[e.place] = m.grad != nullptr;
         }
         return moves.empty() ? 0 : 1;
     }
@@ -576,6 +580,7 @@ PYBIND11_MODULE(_host, m) {
         .def(py::init<>())
         .def("look", wrap_pybind_function(&ParamWatch::look))
         .def("bind", wrap_pybind_function(&ParamWatch::bind), py::arg("groups"), py::arg("more") = std::vector<int64_t>())
+        .def_readonly("changed", &ParamWatch::changed)
         .def("present", wrap_pybind_function(&ParamWatch::present))
         .def("set_grads", wrap_pybind_function(&ParamWatch::set_grads))
         .def("copied", wrap_pybind_function(&ParamWatch::copied))

@@ -271,11 +271,12 @@ class AdamW(torch.optim.Optimizer):
         if self._copies_captured:
             self._kept.append(self._copies)
         self._copies_captured = False
-        params = [p for _, p in sorted((i, p) for ps in self._plans for plan in ps for i, p in zip(plan.which, plan.params))] if self._watch.copied() else []
-        self._copies = {i: (torch.empty_like(params[i]).detach(), params[i]) for i in self._watch.copied()}
+        copied = self._watch.copied()
+        params = [p for _, p in sorted((i, p) for ps in self._plans for plan in ps for i, p in zip(plan.which, plan.params))] if copied else []
+        self._copies = {i: (torch.empty_like(params[i]).detach(), params[i]) for i in copied}
         for ps in self._plans:
             for plan in ps:
-                plan.copies = [self._copies[i][0].data_ptr() if i in self._copies else 0 for i in plan.which]
+                plan.copies = [self._copies[i][0].data_ptr() if i in self._copies else 0 for i in plan.which] if copied else [0] * len(plan.which)
 
     def refresh_lr(self):
         """Bring the learning rates to the device.  step() does so by itself; a program that replays a captured step calls this
@@ -326,11 +327,12 @@ class AdamW(torch.optim.Optimizer):
                 raise
         if seen:
             self._moved = True                          # until the copies have their places, and each table its addresses
-            present = self._watch.present()
             for plans in self._plans:
                 for plan in plans:
                     plan.stale = True
-            self._active = [plan for plans in self._plans for plan in plans if any(present[i] for i in plan.which)]
+            if seen == 2 or self._watch.changed:
+                present = self._watch.present()
+                self._active = [plan for plans in self._plans for plan in plans if any(present[i] for i in plan.which)]
         if self._moved:
             with torch.no_grad():
                 self._copy_places()
