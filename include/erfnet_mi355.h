@@ -284,7 +284,8 @@ int erf_class_log_probs_bwd(const void* logits, int dtype, long long N, int C, l
  * steps: device int per chunk, the steps taken so far; each launch adds 1.  lr: device double.
  * A tensor whose grad is NULL takes no step: its values, moments and counts stay as they are.
  * Tensors of one launch must not overlap.
- * erf_adamw_set_grads writes the grad fields of records 0..count-1; grads: HOST array, read before the call returns. */
+ * erf_adamw_set_grads writes the grad fields of records 0..count-1; grads: HOST array (NULL for no gradient), read before the call
+ * returns. */
 typedef struct {
     void* param;
     const void* grad;
