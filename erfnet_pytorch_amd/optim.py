@@ -323,7 +323,7 @@ class AdamW(torch.optim.Optimizer):
             try:
                 self._watch.look(groups)
             except BaseException:
-                self._plans = None
+                self._drop_plans()
                 raise
         if seen:
             self._moved = True                          # until the copies have their places, and each table its addresses

@@ -283,3 +283,20 @@ def test_state_taken_away_starts_anew(monkeypatch, captured):
     q, = opt._plans[0]
     assert q is not plan and q.steps.tolist() == [0, 0, 0, 0] and opt._kept == ([plan] if captured else [])
     assert set(opt.state[ps[0]]) == {"step", "exp_avg", "exp_avg_sq"}
+
+
+def test_an_error_between_tables_and_gradients_keeps_captured_tables(monkeypatch):
+    opt, ps, rec, plan = _three(monkeypatch)
+    plan.captured = True
+    opt.refresh()
+    looks = opt._watch.w.look
+
+    def look(groups):
+        opt._watch.look = looks
+        raise KeyboardInterrupt
+    opt._watch.look = look
+    with pytest.raises(KeyboardInterrupt):
+        opt.step()
+    assert opt._plans is None and any(k is plan for k in opt._kept)
+    opt.step()
+    assert opt._plans == [[plan]] and opt._kept == []
