@@ -32,13 +32,16 @@ from ._lib import BF16, F32, call, size_query
 from .train_ops import _host
 
 
+_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+
+
 class _Plan:
     """The device tables of one launch: parameters of one group, device and type.  A parameter comes in with its first gradient and
     stays; where it has none its address is NULL and the launch leaves it alone, so its step count is in one place for all launches."""
 
     def __init__(self, group, device, code):
         self.group, self.device, self.code = group, device, code
-        self.params, self.bases, self.which = [], [], []        # which: places among all parameters in tables
+        self.params, self.which = [], []                # which: places among all parameters in tables
         self.captured = False                           # a captured launch may write the grad fields at any time
         self.stale = True                               # the table lacks the gradients' present addresses
 
@@ -196,27 +199,29 @@ class AdamW(torch.optim.Optimizer):
         known = {id(p): (p.device, plan.code) for plan in known for p in plan.params}
         self._drop_plans()
 
-        def held(p):                                    # with a gradient, or as it was in a table before
-            return p.numel() and (p.grad is not None or (known.get(id(p)) == (p.device, _code(p)) and _dense(p)))
+        def again(p):                                   # without a gradient now, but as it was in a table before
+            return p.grad is None and known.get(id(p)) == (p.device, _CODES.get(p.dtype)) and p.numel() and _dense(p)
         _host.adamw_no_overlap(live)
+        more = {id(p): p for g in groups for p in g if again(p)} if known else {}
         try:
-            _host.adamw_no_overlap([p for g in groups for p in g if held(p)])
-        except ValueError:                              # with one that has no gradient now
-            known = {}
+            _host.adamw_no_overlap(live + list(more.values()) if more else [])
+        except ValueError:                              # with one that has a gradient
+            more = {}
+        held = more.keys() | {id(p) for p in live}
         block = size_query("erf_adamw_scale_block")
-        plans, more, base, place, at = [], [], 0, 0, 0
+        plans, base, place, at, places = [], 0, 0, 0, []
         for number, group in enumerate(groups):
-            rows = {}                                   # per device and type: parameter -> (random base, place)
+            rows = {}                                   # per device and type: id -> (parameter, random base, place)
             for p in group:
-                if held(p):
-                    if p.grad is None:
-                        more.append(at)
-                    rows.setdefault((p.device, _code(p)), {})[p] = (base, place)
+                if id(p) in held:
+                    if id(p) in more:
+                        places.append(at)
+                    rows.setdefault((p.device, _CODES[p.dtype]), {})[id(p)] = (p, base, place)
                     place += 1
                 base += -(-p.numel() // block) * block
                 at += 1
             plans.append([plan for key, mine in rows.items() for plan in self._tables(number, *key, mine)])
-        self._watch.bind(groups, more)
+        self._watch.bind(groups, places)
         self._plans = plans
         self._kept = [k for k in self._kept if not any(k is plan for ps in plans for plan in ps)]
 
@@ -226,31 +231,32 @@ class AdamW(torch.optim.Optimizer):
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
         chunk = size_query("erf_adamw_chunk_elements")
 
-        def describe(params):
-            states = [self._state_of(p) for p in params]
+        def describe(of):                               # [(parameter, random base, place)]
+            states = [self._state_of(p) for p, _, _ in of]
             try:
-                states, steps = [[st[k] for k in names] for st in states], np.array([int(st["step"]) for st in states], dtype=np.int32)
+                states, counts = [[st[k] for k in names] for st in states], [float(st["step"]) for st in states]
             except KeyError as e:
                 raise ValueError(f"AdamW: a parameter's state lacks {e} (state_bits={self.state_bits})") from None
-            rows, holds = _host.adamw_table(params, states, [mine[p][0] for p in params])
-            return rows, holds, steps
+            rows, holds = _host.adamw_table([p for p, _, _ in of], states, [base for _, base, _ in of])
+            return rows, holds, counts, np.array(counts).astype(np.int32)
         plans, rest = [], dict(mine)
         for plan in reversed([k for k in self._kept if isinstance(k, _Plan)]):
-            if (plan.group, plan.device, plan.code) != (number, device, code) or any(p not in rest for p in plan.params):
+            if (plan.group, plan.device, plan.code) != (number, device, code) or any(id(p) not in rest for p in plan.params):
                 continue
-            rows, _, steps = describe(plan.params)
+            of = [rest[id(p)] for p in plan.params]
+            rows, _, counts, steps = describe(of)
             if not torch.equal(rows, plan.rows):
                 continue
             plan.steps.copy_(torch.from_numpy(steps[plan.owner]))
-            plan.counts = self._counts(plan.params)
-            plan.which, plan.stale = [mine[p][1] for p in plan.params], True
+            plan.counts = counts                        # as they stand in `state`
+            plan.which, plan.stale = [place for _, _, place in of], True
             plans.append(plan)
             for p in plan.params:
-                del rest[p]
+                del rest[id(p)]
         if rest:
             plan = _Plan(number, device, code)
-            plan.params, plan.bases, plan.which = list(rest), [b for b, _ in rest.values()], [w for _, w in rest.values()]
-            plan.rows, plan.holds, steps = describe(plan.params)
+            plan.params, plan.which = [p for p, _, _ in rest.values()], [place for _, _, place in rest.values()]
+            plan.rows, plan.holds, plan.counts, steps = describe(list(rest.values()))
             per = -(-plan.rows[:, 6].numpy() // chunk)  # chunks of each tensor
             plan.first_chunk = np.cumsum(per) - per
             plan.owner = np.repeat(np.arange(len(per)), per)
@@ -258,13 +264,8 @@ class AdamW(torch.optim.Optimizer):
             plan.table = plan.rows.to(device)
             plan.chunks = torch.from_numpy(where).to(device)
             plan.steps = torch.from_numpy(steps[plan.owner]).to(device)
-            plan.counts = self._counts(plan.params)
             plans.append(plan)
         return plans
-
-    def _counts(self, params):
-        """The counts as they stand in `state`."""
-        return [float(self.state[p]["step"]) for p in params]
 
     def _copy_places(self):
         """Gradients with other strides than their parameter's are copied into its order every step; where the copies lie."""
@@ -380,10 +381,6 @@ class AdamW(torch.optim.Optimizer):
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
-
-
-def _code(t):
-    return {torch.float32: F32, torch.bfloat16: BF16}.get(t.dtype)
 
 
 def _dense(t):
