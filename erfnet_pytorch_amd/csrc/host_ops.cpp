@@ -371,8 +371,8 @@ static std::tuple<Tensor, Tensor, Tensor, Tensor> class_log_probs(const Tensor& 
 }
 
 // ------------------------------------------------------------------------------------------------ AdamW's parameters
-// What the device tables of an optimizer describe: which parameters they hold, which of these have a gradient, and where both lie.  look() compares that with
-// the present; it keeps no gradient alive.
+// What the device tables of an optimizer describe: which parameters they hold, which of these have a gradient, and where both lie.
+// look() compares that with the present; it keeps no gradient alive.
 struct ParamWatch {
     struct Entry {
         const void *param, *grad;

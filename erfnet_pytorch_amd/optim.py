@@ -222,7 +222,7 @@ class AdamW(torch.optim.Optimizer):
                 at += 1
             plans.append([plan for key, mine in rows.items() for plan in self._tables(number, *key, mine)])
         self._watch.bind(groups, places)
-        self._plans = plans
+        self._plans, self._active = plans, None
         self._kept = [k for k in self._kept if not any(k is plan for ps in plans for plan in ps)]
 
     def _tables(self, number, device, code, mine):
@@ -331,7 +331,7 @@ class AdamW(torch.optim.Optimizer):
             for plans in self._plans:
                 for plan in plans:
                     plan.stale = True
-            if seen == 2 or self._watch.changed:
+            if self._active is None or self._watch.changed:
                 present = self._watch.present()
                 self._active = [plan for plans in self._plans for plan in plans if any(present[i] for i in plan.which)]
         if self._moved:
